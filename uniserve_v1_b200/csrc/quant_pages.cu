@@ -1,0 +1,227 @@
+// Cache pages of 8- and 4-bit integers: rows quantised as they are written, and read back as bf16.
+//
+// 64 channels of one token and head form a group with the scale  s = bf16(max|x| / m),  m = 127 or 7,
+// and the codes  c = round(x * (1 / s)) in [-m, m]  (products and the reciprocal in FP32, halves to even);
+// a value is read back as bf16(c * s).  The scale is rounded before it is used, so its rounding costs
+// nothing: only the grid moves by it.  bf16 rather than FP32 scales keep a 4-bit row of 128 channels at
+// 68 bytes instead of 72; bf16 rather than FP16 so that every finite input has one.  A group whose largest
+// magnitude is under m 2^-100 is stored as zeros (its reciprocal would overflow), a group that holds an
+// infinity or a NaN gets a NaN scale and reads back as NaN.
+//
+// Both are bound by memory.  Writing: a thread has 8 channels of K and of V (two 16-byte loads in flight),
+// eight threads a group.  Reading: a block has 16 rows, their places in the pages are looked up once, and a
+// thread expands 16 channels at a time (16- or 8-byte load, two 16-byte stores).
+#include "include/us_common.cuh"
+
+namespace {
+
+struct WriteArgs {
+  const __nv_bfloat16 *k, *v;
+  const void* slots;           // int32 or int64 [rows]; negative: the row is not written
+  uint8_t *kc, *vc;            // [pages, page, heads, dim * bits / 8]
+  __nv_bfloat16 *ks, *vs;      // [pages, heads, page, dim / 64]
+  long long ldk, hsk, ldv, hsv;   // elements between rows and between heads
+  long long capacity;          // pages * page
+  int rows, page, heads, dim, wide;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ float small_int(uint32_t u, float offset) {   // u in [0, 2^22)
+  return __uint_as_float(0x4B000000u | u) - (8388608.f + offset);
+}
+
+template <int BITS>
+__device__ __forceinline__ void quantise8(const uint4& raw, uint32_t (&code)[2], __nv_bfloat16& scale) {
+  constexpr float kMost = BITS == 8 ? 127.f : 7.f;
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t top = 0;            // magnitudes as 15-bit integers: NaN above infinity above every number
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+  top = max(top & 0xffffu, top >> 16);
+  const float most = __uint_as_float(top << 16);
+  float inv = 0.f;
+  scale = us::f2bf(0.f);
+  if (top >= 0x7f80u) {
+    scale = __ushort_as_bfloat16(0x7fffu);
+  } else if (most >= kMost * 0x1p-100f) {
+    scale = us::f2bf(__fdiv_rn(most, kMost));
+    inv = __frcp_rn(us::bf2f(scale));
+  }
+  // 1.5 * 2^23 + c: the rounded integer in the low mantissa bits (halves to even, as the sum is rounded).
+  // The product is rounded before the sum, as in the definition: no fused multiply-add.
+  uint32_t t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = top >= 0x7f80u ? 0.f : __uint_as_float(i & 1 ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
+    const float y = fminf(fmaxf(__fmul_rn(x, inv), -kMost), kMost);
+    t[i] = __float_as_uint(__fadd_rn(y, 12582912.f + (BITS == 4 ? 8.f : 0.f)));
+  }
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      code[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
+  } else {
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c |= (t[i] & 15u) << (4 * i);
+    code[0] = c;
+    code[1] = 0;
+  }
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(256) quant_write_kernel(const WriteArgs a) {
+  US_PDL_PROLOGUE();
+  const int per_head = a.dim >> 3, per_row = a.heads * per_head;
+  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
+  // the last block's idle threads repeat the last row's work up to the store: a group's eight threads stay
+  // together in the shuffles
+  const long long total = (long long)a.rows * per_row;
+  const long long at = idx < total ? idx : total - 8 + (idx & 7);
+  const int row = (int)(at / per_row), rest = (int)(at - (long long)row * per_row);
+  const int head = rest / per_head, ch = (rest - head * per_head) * 8;
+  const uint4 rk = *reinterpret_cast<const uint4*>(a.k + row * a.ldk + head * a.hsk + ch);
+  const uint4 rv = *reinterpret_cast<const uint4*>(a.v + row * a.ldv + head * a.hsv + ch);
+  const long long slot = a.wide ? ((const long long*)a.slots)[row] : (long long)((const int*)a.slots)[row];
+  uint32_t ck[2], cv[2];
+  __nv_bfloat16 sk, sv;
+  quantise8<BITS>(rk, ck, sk);
+  quantise8<BITS>(rv, cv, sv);
+  if (idx >= total || slot < 0) return;
+  if (slot >= a.capacity) {
+    us_dev_fail(a.status, US_DEV_BOUNDS);
+    return;
+  }
+  const long long byte = (slot * a.heads + head) * (a.dim * BITS / 8) + ch * BITS / 8;
+  if constexpr (BITS == 8) {
+    *reinterpret_cast<uint2*>(a.kc + byte) = make_uint2(ck[0], ck[1]);
+    *reinterpret_cast<uint2*>(a.vc + byte) = make_uint2(cv[0], cv[1]);
+  } else {
+    *reinterpret_cast<uint32_t*>(a.kc + byte) = ck[0];
+    *reinterpret_cast<uint32_t*>(a.vc + byte) = cv[0];
+  }
+  if ((ch & 63) == 0) {
+    const long long p = slot / a.page;
+    const long long s = ((p * a.heads + head) * a.page + (slot - p * a.page)) * (a.dim >> 6) + (ch >> 6);
+    a.ks[s] = sk;
+    a.vs[s] = sv;
+  }
+}
+
+struct ReadArgs {
+  const uint8_t *kc, *vc;
+  const __nv_bfloat16 *ks, *vs;
+  const int *table, *cu, *out_cu;
+  __nv_bfloat16 *ko, *vo;
+  long long ldo;
+  int B, max_pages, pages, page, heads, dim, total;
+  unsigned int* status;
+};
+
+constexpr int kReadRows = 16;
+
+template <int BITS>
+__global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
+  US_PDL_PROLOGUE();
+  __shared__ long long src[kReadRows], dst[kReadRows];   // slot (-1: nothing to read), row of the output
+  const int r0 = blockIdx.x * kReadRows;
+  if (threadIdx.x < kReadRows) {
+    const int r = r0 + threadIdx.x;
+    long long s = -1, d = 0;
+    if (r < min(a.total, a.cu[a.B])) {
+      int lo = 0, hi = a.B - 1;                 // sequence of packed row r
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.cu[mid] <= r) lo = mid; else hi = mid - 1;
+      }
+      const int pos = r - a.cu[lo], pi = pos / a.page;
+      const int pg = pi < a.max_pages ? a.table[(long long)lo * a.max_pages + pi] : -1;
+      d = (a.out_cu ? a.out_cu[lo] : a.cu[lo]) + pos;
+      if (pg >= 0 && pg < a.pages) s = (long long)pg * a.page + (pos - pi * a.page);
+      else us_dev_fail(a.status, US_DEV_BOUNDS);
+    }
+    src[threadIdx.x] = s;
+    dst[threadIdx.x] = d;
+  }
+  __syncthreads();
+  const int per_head = a.dim >> 4, per_row = a.heads * per_head, groups = a.dim >> 6;
+  const bool plane_v = blockIdx.y != 0;
+  const uint8_t* cache = plane_v ? a.vc : a.kc;
+  const __nv_bfloat16* scales = plane_v ? a.vs : a.ks;
+  __nv_bfloat16* out = plane_v ? a.vo : a.ko;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < kReadRows * per_row; e += 256) {
+    const int i = e / per_row, rest = e - i * per_row;
+    const int head = rest / per_head, ch = (rest - head * per_head) * 16;
+    const long long slot = src[i];
+    if (slot < 0) continue;
+    const long long p = slot / a.page;
+    const float sc = us::bf2f(scales[((p * a.heads + head) * a.page + (slot - p * a.page)) * groups + (ch >> 6)]);
+    const uint8_t* c = cache + (slot * a.heads + head) * (a.dim * BITS / 8) + ch * BITS / 8;
+    uint32_t o[8];
+    if constexpr (BITS == 8) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(c);
+      const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t u = w[j >> 1] >> (16 * (j & 1));
+        const __nv_bfloat162 b = __floats2bfloat162_rn(small_int(u & 255u, 128.f) * sc, small_int((u >> 8) & 255u, 128.f) * sc);
+        o[j] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    } else {
+      const uint2 raw = *reinterpret_cast<const uint2*>(c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t u = (j < 4 ? raw.x : raw.y) >> (8 * (j & 3));
+        const __nv_bfloat162 b = __floats2bfloat162_rn(small_int(u & 15u, 8.f) * sc, small_int((u >> 4) & 15u, 8.f) * sc);
+        o[j] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    }
+    uint4* to = reinterpret_cast<uint4*>(out + dst[i] * a.ldo + head * a.dim + ch);
+    to[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
+
+}  // namespace
+
+// Rows k, v [rows, heads, dim] (bf16; row and head strides in elements, multiples of 8) into integer pages at
+// `slots` (page * page_size + offset; int32, or int64 with wide != 0).  The slots of a call are distinct.
+US_API int us_quant_write(const void* k, const void* v, long long ldk, long long hsk, long long ldv, long long hsv,
+                          const void* slots, int wide, void* kc, void* vc, void* ks, void* vs, int rows, int pages,
+                          int page, int heads, int dim, int bits, void* stream_) {
+  US_REQUIRE(rows >= 0 && pages >= 1 && page >= 1 && heads >= 1 && dim >= 64 && dim % 64 == 0 && (bits == 8 || bits == 4));
+  if (rows == 0) return US_OK;
+  US_REQUIRE(k && v && slots && kc && vc && ks && vs);
+  US_REQUIRE(((ldk | hsk | ldv | hsv) % 8) == 0 && aligned16(k) && aligned16(v) && aligned16(kc) && aligned16(vc));
+  const WriteArgs a{(const __nv_bfloat16*)k, (const __nv_bfloat16*)v, slots, (uint8_t*)kc, (uint8_t*)vc,
+                    (__nv_bfloat16*)ks, (__nv_bfloat16*)vs, ldk, hsk, ldv, hsv, (long long)pages * page, rows, page,
+                    heads, dim, wide, us_status_ptr()};
+  const long long blocks = ((long long)rows * heads * (dim / 8) + 255) / 256;
+  if (blocks > 0x7fffffffLL) return US_ERR_LIMIT;
+  US_CUDA_CHECK(us::launch_pdl(bits == 8 ? quant_write_kernel<8> : quant_write_kernel<4>, dim3((unsigned)blocks),
+                               dim3(256), 0, (cudaStream_t)stream_, a));
+  return US_OK;
+}
+
+// The first cu[s + 1] - cu[s] cached rows of every sequence as bf16 rows [total, heads, dim] (row pitch ldo), packed,
+// or from row out_cu[s] on.  Rows past cu[B] are not written; a page outside the cache sets the status word.
+US_API int us_quant_gather(const void* kc, const void* vc, const void* ks, const void* vs, const int* table,
+                           int max_pages, const int* cu, const int* out_cu, int B, int total, int pages, int page,
+                           int heads, int dim, int bits, void* ko, void* vo, long long ldo, void* stream_) {
+  US_REQUIRE(B >= 0 && total >= 0 && pages >= 1 && page >= 1 && heads >= 1 && dim >= 64 && dim % 64 == 0 &&
+             (bits == 8 || bits == 4) && max_pages >= 0);
+  if (B == 0 || total == 0) return US_OK;
+  US_REQUIRE(kc && vc && ks && vs && table && cu && ko && vo && (ldo % 8) == 0);
+  US_REQUIRE(aligned16(kc) && aligned16(vc) && aligned16(ko) && aligned16(vo));
+  const ReadArgs a{(const uint8_t*)kc, (const uint8_t*)vc, (const __nv_bfloat16*)ks, (const __nv_bfloat16*)vs, table, cu,
+                   out_cu, (__nv_bfloat16*)ko, (__nv_bfloat16*)vo, ldo, B, max_pages, pages, page, heads, dim, total,
+                   us_status_ptr()};
+  US_CUDA_CHECK(us::launch_pdl(bits == 8 ? quant_gather_kernel<8> : quant_gather_kernel<4>,
+                               dim3((total + kReadRows - 1) / kReadRows, 2), dim3(256), 0, (cudaStream_t)stream_, a));
+  return US_OK;
+}

@@ -1,0 +1,398 @@
+"""Softmax attention whose scores are capped, biased by distance or masked.
+
+A row at position p of its sequence (the last row stands at the last key) sees key j under the score
+
+    s = scale q . k_j        s = cap tanh(s / cap)        s -= slope_h |p - j|
+
+where ``ScoreRules`` says so, and out_h = softmax(s) V over the keys that are visible to it, zeros where none is.
+
+* ``prompt_attention``: packed sequences of rows against packed keys (``attention.varlen_attention`` with rules); a
+  mask by documents, by a prefix that every row sees, by a window.  On a GPU ``csrc/scored_flash_tc05.cu``.
+* ``decode_attention``: one new row a sequence against cache pages, bf16 or integer (``quant_pages``); sequences may
+  share a prefix that is then read once for all of them.  On a GPU ``csrc/scored_decode.cu``, the prefix in
+  ``csrc/scored_flash_tc05.cu``.
+
+On the CPU both are FP32 formulas."""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import native as N
+
+P, I, L = N.P, N.I, N.L
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+N.register_signatures({
+    "us_scored_decode_scratch": (L, [I]),
+    "us_scored_decode": (I, [P, L, P, P, P, P, P, I, P, P, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, P, P, P, P,
+                             I, I, I, P]),
+    "us_scored_flash": (I, [P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, I, P, P, P, P]),
+    "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
+})
+
+MAX_SEQS = 1024            # sequences of one decode launch; larger batches go in slices
+MAX_KEYS = 1 << 20         # keys of a prompt's sequence
+_TILE = 128                # rows of a tile, keys of a block of the prompt kernel
+
+
+@dataclass(frozen=True)
+class ScoreRules:
+    """What happens to a score between scale q.k and the softmax."""
+    cap: float = 0.0                            # > 0: cap * tanh(score / cap)
+    slopes: Optional[torch.Tensor] = None       # FP32 [Hq]: - slope * |position - key|
+    window: int = 0                             # > 0: the last `window` keys, the row's own included
+
+
+@dataclass
+class SharedPrefix:
+    """Rows [cu_rows[g], cu_rows[g + 1]) of a decode batch share their first lens[g] keys: those are read through the
+    page list of the group's first row, once for all its rows.  ``max_rows`` and ``max_len`` bound the groups' sizes
+    for the host.  Rows past the last group share nothing."""
+    cu_rows: torch.Tensor      # int32 [groups + 1]
+    lens: torch.Tensor         # int32 [groups]
+    max_rows: int
+    max_len: int
+
+    @property
+    def groups(self) -> int:
+        return self.lens.shape[0]
+
+
+class on_device:
+    """The device of `tensors` (all on one; None is left out) as the current one."""
+
+    def __init__(self, *tensors):
+        at = None
+        for t in tensors:
+            if t is not None:
+                i = t.get_device()
+                if at is None:
+                    at = i
+                elif i != at:
+                    raise ValueError("the tensors of a call are on one device")
+        self.ctx = None if at == torch._C._cuda_getDevice() else torch.cuda.device(at)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *e):
+        if self.ctx is not None:
+            self.ctx.__exit__(*e)
+
+
+def _check_rules(rules, Hq, dev):
+    if not (rules.cap >= 0.0 and math.isfinite(rules.cap)) or rules.window < 0:
+        raise ValueError(f"cap {rules.cap} and window {rules.window} are not negative, and finite")
+    s = rules.slopes
+    if s is not None and (s.dtype != F32 or tuple(s.shape) != (Hq,) or not s.is_contiguous() or s.device != dev):
+        raise ValueError(f"slopes are a contiguous float32 [{Hq}] beside the queries; got {tuple(s.shape)} {s.dtype}")
+
+
+def _heads(q, k, v, what):
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
+        raise ValueError(f"{what}: q [rows, Hq, D], k and v [keys, Hkv, D]; got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    if not k.shape[1] or not q.shape[1] or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{what}: {q.shape[1]} query heads over {k.shape[1]} key heads")
+
+
+# ----------------------------------------------------------------- prompts --
+def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules = ScoreRules(), causal=True, docs=None,
+                     prefix=None, out=None):
+    """q [Tq, Hq, D], k / v [Tk, Hkv, D] bf16 (any strides; D a multiple of 8 up to 128), cu_q / cu_k int32 [n + 1] on the device,
+    max_q / max_k at least the longest sequence's rows and keys.  Row i of a sequence with nq rows and nk keys stands
+    at position p = i + nk - nq.  A key j is visible where
+
+        (not causal or j <= p) and (no window or j > p - window),    or j < prefix[sequence],
+
+    and, with ``docs`` (int32 [Tk], a number for every key; a row has that of the key at its position), where both
+    belong to the same document.  A row before its sequence's first key (nq > nk) has no document and sees nothing
+    under ``docs``.  ``prefix``: int32 [n].  Returns bf16 [Tq, Hq, D]; rows past cu_q[n] of a given ``out`` are left
+    as they were.  What keys and values hold past a sequence's end never reaches it; a key or value that is not finite
+    may reach any row of its own sequence that shares a block of 128 keys with one that sees it."""
+    _heads(q, k, v, "prompt_attention")
+    Tq, Hq, D = q.shape
+    _check_rules(rules, Hq, q.device)
+    n = cu_q.numel() - 1
+    if n < 0 or cu_k.numel() != n + 1 or cu_q.dtype != I32 or cu_k.dtype != I32:
+        raise ValueError("cu_q and cu_k are int32 [sequences + 1]")
+    if docs is not None and (docs.dtype != I32 or docs.shape != k.shape[:1]):
+        raise ValueError("docs is int32, one number a key")
+    if prefix is not None and (prefix.dtype != I32 or prefix.numel() != n):
+        raise ValueError("prefix is int32, one length a sequence")
+    if out is not None and (out.shape != q.shape or out.dtype != BF16):
+        raise ValueError("out has the shape of q, in bfloat16")
+    if not q.is_cuda:
+        res = _prompt_cpu(q, k, v, cu_q, cu_k, scale, rules, causal, docs, prefix)
+        if out is None:
+            return res
+        end = int(cu_q[-1])
+        out[:end] = res[:end]
+        return out
+    if q.dtype != BF16 or k.dtype != BF16 or v.dtype != BF16:
+        raise ValueError(f"scored attention is served in bfloat16; got {q.dtype}, {k.dtype}, {v.dtype}")
+    if D % 8 or D > 128 or max_k > MAX_KEYS:
+        raise ValueError(f"scored attention serves head widths that are multiples of 8 up to 128, and sequences of up to "
+                         f"{MAX_KEYS} keys; got width {D}, {max_k} keys")
+    with on_device(q, k, v, cu_q, cu_k, docs, prefix, rules.slopes, out):
+        if D not in (64, 128):          # zero channels add nothing to q.k and give zero channels, cut off again
+            wide = 64 if D < 64 else 128
+            q, k, v = (torch.nn.functional.pad(t, (0, wide - D)) for t in (q, k, v))
+            got = prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules, causal, docs, prefix)[..., :D]
+            if out is None:
+                return got.contiguous()
+            keep = torch.arange(Tq, device=q.device)[:, None, None] < cu_q[-1]
+            return out.copy_(torch.where(keep, got, out))
+        q, k, v = (_dense_heads(t) for t in (q, k, v))
+        to = out if out is not None and _fits(out) else torch.empty(Tq, Hq, D, dtype=BF16, device=q.device)
+        if out is not None and to is not out:
+            to.copy_(out)
+        if n and Tq and max_q > 0:
+            if not k.shape[0]:
+                k = v = torch.zeros(1, k.shape[1], D, dtype=BF16, device=q.device)
+                docs = None
+            ranges = None
+            if docs is not None:
+                docs = docs.contiguous()
+                ranges = torch.empty(2 * (k.shape[0] // _TILE + n + 1), dtype=I32, device=q.device)
+            N.call("us_scored_flash", N.ptr(q), q.stride(0), N.ptr(k), k.stride(0), N.ptr(v), v.stride(0), N.ptr(to),
+                   to.stride(0), N.ptr(cu_q.contiguous()), N.ptr(cu_k.contiguous()), n, Tq, k.shape[0], Hq, k.shape[1], D,
+                   max_q, max_k, scale, rules.cap, N.ptr(rules.slopes), int(causal), rules.window, N.ptr(docs),
+                   N.ptr(prefix.contiguous() if prefix is not None else None), N.ptr(ranges), N.stream(),
+                   launches=1 if docs is None else 2)
+        if out is not None and to is not out:
+            out.copy_(to)
+            return out
+        return to
+
+
+def _fits(t):
+    return t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+
+
+def _dense_heads(t):
+    """`t` with dense heads and rows on 16 bytes: as it is, or copied."""
+    if _fits(t):
+        return t
+    return t.clone() if t.is_contiguous() else t.contiguous()
+
+
+def _prompt_cpu(q, k, v, cu_q, cu_k, scale, rules, causal, docs, prefix):
+    out = torch.zeros_like(q)
+    G = q.shape[1] // k.shape[1]
+    for i in range(cu_q.numel() - 1):
+        q0, q1, k0, k1 = int(cu_q[i]), int(cu_q[i + 1]), int(cu_k[i]), int(cu_k[i + 1])
+        nq, nk = q1 - q0, k1 - k0
+        if nq <= 0 or nk <= 0:
+            continue
+        p, j = torch.arange(nk - nq, nk)[:, None], torch.arange(nk)[None]
+        see = torch.ones(nq, nk, dtype=torch.bool)
+        if causal:
+            see &= j <= p
+        if rules.window:
+            see &= j > p - rules.window
+        if prefix is not None:
+            see |= j < int(prefix[i])
+        if docs is not None:
+            d = docs[k0:k1]
+            see &= (d[p[:, 0].clamp(min=0)][:, None] == d[None]) & (p >= 0)
+        qq = q[q0:q1].float().unflatten(1, (-1, G))
+        s = torch.einsum("qhgd,khd->hgqk", qq, k[k0:k1].float()) * scale
+        w = _softmax(s, rules, (p - j).abs(), see)
+        out[q0:q1] = torch.einsum("hgqk,khd->qhgd", w, v[k0:k1].float()).flatten(1, 2).to(out.dtype)
+    return out
+
+
+def _softmax(s, rules, distance, see):
+    """Weights of scores s [Hkv, G, rows, keys]."""
+    if rules.cap:
+        s = rules.cap * torch.tanh(s / rules.cap)
+    if rules.slopes is not None:
+        s = s - rules.slopes.view(s.shape[0], s.shape[1], 1, 1) * distance.float()
+    s = s.masked_fill(~see, float("-inf"))
+    w = torch.softmax(s, -1)
+    return torch.where(see.any(-1, keepdim=True), w, torch.zeros_like(w))
+
+
+# ------------------------------------------------------------- single rows --
+@dataclass
+class DecodeWork:
+    """Workspace of ``decode_attention``: one serves every layer and step of a batch size, calls that share it being
+    ordered on the device (two captured graphs that may run side by side have one each)."""
+    scratch: torch.Tensor
+    counters: torch.Tensor                       # zero between calls
+    prefix_o: Optional[torch.Tensor] = None      # partial results of shared prefixes
+    prefix_ml: Optional[torch.Tensor] = None
+
+
+def _chunks(Hq, Hkv):
+    return -(-(Hq // Hkv) // 16)
+
+
+def _prefix_plan(shared: SharedPrefix, Hq, Hkv, sms):
+    """(tile pairs a group, parts, key blocks a part) of the prefix launch: its CTAs have 256 rows (query heads of a
+    key head times sequences) and a share of the prefix's 128-key blocks, as many shares as fill the GPU once."""
+    per = _TILE // (Hq // Hkv)                   # sequences of a tile
+    pairs = -(-shared.max_rows // (2 * per))
+    blocks = max(1, -(-shared.max_len // _TILE))
+    parts = max(1, min(sms // max(1, shared.groups * pairs * Hkv), -(-blocks // 2)))
+    each = -(-blocks // parts)
+    return pairs, -(-blocks // each), each
+
+
+_sms: dict = {}
+
+
+def _sm_count(device) -> int:
+    i = device.index if device.index is not None else torch.cuda.current_device()
+    if i not in _sms:
+        _sms[i] = torch.cuda.get_device_properties(i).multi_processor_count
+    return _sms[i]
+
+
+def decode_work(B, Hq, Hkv, D, device, shared: Optional[SharedPrefix] = None) -> DecodeWork:
+    """A workspace for batches of up to ``B`` sequences of these heads (and shared prefixes of up to these sizes)."""
+    device = torch.device(device)
+    with torch.cuda.device(device):
+        bytes_ = N.kernels().us_scored_decode_scratch(D)
+        w = DecodeWork(torch.empty(bytes_ // 4, dtype=F32, device=device),
+                       torch.zeros(min(B, MAX_SEQS) * Hkv * _chunks(Hq, Hkv), dtype=I32, device=device))
+        if shared is not None and shared.groups:
+            pairs, parts, _ = _prefix_plan(shared, Hq, Hkv, _sm_count(device))
+            rows = shared.groups * pairs * Hkv * parts * 2 * _TILE
+            w.prefix_o = torch.empty(rows * D, dtype=F32, device=device)
+            w.prefix_ml = torch.empty(rows * 2, dtype=F32, device=device)
+    return w
+
+
+def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: ScoreRules = ScoreRules(), starts=None,
+                     k_scale=None, v_scale=None, shared: Optional[SharedPrefix] = None, work: Optional[DecodeWork] = None,
+                     out=None):
+    """q [B, Hq, D] bf16, D 64 or 128; caches [pages, page_size, Hkv, D] bf16, or integer pages with their scales
+    (``quant_pages``); ``page_table`` int32 [B, max_pages], ``seq_lens`` int32 [B] (the new row's key included, so
+    the row stands at position length - 1; 0: the row's output is zero).  Keys from max(``starts`` (int32 [B]),
+    length - window) on are visible.  ``shared``: see ``SharedPrefix``; it goes with neither ``starts`` nor a window.
+    A page outside the cache counts as not visible and sets the device status, as does a length past the page table
+    (which is cut there).  Returns bf16 [B, Hq, D]."""
+    B, Hq, D = q.shape
+    if kcache.dim() != 4 or kcache.shape != vcache.shape:
+        raise ValueError("K and V pages have the same shape [pages, page_size, Hkv, D]")
+    pages, page, Hkv, width = kcache.shape
+    bits = 16
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("integer pages come with the scales of both planes")
+    if k_scale is not None:
+        from .quant_pages import GROUP, page_bits
+        bits = page_bits(kcache, vcache, k_scale, v_scale)
+        if k_scale.shape[3] * GROUP != D:
+            raise ValueError(f"queries of width {D} over pages of width {k_scale.shape[3] * GROUP}")
+    elif width != D or kcache.dtype != q.dtype or vcache.dtype != q.dtype:
+        raise ValueError(f"queries [.., {D}] {q.dtype} over pages [.., {width}] {kcache.dtype}")
+    if Hq % Hkv:
+        raise ValueError(f"{Hq} query heads over {Hkv} key heads")
+    _check_rules(rules, Hq, q.device)
+    if page_table.dim() != 2 or page_table.shape[0] < B or seq_lens.numel() < B or page_table.dtype != I32 or seq_lens.dtype != I32:
+        raise ValueError("page_table is int32 [B, max_pages], seq_lens int32 [B]")
+    if starts is not None and (starts.dtype != I32 or starts.numel() < B):
+        raise ValueError("starts is int32 [B]")
+    if out is not None and (tuple(out.shape) != (B, Hq, D) or out.dtype != BF16):
+        raise ValueError("out has the shape of q, in bfloat16")
+    if shared is not None and not shared.groups:
+        shared = None
+    if shared is not None:
+        if starts is not None or rules.window:
+            raise ValueError("a shared prefix goes with neither starts nor a window")
+        if shared.cu_rows.dtype != I32 or shared.lens.dtype != I32 or shared.cu_rows.numel() != shared.groups + 1:
+            raise ValueError("a shared prefix has int32 cu_rows [groups + 1] and lens [groups]")
+        if Hq // Hkv > _TILE or B > MAX_SEQS:
+            raise ValueError(f"a shared prefix is served for up to {_TILE} query heads a key head and {MAX_SEQS} sequences")
+    if not q.is_cuda:
+        res = _decode_cpu(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k_scale, v_scale, shared)
+        return res if out is None else out.copy_(res)
+    if q.dtype != BF16 or D not in (64, 128):
+        raise ValueError(f"scored decode attention serves bfloat16 queries of width 64 or 128; got {q.dtype}, {D}")
+    if not (page_table.is_contiguous() and seq_lens.is_contiguous() and kcache.is_contiguous() and vcache.is_contiguous()):
+        raise ValueError("pages, page table and lengths are contiguous")
+    if B > MAX_SEQS:
+        out = torch.empty(B, Hq, D, dtype=BF16, device=q.device) if out is None else out
+        for b in range(0, B, MAX_SEQS):
+            e = min(B, b + MAX_SEQS)
+            decode_attention(q[b:e], kcache, vcache, page_table[b:e], seq_lens[b:e], scale, rules,
+                             None if starts is None else starts[b:e], k_scale, v_scale, None, work, out[b:e])
+        return out
+    with on_device(q, kcache, vcache, k_scale, v_scale, page_table, seq_lens, starts, rules.slopes, out,
+                   shared.cu_rows if shared else None, shared.lens if shared else None):
+        q = _dense_heads(q)
+        to = out if out is not None and out.stride(2) == 1 and out.stride(1) == D and out.stride(0) % 2 == 0 and \
+            out.data_ptr() % 4 == 0 else torch.empty(B, Hq, D, dtype=BF16, device=q.device)
+        if work is None:
+            work = decode_work(B, Hq, Hkv, D, q.device, shared)
+        elif work.counters.numel() < B * Hkv * _chunks(Hq, Hkv) or work.counters.device != q.device or \
+                work.scratch.numel() * 4 < N.kernels().us_scored_decode_scratch(D):
+            raise ValueError("the workspace is of a smaller batch, fewer heads, or another device")
+        groups = 0
+        pre = (None,) * 4 + (1, 1, 1)
+        if B and shared is not None:
+            pairs, parts, each = _prefix_plan(shared, Hq, Hkv, _sm_count(q.device))
+            groups = shared.groups
+            rows = groups * pairs * Hkv * parts * 2 * _TILE
+            if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.prefix_ml.numel() < rows * 2:
+                raise ValueError("the workspace is of smaller shared prefixes")
+            k, v, cu = kcache, vcache, None
+            if bits != 16:       # the prefix is expanded once for all its readers; it stays in the L2 cache
+                from .quant_pages import kv_gather_quant
+                cu = torch.zeros(groups + 1, dtype=I32, device=q.device)
+                torch.cumsum(shared.lens, 0, out=cu[1:])
+                first = page_table.index_select(0, shared.cu_rows[:-1].clamp(max=B - 1))
+                k, v = kv_gather_quant(kcache, vcache, k_scale, v_scale, first, cu, groups * shared.max_len)
+            N.call("us_scored_prefix", N.ptr(q), q.stride(0), N.ptr(k), pages, N.ptr(v), page, N.ptr(cu), N.ptr(page_table),
+                   page_table.shape[1], k.shape[0], B, N.ptr(seq_lens), N.ptr(shared.cu_rows), N.ptr(shared.lens), groups,
+                   Hq, Hkv, D, shared.max_rows, scale, rules.cap, N.ptr(rules.slopes), N.ptr(work.prefix_o),
+                   N.ptr(work.prefix_ml), pairs, parts, each, N.stream())
+            pre = (N.ptr(shared.cu_rows), N.ptr(shared.lens), N.ptr(work.prefix_o), N.ptr(work.prefix_ml), pairs, parts, each)
+        if B:
+            N.call("us_scored_decode", N.ptr(q), q.stride(0), N.ptr(kcache), N.ptr(vcache), N.ptr(k_scale), N.ptr(v_scale),
+                   N.ptr(page_table), page_table.shape[1], N.ptr(seq_lens), N.ptr(starts), N.ptr(to), to.stride(0),
+                   N.ptr(work.scratch), N.ptr(work.counters), B, Hq, Hkv, D, bits, pages, page, rules.window, scale,
+                   rules.cap, N.ptr(rules.slopes), groups, *pre, N.stream())
+        if out is not None and to is not out:
+            return out.copy_(to)
+        return to
+
+
+def _decode_cpu(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k_scale, v_scale, shared):
+    from .quant_pages import dequantise
+    B, Hq, D = q.shape
+    pages, page, Hkv, _ = kcache.shape
+    out = torch.zeros_like(q)
+    for b in range(B):
+        n = int(seq_lens[b])
+        if n > page_table.shape[1] * page:
+            raise IndexError(f"sequence {b} has {n} keys, its page list {page_table.shape[1]} pages of {page}")
+        if n <= 0:
+            continue
+        j = torch.arange(n)
+        at = page_table[b, j // page].long()
+        if shared is not None:
+            g = int(torch.searchsorted(shared.cu_rows, b, right=True)) - 1
+            if g < shared.groups:
+                other = page_table[int(shared.cu_rows[g]), j // page].long()
+                at = torch.where(j < int(shared.lens[g]), other, at)
+        if int(at.min()) < 0 or int(at.max()) >= pages:
+            raise IndexError(f"sequence {b} names a page outside a cache of {pages}")
+        k, v = kcache[at, j % page], vcache[at, j % page]
+        if k_scale is not None:
+            k, v = dequantise(k, k_scale[at, :, j % page]), dequantise(v, v_scale[at, :, j % page])
+        see = torch.ones(1, n, dtype=torch.bool)
+        if starts is not None:
+            see &= j >= int(starts[b])
+        if rules.window:
+            see &= j >= n - rules.window
+        s = torch.einsum("hgd,khd->hgk", q[b].float().unflatten(0, (Hkv, -1)), k.float())[:, :, None] * scale
+        w = _softmax(s, rules, (n - 1 - j)[None], see)
+        out[b] = torch.einsum("hgqk,khd->qhgd", w, v.float()).reshape(Hq, D).to(out.dtype)
+    return out
