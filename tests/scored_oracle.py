@@ -27,7 +27,7 @@ def attend(q, k, v, scale, cap, slopes, p, see):
     s = s.masked_fill(~see, float("-inf"))
     some = see.any(1)
     if some.any():
-        err += float(s[:, see].abs().max()) * 2.0 ** -22
+        err += float(s[:, see].abs().max()) * 2.0 ** -19
     w = torch.where(some[None, :, None], torch.softmax(s, -1), torch.zeros_like(s))
     w = torch.where(see[None], w, torch.zeros_like(w))
     v = torch.where(see.any(0)[:, None, None], v, torch.zeros_like(v))   # what nobody sees weighs nothing
@@ -57,8 +57,9 @@ def cached(kc, ks, pages, count):
     return rows.reshape(-1, *rows.shape[2:])[:count]
 
 
-def decode(q, kc, vc, table, lens, scale, cap=0.0, slopes=None, window=0, starts=None, ks=None, vs=None):
-    """Row by row -> (out, bound) [B, Hq, D]."""
+def decode(q, kc, vc, table, lens, scale, cap=0.0, slopes=None, window=0, starts=None, ks=None, vs=None, rounded=None):
+    """Row by row -> (out, bound) [B, Hq, D].  The first `rounded[b]` keys and values of a row are those of the cache
+    rounded to bf16 (an expanded prefix)."""
     outs, bounds = [], []
     page = kc.shape[1]
     for b, n in enumerate(lens.tolist()):
@@ -69,6 +70,8 @@ def decode(q, kc, vc, table, lens, scale, cap=0.0, slopes=None, window=0, starts
         pages = table[b, :-(-n // page)].long()
         k, v = cached(kc, ks, pages, n), cached(vc, vs, pages, n)
         j = torch.arange(n, device=q.device)
+        if rounded is not None:
+            k, v = (torch.cat([t[:rounded[b]].bfloat16().double(), t[rounded[b]:]]) for t in (k, v))
         lo = max(n - window if window else 0, int(starts[b]) if starts is not None else 0)
         # keys that are not visible weigh nothing whatever they hold
         k, v = (torch.where((j >= lo)[:, None, None], t, torch.zeros_like(t)) for t in (k, v))

@@ -125,11 +125,11 @@ constexpr int kReadRows = 16;
 template <int BITS>
 __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
   US_PDL_PROLOGUE();
-  __shared__ long long src[kReadRows], dst[kReadRows];   // slot (-1: nothing to read), row of the output
+  __shared__ long long src[kReadRows], dst[kReadRows];   // slot (-1: a page outside the cache), output row (-1: none)
   const int r0 = blockIdx.x * kReadRows;
   if (threadIdx.x < kReadRows) {
     const int r = r0 + threadIdx.x;
-    long long s = -1, d = 0;
+    long long s = -1, d = -1;
     if (r < min(a.total, a.cu[a.B])) {
       int lo = 0, hi = a.B - 1;                 // sequence of packed row r
       while (lo < hi) {
@@ -156,7 +156,12 @@ __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
     const int i = e / per_row, rest = e - i * per_row;
     const int head = rest / per_head, ch = (rest - head * per_head) * 16;
     const long long slot = src[i];
-    if (slot < 0) continue;
+    if (dst[i] < 0) continue;
+    uint4* to = reinterpret_cast<uint4*>(out + dst[i] * a.ldo + head * a.dim + ch);
+    if (slot < 0) {
+      to[0] = to[1] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
     const long long p = slot / a.page;
     const float sc = us::bf2f(scales[((p * a.heads + head) * a.page + (slot - p * a.page)) * groups + (ch >> 6)]);
     const uint8_t* c = cache + (slot * a.heads + head) * (a.dim * BITS / 8) + ch * BITS / 8;
@@ -179,7 +184,6 @@ __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
         o[j] = *reinterpret_cast<const uint32_t*>(&b);
       }
     }
-    uint4* to = reinterpret_cast<uint4*>(out + dst[i] * a.ldo + head * a.dim + ch);
     to[0] = make_uint4(o[0], o[1], o[2], o[3]);
     to[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
@@ -209,7 +213,7 @@ US_API int us_quant_write(const void* k, const void* v, long long ldk, long long
 }
 
 // The first cu[s + 1] - cu[s] cached rows of every sequence as bf16 rows [total, heads, dim] (row pitch ldo), packed,
-// or from row out_cu[s] on.  Rows past cu[B] are not written; a page outside the cache sets the status word.
+// or from row out_cu[s] on.  Rows past cu[B] are not written; a page outside the cache is read as zeros and sets the status word.
 US_API int us_quant_gather(const void* kc, const void* vc, const void* ks, const void* vs, const int* table,
                            int max_pages, const int* cu, const int* out_cu, int B, int total, int pages, int page,
                            int heads, int dim, int bits, void* ko, void* vo, long long ldo, void* stream_) {

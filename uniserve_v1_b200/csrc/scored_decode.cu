@@ -532,8 +532,12 @@ __global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const Decode
         if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
       }
       const int blocks = (a.shared[g] + 127) >> 7;
-      np = (blocks + a.blocks_per_part - 1) / a.blocks_per_part;
+      np = min((blocks + a.blocks_per_part - 1) / a.blocks_per_part, a.parts);
       const int per = 128 / share, r = b - a.cu_rows[g];       // sequences of a 128-row tile of the prefix kernel
+      if (blocks > a.parts * a.blocks_per_part || r >= a.pairs * 2 * per) {   // a group larger than the host was told
+        us_dev_fail(a.status, US_DEV_BOUNDS);
+        if (r >= a.pairs * 2 * per) np = 0;
+      }
       const int tile = r / per, in_tile = (r - tile * per) * share + chunk * 16 + gi;
       at = ((((long long)g * a.pairs + (tile >> 1)) * a.Hkv + hk) * a.parts) * 256 + (tile & 1) * 128 + in_tile;
     }

@@ -1,0 +1,811 @@
+// Softmax attention of prompts whose scores are capped by a tanh, biased by distance, or masked by a window, a prefix
+// or documents; and the part of a decode batch's attention that a shared prefix has (scored_decode.cu has the rest).
+//
+//   s = scale q.k_j;  s = cap tanh(s / cap);  s -= slope |p - j|;  out = sum_j e^s v_j / sum_j e^s over visible j
+//
+// A CTA has two tiles of 128 rows and walks the 128-key blocks that any of them sees; the tensor pipe alternates
+// between the tiles, so one tile's softmax runs under the other's products.  S_X = Q_X K^T and O_X += P_X V are
+// tcgen05 products with S, P and O in tensor memory (P over the first half of S), operands by TMA, one thread a row in
+// the softmax (the layout of flash_attn2_tc05.cu).  What differs:
+//
+// * Blocks.  Before it starts a CTA writes down, one bit a block and tile, which blocks its rows see, from positions,
+//   window, prefix and, for documents, the smallest and largest document of each block; all roles walk these bits.
+//   A tile that does not see a block that the other one does takes no part in it.
+// * Masks.  In a block that not all rows of a warp see whole, a row's visible keys are 128 bits: intervals by
+//   arithmetic, documents by a ballot per distinct document among the warp's rows.
+// * Cap.  tanh costs the special-function unit, which the exponentials alone fill as long as the tensor pipe is
+//   busy (16,384 of either a block and tile, 1024 cycles), as much again or, by e^(2y) and a reciprocal, twice.  So
+//   cap tanh(s / cap) is an odd polynomial of degree seven in s on the FMA pipe, two scores an instruction, five
+//   instructions a pair (off by at most 3.6e-6 cap for |s| <= 0.75 cap; fitted here by weighted least squares to
+//   tanh's values); a warp that meets a larger score in a block takes the exponential form there.
+// * Bias.  Keys on one side of a row are a line in j, added within the polynomial's last multiply-add; a block
+//   with keys on both sides takes magnitudes.
+// * Values behind the last key of a sequence are put to zero in shared memory before their product: they belong to
+//   another sequence, or to nobody, and 0 x NaN is NaN.
+//
+// A shared prefix: rows of a tile are (sequence, query head of the key head) pairs of one group, the keys come through
+// the page list of the group's first row (or packed), split into `parts` of the blocks; unnormalised outputs, maxima and
+// sums go to the workspace.  Every wait is bounded.
+#include "include/us_common.cuh"
+#include "include/us_flash.cuh"
+#include "include/us_tc05.cuh"
+#include "include/us_tmap.h"
+
+namespace {
+
+using namespace flash;
+
+constexpr int kBM = 128, kBN = 128;
+constexpr int kHalf = 128 * 128;              // bytes of 64 columns of a tile
+constexpr float kRescaleThreshold = 8.f;      // log2 units
+constexpr int kMaxBlocks = 8192;              // key blocks of a sequence
+constexpr int kWords = kMaxBlocks / 32;
+constexpr int kThreads = 320;
+constexpr float kPolyReach = 0.75f;           // of the cap
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct ScoredArgs {
+  const int *cu_q, *cu_k;
+  __nv_bfloat16* out;
+  long long ldo;
+  int Tq, Tk, Hq, Hkv, causal, window;
+  const int *docs, *prefix;
+  const int2* ranges;                         // smallest and largest document of block j of sequence s at cu_k[s] / 128 + s + j
+  const float* slopes;
+  float scale_log2;
+  float poly[4], reach, scale_cap, cap_log2;  // cap: x = s (p0 + p1 s^2 + ...) where |s| <= reach
+  // shared prefixes
+  const int *table, *lens, *cu_rows, *shared, *cu_shared;
+  int max_pages, pages, page, batch, pairs, parts, blocks_per_part;
+  float *part_o, *part_ml;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ unsigned long long add2_rm(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rm.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2^t for two arguments in [-126, 128) on the FMA pipe (flash_attn2_tc05.cu): relative error 8.6e-5.
+__device__ __forceinline__ void ex2_poly2(float t0, float t1, float& p0, float& p1) {
+  const float kMagic = 12582912.f;
+  const unsigned long long x = pack2(fmaxf(t0, -126.f), fmaxf(t1, -126.f));
+  const unsigned long long tt = add2_rm(x, pack2(kMagic, kMagic));
+  const unsigned long long fr = fma2(add2(tt, pack2(-kMagic, -kMagic)), pack2(-1.f, -1.f), x);
+  unsigned long long p = fma2(fr, pack2(0.07706704f, 0.07706704f), pack2(0.22764499f, 0.22764499f));
+  p = fma2(p, fr, pack2(0.69511676f, 0.69511676f));
+  p = fma2(p, fr, pack2(1.f, 1.f));
+  float q0, q1, u0, u1;
+  unpack2(p, q0, q1);
+  unpack2(tt, u0, u1);
+  p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(u0) << 23));
+  p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(u1) << 23));
+}
+
+// bits [lo, hi) of 32
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 32);
+  return hi <= lo ? 0u : (0xffffffffu >> (32 - (hi - lo))) << lo;
+}
+
+// The blocks that a CTA walks, in order.
+struct Blocks {
+  const uint32_t* bits;     // [kWords] of tile A, then of tile B
+  int word, words;
+  uint32_t left;
+  __device__ __forceinline__ Blocks(const uint32_t* b, int n) : bits(b), word(0), words(n), left(n > 0 ? b[0] | b[kWords] : 0) {}
+  // the next block, and whether the tiles take part in it; -1 at the end
+  __device__ __forceinline__ int next(bool& a, bool& b) {
+    while (left == 0) {
+      if (++word >= words) return -1;
+      left = bits[word] | bits[kWords + word];
+    }
+    const int i = __ffs(left) - 1;
+    left &= left - 1;
+    a = (bits[word] >> i) & 1u;
+    b = (bits[kWords + word] >> i) & 1u;
+    return word * 32 + i;
+  }
+};
+
+// MODE 0: prompts.  1: shared prefixes.
+template <int kD, bool CAP, bool BIAS, int MODE, uint32_t EMU>
+__global__ void __launch_bounds__(kThreads, 1)
+scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV, const ScoredArgs a) {
+  US_PDL_PROLOGUE();
+  constexpr int kHalves = kD / 64, kTile = kHalves * kHalf;
+  constexpr int kTmaWarp = 8, kMmaWarp = 9;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int share = a.Hq / a.Hkv;
+  int seq, h = 0, hk, q0, q_start = 0, q_len, k_start, kv_len, shift = 0, per = kBM, pre = 0, part = 0;
+  long long prow0 = 0;
+  if constexpr (MODE == 0) {
+    seq = blockIdx.z;
+    h = blockIdx.y;
+    hk = h / share;
+    // under a causal mask the last rows walk the most blocks: they start first
+    q0 = (a.causal ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x) * 2 * kBM;
+    q_start = a.cu_q[seq];
+    q_len = min(a.cu_q[seq + 1], a.Tq) - q_start;
+    k_start = a.cu_k[seq];
+    kv_len = min(a.cu_k[seq + 1] - k_start, a.Tk - k_start);
+    shift = (a.cu_k[seq + 1] - k_start) - (a.cu_q[seq + 1] - q_start);
+    if (a.prefix) pre = max(0, min(a.prefix[seq], kv_len));
+  } else {
+    seq = blockIdx.z;
+    hk = blockIdx.y % a.Hkv;
+    const int pair = blockIdx.y / a.Hkv;
+    part = blockIdx.x;
+    per = kBM / share;
+    q_start = a.cu_rows[seq];                                   // sequences of the group
+    q_len = min(a.cu_rows[seq + 1], a.batch) - q_start;
+    q0 = pair * 2 * per;
+    k_start = a.cu_shared ? a.cu_shared[seq] : 0;
+    kv_len = a.shared[seq];
+    if (!a.cu_shared) kv_len = (int)min((long long)kv_len, (long long)a.max_pages * a.page);
+    prow0 = ((((long long)seq * a.pairs + pair) * a.Hkv + hk) * a.parts + part) * (2 * kBM);
+  }
+  if (q0 >= q_len) return;
+  kv_len = max(kv_len, 0);
+  int nb = min((kv_len + kBN - 1) / kBN, kMaxBlocks), jb = 0;
+  if constexpr (MODE == 1) {
+    jb = part * a.blocks_per_part;
+    nb = min(nb - jb, a.blocks_per_part);
+    if (nb <= 0) return;                                        // such a part is not read
+  }
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = smem;                  // two tiles
+  uint8_t* sK = smem + 2 * kTile;      // two stages
+  uint8_t* sV = smem + 4 * kTile;      // two stages
+  uint64_t* bars = (uint64_t*)(smem + 6 * kTile);
+  uint64_t* q_full = bars;
+  uint64_t* kv_full = bars + 1;        // [2]: V of a block and K of the next one
+  uint64_t* kv_empty = bars + 3;       // [2]
+  uint64_t* s_full = bars + 5;         // [2] by tile, like the next two
+  uint64_t* p_full = bars + 7;
+  uint64_t* o_full = bars + 9;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 11);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  int* taken = (int*)(tmem_slot + 2);  // [2]: blocks of each tile
+  uint32_t* bits = tmem_slot + 4;      // [2][kWords]
+
+  if (tid == 0) {
+    tc::mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&kv_full[i], 1);
+      tc::mbar_init(&kv_empty[i], 1);
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_full[i], 128);
+      tc::mbar_init(&o_full[i], 1);
+      taken[i] = 0;
+    }
+    *abort_flag = 0;
+    tc::mbar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    tc::tmem_alloc(tmem_slot, 512);
+    tc::tmem_relinquish();
+  }
+  __syncthreads();
+  // ---- which blocks the tiles see ----
+  const int words = (nb + 31) / 32;
+  const int2* ranges = nullptr;
+  if constexpr (MODE == 0) {
+    if (a.docs) ranges = a.ranges + (k_start / kBN + seq);
+  }
+  for (int w = warp; w < 2 * words; w += kThreads / 32) {
+    const int x = w >= words, wi = w - x * words;
+    const int j = wi * 32 + lane;
+    bool see = j < nb;
+    if constexpr (MODE == 0) {
+      const int r0 = q0 + x * kBM, r1 = min(r0 + kBM, q_len) - 1;          // the tile's rows
+      const int pa = r0 + shift, pb = r1 + shift;                         // and their positions
+      const int k0 = j * kBN, k1 = min(k0 + kBN, kv_len);
+      see &= r0 < q_len;
+      bool by_place = !a.causal || k0 <= pb;
+      if (a.window > 0) by_place &= k1 - 1 > pa - a.window;
+      see &= by_place || k0 < pre;
+      if (see && ranges) {
+        see = pb >= 0;
+        if (see) {
+          const int2 d0 = ranges[max(pa, 0) / kBN], d1 = ranges[min(pb, kv_len - 1) / kBN], d = ranges[j];
+          see = d.x <= max(d0.y, d1.y) && d.y >= min(d0.x, d1.x);
+        }
+      }
+    } else {
+      see &= q0 + x * per < q_len;
+    }
+    const uint32_t got = __ballot_sync(0xffffffffu, see);
+    if (lane == 0) {
+      bits[x * kWords + wi] = got;
+      if (got) atomicAdd(&taken[x], __popc(got));
+    }
+  }
+  tc::tc_fence_before_sync();
+  __syncthreads();
+  tc::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const int taken_a = taken[0], taken_b = taken[1];
+
+  if (MODE == 0 && tid < 2 * kBM) {    // rows that see nothing
+    const int x = tid >> 7, qi = q0 + tid;
+    if ((x ? taken_b : taken_a) == 0 && qi < q_len) {
+      uint4* dst = reinterpret_cast<uint4*>(a.out + (long long)(q_start + qi) * a.ldo + (long long)h * kD);
+      for (int i = 0; i < kD / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  if (taken_a + taken_b > 0) {
+    if (warp == kTmaWarp) {
+      // ---------------------------------------------------------------- loads --
+      // The whole warp walks; lane 0 loads whole tiles, or every lane its page of a tile.
+      const bool paged = MODE == 1 && a.table && !a.cu_shared;
+      const int rows_at_once = paged ? min(a.page, kBN) : kBN;
+      const int loads = kBN / rows_at_once;
+      auto row_of = [&](int j) -> int {      // first row of this lane's load of block j
+        const int key = (jb + j) * kBN + lane * rows_at_once;
+        if (!paged) return k_start + key;
+        if (lane >= loads || key >= kv_len) return a.pages * a.page;      // out of the tensor: zeros
+        const int pi = key / a.page;
+        const int pg = a.table[(long long)q_start * a.max_pages + pi];
+        if ((unsigned)pg >= (unsigned)a.pages) {
+          us_dev_fail(a.status, US_DEV_BOUNDS);
+          return a.pages * a.page;
+        }
+        return pg * a.page + (key - pi * a.page);
+      };
+      auto load_tile = [&](uint8_t* to, const CUtensorMap* m, uint64_t* bar, int row) {
+        if (lane < loads) {
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf)
+            tc::tma_load_2d(to + hf * kHalf + lane * rows_at_once * 128, m, bar, hk * kD + 64 * hf, row);
+        }
+      };
+      Blocks walk(bits, words);
+      bool ta, tb;
+      int j = walk.next(ta, tb);
+      int row = row_of(j);
+      const uint32_t q_bytes = MODE == 0 ? 2 * kTile : 2 * kHalves * per * share * 128;
+      if (lane == 0) {
+        tc::tma_prefetch_desc(&tmQ);
+        tc::tma_prefetch_desc(&tmK);
+        tc::tma_prefetch_desc(&tmV);
+        tc::mbar_expect_tx(q_full, q_bytes + kTile);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf) {
+            uint8_t* to = sQ + x * kTile + hf * kHalf;
+            if constexpr (MODE == 0) tc::tma_load_2d(to, &tmQ, q_full, h * kD + 64 * hf, q_start + q0 + x * kBM);
+            else tc::tma_load_3d(to, &tmQ, q_full, 64 * hf, hk * share, q_start + q0 + x * per);
+          }
+      }
+      __syncwarp();
+      load_tile(sK, &tmK, q_full, row);
+      for (int e = 0; j >= 0; ++e) {
+        const int st = e & 1;
+        const int jn = walk.next(ta, tb);
+        const int row_n = jn >= 0 ? row_of(jn) : 0;
+        // kv_empty[1] completes first after the first S products: K stage 0 is free again
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(&kv_empty[st], ((uint32_t)((e + 1) >> 1) & 1u) ^ 1u, abort_flag))) {
+          if (lane == 0) {
+            us_dev_fail(a.status, US_DEV_TIMEOUT_EMPTY);
+            *abort_flag = 1;
+          }
+          break;
+        }
+        if (lane == 0) tc::mbar_expect_tx(&kv_full[st], jn >= 0 ? 2 * kTile : kTile);
+        __syncwarp();
+        load_tile(sV + st * kTile, &tmV, &kv_full[st], row);
+        if (jn >= 0) load_tile(sK + (st ^ 1) * kTile, &tmK, &kv_full[st], row_n);
+        j = jn;
+        row = row_n;
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------- products --
+      auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag));
+      };
+      constexpr uint32_t kIdescQK = tc::make_idesc(kBM, kBN, tc::kFmtBF16, tc::kFmtBF16, 0, 0);
+      constexpr uint32_t kIdescPV = tc::make_idesc(kBM, kD, tc::kFmtBF16, tc::kFmtBF16, 0, 1);
+      const uint64_t dq = tc::smem_desc_kmajor_sw128(tc::smem_u32(sQ));
+      const uint64_t dk = tc::smem_desc_kmajor_sw128(tc::smem_u32(sK));
+      const uint64_t dv = tc::smem_desc_mnmajor_sw128(tc::smem_u32(sV), kHalf, 1024);
+      const uint32_t q_lo = (uint32_t)dq, k_lo = (uint32_t)dk, v_lo = (uint32_t)dv;
+      const uint32_t km_hi = (uint32_t)(dq >> 32), mn_hi = (uint32_t)(dv >> 32);
+      auto issue_qk = [&](int x, int e) {
+        const uint32_t qa = q_lo + (uint32_t)x * (kTile >> 4), kb = k_lo + (uint32_t)(e & 1) * (kTile >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {
+          const uint32_t off = (uint32_t)(kk >> 2) * (kHalf >> 4) + 2u * (uint32_t)(kk & 3);
+          umma_f16_words(tmem_base + (uint32_t)x * kBN, qa + off, km_hi, kb + off, km_hi, kIdescQK, kk != 0);
+        }
+        umma_commit_elect(&s_full[x]);
+      };
+      auto issue_pv = [&](int x, int e, int n, int all) {      // n: blocks of this tile so far
+        const uint32_t vb = v_lo + (uint32_t)(e & 1) * (kTile >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_f16_ts_words(tmem_base + 256 + (uint32_t)x * kD, tmem_base + (uint32_t)x * kBN + kk * 8,
+                            vb + (uint32_t)kk * (2048 >> 4), mn_hi, kIdescPV, (n | kk) != 0);
+        if (n == all - 1) umma_commit_elect(&o_full[x]);
+      };
+      Blocks walk(bits, words);
+      bool a0 = false, b0 = false, a1 = false, b1 = false;
+      int j = walk.next(a0, b0), na = 0, nbb = 0;
+      bool ok = warp_wait(q_full, 0);
+      if (ok) {
+        tc::tc_fence_after_sync();
+        if (a0) issue_qk(0, 0);
+        if (b0) issue_qk(1, 0);
+        umma_commit_elect(&kv_empty[1]);
+      }
+      for (int e = 0; ok && j >= 0; ++e) {
+        a1 = b1 = false;
+        const int jn = walk.next(a1, b1);
+        if (!warp_wait(&kv_full[e & 1], (uint32_t)(e >> 1) & 1u)) { ok = false; break; }
+        const int there = kv_len - (jb + j) * kBN;
+        if (there < kBN) {               // the sequence ends in this block
+          for (int r = there + (lane >> 3); r < kBN; r += 4)
+#pragma unroll
+            for (int hf = 0; hf < kHalves; ++hf)
+              *reinterpret_cast<uint4*>(sV + (e & 1) * kTile + hf * kHalf + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          tc::fence_async_smem();
+          __syncwarp();
+        }
+        if (a0) {
+          if (!warp_wait(&p_full[0], (uint32_t)na & 1u)) { ok = false; break; }
+          tc::tc_fence_after_sync();
+          issue_pv(0, e, na++, taken_a);
+        }
+        if (a1) issue_qk(0, e + 1);
+        if (b0) {
+          if (!warp_wait(&p_full[1], (uint32_t)nbb & 1u)) { ok = false; break; }
+          tc::tc_fence_after_sync();
+          issue_pv(1, e, nbb++, taken_b);
+        }
+        if (b1) issue_qk(1, e + 1);
+        umma_commit_elect(&kv_empty[e & 1]);
+        j = jn;
+        a0 = a1;
+        b0 = b1;
+      }
+      if (!ok && lane == 0) {
+        us_dev_fail(a.status, US_DEV_TIMEOUT_FULL);
+        *abort_flag = 1;
+      }
+    } else {
+      // -------------------------------------------------------------- softmax --
+      const int x = warp >> 2, r = (warp & 3) * 32 + lane;
+      const uint32_t lane_addr = ((uint32_t)((warp & 3) * 32) << 16);
+      const uint32_t s_tmem = tmem_base + (uint32_t)x * kBN + lane_addr;
+      const uint32_t o_tmem = tmem_base + 256 + (uint32_t)x * kD + lane_addr;
+      // the row: its position, its visible keys [lo, hi) and [0, pr), its document
+      int p, lo = 0, hi = 0, pr = 0, doc = 0, row = 0;
+      float sl = 0.f;
+      bool row_ok;
+      if constexpr (MODE == 0) {
+        row = q0 + x * kBM + r;
+        row_ok = row < q_len;
+        p = row + shift;
+        if (row_ok) {
+          hi = a.causal ? min(kv_len, p + 1) : kv_len;
+          if (a.window > 0) lo = max(0, p - a.window + 1);
+          pr = pre;
+          if (a.docs) {
+            if (p >= 0 && p < kv_len) doc = a.docs[k_start + p];
+            else hi = pr = 0;
+          }
+        }
+        if (BIAS) sl = a.slopes[h] * kLog2e;
+      } else {
+        const int b_local = q0 + x * per + r / share;
+        row_ok = r < per * share && b_local < q_len;
+        p = 0;
+        if (row_ok) {
+          const int len = a.lens[q_start + b_local];
+          p = len - 1;
+          hi = min(kv_len, len);
+        }
+        if (BIAS) sl = row_ok ? a.slopes[hk * share + r % share] * kLog2e : 0.f;
+      }
+      const unsigned long long sc2 = pack2(a.scale_log2, a.scale_log2);
+      unsigned long long c0 = 0, c1 = 0, c2 = 0, c3 = 0;
+      if (CAP) {
+        c0 = pack2(a.poly[0], a.poly[0]);
+        c1 = pack2(a.poly[1], a.poly[1]);
+        c2 = pack2(a.poly[2], a.poly[2]);
+        c3 = pack2(a.poly[3], a.poly[3]);
+      }
+      float m_used = -INFINITY, l_sum = 0.f;
+      Blocks walk(bits, words);
+      int n = 0;
+      bool ok = true;
+      while (ok) {
+        bool mine, other;
+        int j;
+        do {
+          bool ta, tb;
+          j = walk.next(ta, tb);
+          mine = x ? tb : ta;
+        } while (j >= 0 && !mine);
+        (void)other;
+        if (j < 0) break;
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_full[x], (uint32_t)n & 1u, abort_flag))) { ok = false; break; }
+        tc::tc_fence_after_sync();
+        uint32_t v[kBN];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+        const int kbase = (jb + j) * kBN;
+        // what of the block is visible to the row
+        const bool whole = (lo <= kbase && hi >= kbase + kBN) || pr >= kbase + kBN;
+        bool mixed = false;
+        if (MODE == 0 && ranges) {
+          const int2 d = ranges[j];
+          mixed = d.x != doc || d.y != doc;
+        }
+        const bool masked = __any_sync(0xffffffffu, !whole || mixed);
+        uint32_t see[4];
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            see[c] = bits_between(lo - kbase - 32 * c, hi - kbase - 32 * c) | bits_between(0, pr - kbase - 32 * c);
+          if (MODE == 0 && a.docs) {
+            int kd[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int key = kbase + 32 * c + lane;
+              kd[c] = key < kv_len ? a.docs[k_start + key] : 0;      // past the end: not visible by place
+            }
+            uint32_t left = 0xffffffffu;
+            while (left) {                   // once for every document among the warp's rows
+              const int d = __shfl_sync(0xffffffffu, doc, __ffs(left) - 1);
+              const bool is = doc == d;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const uint32_t same = __ballot_sync(0xffffffffu, kd[c] == d);
+                if (is) see[c] &= same;
+              }
+              left &= ~__ballot_sync(0xffffffffu, is);
+            }
+          }
+        }
+        tc::tmem_ld_wait();
+        // v: raw scores, or with a cap or a bias scores in units of log2(e)
+        const int delta = p - kbase;
+        if (CAP || BIAS) {
+          bool poly = true;
+          if (CAP) {
+            float big[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                big[c] = max3_abs(big[c], __uint_as_float(v[32 * c + i]), __uint_as_float(v[32 * c + i + 1]));
+            // (a comparison that a NaN fails: such a block takes the other form, which passes it on)
+            poly = __all_sync(0xffffffffu, fabsf(fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]))) <= a.reach);
+            if (!poly) {
+#pragma unroll
+              for (int i = 0; i < kBN; ++i)   // tanh y = 1 - 2 / (1 + e^(2 y))
+                v[i] = __float_as_uint(fmaf(-2.f * a.cap_log2, rcpf(1.f + ex2f(__uint_as_float(v[i]) * a.scale_cap)), a.cap_log2));
+            }
+          }
+          if (BIAS && __any_sync(0xffffffffu, delta > 0 && delta < kBN - 1)) {
+            // keys on both sides of some row
+#pragma unroll
+            for (int i = 0; i < kBN; ++i) {
+              const float bias = -sl * fabsf((float)(delta - i));
+              const float s = __uint_as_float(v[i]);
+              if (CAP && poly) {
+                const float w = s * s;
+                v[i] = __float_as_uint(fmaf(s, fmaf(fmaf(fmaf(a.poly[3], w, a.poly[2]), w, a.poly[1]), w, a.poly[0]), bias));
+              } else {
+                v[i] = __float_as_uint(CAP ? s + bias : fmaf(s, a.scale_log2, bias));
+              }
+            }
+          } else if (BIAS || poly) {
+            const float step = delta > 0 ? sl : -sl, at = -sl * fabsf((float)delta);
+            unsigned long long b2[4];
+            const unsigned long long st2 = pack2(2.f * step, 2.f * step);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              b2[c] = BIAS ? pack2(fmaf(step, 32.f * c, at), fmaf(step, 32.f * c + 1.f, at)) : 0ull;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint32_t& e0 = v[32 * c + i];
+                uint32_t& e1 = v[32 * c + i + 1];
+                const unsigned long long s2 = pack2(__uint_as_float(e0), __uint_as_float(e1));
+                unsigned long long y;
+                if (CAP && poly) {
+                  const unsigned long long w = mul2(s2, s2);
+                  y = fma2(fma2(fma2(c3, w, c2), w, c1), w, c0);
+                  y = BIAS ? fma2(s2, y, b2[c]) : mul2(s2, y);
+                } else {
+                  y = CAP ? add2(s2, b2[c]) : fma2(s2, sc2, b2[c]);
+                }
+                if (BIAS) b2[c] = add2(b2[c], st2);
+                float y0, y1;
+                unpack2(y, y0, y1);
+                e0 = __float_as_uint(y0);
+                e1 = __float_as_uint(y1);
+              }
+            }
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((see[c] >> i) & 1u)) v[32 * c + i] = 0xff800000u;
+        }
+        float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            mxs[c] = max3(mxs[c], __uint_as_float(v[32 * c + i]), __uint_as_float(v[32 * c + i + 1]));
+        const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+        const float m_new = fmaxf(m_used, (CAP || BIAS) ? mx : mx * a.scale_log2);
+        if (__any_sync(0xffffffffu, m_new - m_used > kRescaleThreshold || (m_used == -INFINITY && m_new > -INFINITY))) {
+          const float alpha = m_used == -INFINITY ? 0.f : ex2f(m_used - m_new);
+          if (n > 0) {
+            // O_X is still: this block's S was issued after the last block's product, by the same thread
+#pragma unroll 1
+            for (int c = 0; c < kD; c += 32) {
+              uint32_t w[32];
+              tc::tmem_ld32(o_tmem + c, w);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * alpha);
+              tc::tmem_st32(o_tmem + c, w);
+            }
+          }
+          l_sum *= alpha;
+          m_used = m_new;
+        }
+        const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+        const unsigned long long nm2 = pack2(neg_m, neg_m);
+        unsigned long long ls[4] = {0ull, 0ull, 0ull, 0ull};
+        uint32_t pk[kBN / 2];
+        auto exp_pair = [&](uint32_t s0, uint32_t s1, unsigned long long& l, bool poly) -> uint32_t {
+          const unsigned long long s2 = pack2(__uint_as_float(s0), __uint_as_float(s1));
+          float t0, t1, p0, p1;
+          unpack2((CAP || BIAS) ? add2(s2, nm2) : fma2(s2, sc2, nm2), t0, t1);
+          if (poly) {
+            ex2_poly2(t0, t1, p0, p1);
+          } else {
+            p0 = ex2f(t0);
+            p1 = ex2f(t1);
+          }
+          l = add2(l, pack2(p0, p1));
+          const __nv_bfloat162 t = __floats2bfloat162_rn(p0, p1);
+          return *reinterpret_cast<const uint32_t*>(&t);
+        };
+        if (EMU != 0 && !masked) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              pk[16 * c + (i >> 1)] = exp_pair(v[32 * c + i], v[32 * c + i + 1], ls[c], (EMU >> (((i >> 1) & 1) * 4 + c)) & 1u);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              pk[16 * c + (i >> 1)] = exp_pair(v[32 * c + i], v[32 * c + i + 1], ls[c], false);
+        }
+        {
+          float s0, s1;
+          unpack2(add2(add2(ls[0], ls[1]), add2(ls[2], ls[3])), s0, s1);
+          l_sum += s0 + s1;
+        }
+        tc::tmem_st32(s_tmem, *reinterpret_cast<const uint32_t(*)[32]>(pk));
+        tc::tmem_st32(s_tmem + 32, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32));
+        tc::tmem_st_wait();
+        tc::tc_fence_before_sync();
+        tc::mbar_arrive(&p_full[x]);
+        ++n;
+      }
+      if (n > 0 || !ok) {
+        if (ok && __all_sync(0xffffffffu, tc::mbar_wait(&o_full[x], 0, abort_flag))) {
+          tc::tc_fence_after_sync();
+          const float inv = MODE == 0 ? (l_sum == 0.f ? 0.f : 1.f / l_sum) : 1.f;
+          const long long prow = prow0 + x * kBM + r;
+          if (MODE == 1 && row_ok) *reinterpret_cast<float2*>(a.part_ml + prow * 2) = make_float2(m_used, l_sum);
+#pragma unroll 1
+          for (int c = 0; c < kD; c += 32) {
+            uint32_t w[32];
+            tc::tmem_ld32(o_tmem + c, w);
+            tc::tmem_ld_wait();
+            if (row_ok) {
+              if constexpr (MODE == 0) {
+                __nv_bfloat16* orow = a.out + (long long)(q_start + row) * a.ldo + (long long)h * kD;
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                  us::Pack16 o;
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) o.b[i] = us::f2bf(__uint_as_float(w[q4 * 8 + i]) * inv);
+                  *reinterpret_cast<uint4*>(orow + c + q4 * 8) = o.u;
+                }
+              } else {
+#pragma unroll
+                for (int q4 = 0; q4 < 8; ++q4)
+                  *reinterpret_cast<uint4*>(a.part_o + prow * kD + c + q4 * 4) =
+                      make_uint4(w[q4 * 4], w[q4 * 4 + 1], w[q4 * 4 + 2], w[q4 * 4 + 3]);
+              }
+            }
+          }
+        } else {
+          us_dev_fail(a.status, US_DEV_TIMEOUT_ACC);
+          *abort_flag = 1;
+        }
+      }
+    }
+  }
+  tc::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc::tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Smallest and largest document of every 128-key block: a warp a block.
+__global__ void __launch_bounds__(128) doc_ranges_kernel(const int* docs, const int* cu_k, int Tk, int2* ranges) {
+  US_PDL_PROLOGUE();
+  const int seq = blockIdx.y, j = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int start = cu_k[seq], end = min(cu_k[seq + 1], Tk);
+  if (start + j * kBN >= end) return;
+  int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int k = start + j * kBN + 32 * c + lane;
+    if (k < end) {
+      const int d = docs[k];
+      lo = min(lo, d);
+      hi = max(hi, d);
+    }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) ranges[start / kBN + seq + j] = make_int2(lo, hi);
+}
+
+size_t shared_bytes(int D) { return 6 * (size_t)(D / 64) * kHalf + 11 * 8 + 16 + 2 * kWords * 4 + 1024; }
+
+void set_rules(ScoredArgs& a, float scale, float cap, const float* slopes) {
+  a.scale_log2 = scale * kLog2e;
+  a.slopes = slopes;
+  if (cap > 0.f) {
+    // tanh(y) ~ y (t0 + t1 y^2 + t2 y^4 + t3 y^6) for |y| <= 0.75, with y = s scale / cap; out of a reasonable range
+    // of scale / cap the powers leave FP32's and the exponential form serves alone
+    const double t[4] = {0.9999556, -0.33222756, 0.1257706, -0.0337779}, k = (double)scale / cap;
+    double f = k * cap * (double)kLog2e;
+    for (int i = 0; i < 4; ++i, f *= k * k) a.poly[i] = (float)(t[i] * f);
+    const double mag = k < 0 ? -k : k;
+    a.reach = mag > 1e-4 && mag < 1e4 ? (float)(kPolyReach / mag) : -1.f;
+    a.scale_cap = (float)(2.0 * k * kLog2e);
+    a.cap_log2 = cap * kLog2e;
+  }
+}
+
+template <int D, bool CAP, bool BIAS, int MODE>
+int start(dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ScoredArgs& a, cudaStream_t stream) {
+  // 64-wide heads have half the tensor work per exponential: a quarter of them on the FMA pipe (flash_attn2_tc05.cu)
+  constexpr uint32_t kEmu = D == 64 && !CAP ? 0x21u : 0u;
+  const size_t bytes = shared_bytes(D);
+  US_CUDA_CHECK((us::allow_shared<scored_flash_kernel<D, CAP, BIAS, MODE, kEmu>>((int)bytes)));
+  US_CUDA_CHECK(us::launch_pdl(scored_flash_kernel<D, CAP, BIAS, MODE, kEmu>, grid, dim3(kThreads), bytes, stream, q, k, v, a));
+  return US_OK;
+}
+template <int MODE>
+int start_any(int D, bool cap, dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ScoredArgs& a,
+              cudaStream_t stream) {
+  const bool bias = a.slopes != nullptr;
+  if (D == 128) {
+    if (cap) return bias ? start<128, true, true, MODE>(grid, q, k, v, a, stream) : start<128, true, false, MODE>(grid, q, k, v, a, stream);
+    return bias ? start<128, false, true, MODE>(grid, q, k, v, a, stream) : start<128, false, false, MODE>(grid, q, k, v, a, stream);
+  }
+  if (cap) return bias ? start<64, true, true, MODE>(grid, q, k, v, a, stream) : start<64, true, false, MODE>(grid, q, k, v, a, stream);
+  return bias ? start<64, false, true, MODE>(grid, q, k, v, a, stream) : start<64, false, false, MODE>(grid, q, k, v, a, stream);
+}
+
+}  // namespace
+
+// q [Tq, Hq, D], k / v [Tk, Hkv, D], out [Tq, Hq, D], bf16 with row pitches; cu_q / cu_k [n + 1].  docs [Tk] with ranges
+// (int32 [2 (Tk / 128 + n + 1)], written here), prefix [n], slopes [Hq]: or null.  cap 0, window 0: none.
+US_API int us_scored_flash(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out,
+                           long long ldo, const int* cu_q, const int* cu_k, int n, int Tq, int Tk, int Hq, int Hkv, int D,
+                           int max_q, int max_k, float scale, float cap, const float* slopes, int causal, int window,
+                           const int* docs, const int* prefix, void* ranges, void* stream_) {
+  US_REQUIRE(q && k && v && out && cu_q && cu_k && n >= 1 && n <= 65535 && Tq >= 1 && Tk >= 1 && max_q >= 1 && max_k >= 0);
+  US_REQUIRE((D == 64 || D == 128) && Hkv >= 1 && Hq >= 1 && Hq <= 65535 && Hq % Hkv == 0 && window >= 0 && cap >= 0.f);
+  US_REQUIRE(((ldq | ldk | ldv | ldo) % 8) == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16) == 0);
+  US_REQUIRE(!docs || ranges);
+  US_REQUIRE(max_k <= kMaxBlocks * kBN);
+  CUtensorMap tmQ, tmK, tmV;
+  int rc = us_tmap_2d(&tmQ, q, US_TMAP_BF16, (uint64_t)Tq, (uint64_t)Hq * D, (uint64_t)ldq, kBM, 64, US_SWZ_128);
+  if (!rc) rc = us_tmap_2d(&tmK, k, US_TMAP_BF16, (uint64_t)Tk, (uint64_t)Hkv * D, (uint64_t)ldk, kBN, 64, US_SWZ_128);
+  if (!rc) rc = us_tmap_2d(&tmV, v, US_TMAP_BF16, (uint64_t)Tk, (uint64_t)Hkv * D, (uint64_t)ldv, kBN, 64, US_SWZ_128);
+  if (rc) return rc;
+  cudaStream_t stream = (cudaStream_t)stream_;
+  ScoredArgs a = {};
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.out = (__nv_bfloat16*)out;
+  a.ldo = ldo;
+  a.Tq = Tq;
+  a.Tk = Tk;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.causal = causal;
+  a.window = window;
+  a.docs = docs;
+  a.prefix = prefix;
+  a.ranges = (const int2*)ranges;
+  a.status = us_status_ptr();
+  set_rules(a, scale, cap, slopes);
+  if (docs && max_k > 0)
+    US_CUDA_CHECK(us::launch_pdl(doc_ranges_kernel, dim3(((max_k + kBN - 1) / kBN + 3) / 4, n), dim3(128), 0, stream, docs, cu_k, Tk, (int2*)ranges));
+  return start_any<0>(D, cap > 0.f, dim3((max_q + 2 * kBM - 1) / (2 * kBM), Hq, n), tmQ, tmK, tmV, a, stream);
+}
+
+// The part that the shared prefixes of a decode batch have in its attention (scored_decode.cu): rows
+// [cu_rows[g], cu_rows[g + 1]) of q [B, Hq, D] against the first shared[g] keys behind row cu_rows[g]'s page list in
+// k / v [pages, page, Hkv, D], or, with cu_shared [groups + 1], against packed rows k / v [key_rows, Hkv, D].
+// part_o, part_ml: [groups][pairs][Hkv][parts][256][D and 2].
+US_API int us_scored_prefix(const void* q, long long ldq, const void* k, long long pages, const void* v, long long page,
+                            const int* cu_shared, const int* table, int max_pages, int key_rows, int B, const int* lens,
+                            const int* cu_rows, const int* shared, int groups, int Hq, int Hkv, int D, int max_rows, float scale,
+                            float cap, const float* slopes, float* part_o, float* part_ml, int pairs, int parts,
+                            int blocks_per_part, void* stream_) {
+  US_REQUIRE(q && k && v && lens && cu_rows && shared && part_o && part_ml && (cu_shared || table) && groups >= 1 && groups <= 65535 && B >= 1);
+  US_REQUIRE((D == 64 || D == 128) && Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= kBM && cap >= 0.f && max_rows >= 1);
+  US_REQUIRE((ldq % 8) == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16) == 0 && pairs >= 1 && parts >= 1 &&
+             blocks_per_part >= 1 && blocks_per_part <= kMaxBlocks && (long long)pairs * Hkv <= 65535);
+  const int share = Hq / Hkv, per = kBM / share;
+  US_REQUIRE((long long)pairs * 2 * per >= max_rows);
+  uint64_t rows = (uint64_t)key_rows;
+  uint32_t box = kBN;
+  if (!cu_shared) {
+    US_REQUIRE(pages >= 1 && page >= 8 && (kBN % page == 0 || page % kBN == 0) && pages * page <= 0x7fffff00LL && max_pages >= 1);
+    rows = (uint64_t)(pages * page);
+    box = (uint32_t)(page < kBN ? page : kBN);
+  }
+  US_REQUIRE(rows >= 1);
+  CUtensorMap tmQ, tmK, tmV;
+  const uint64_t dims[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)B};
+  const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)ldq * 2};
+  const uint32_t qbox[3] = {64, (uint32_t)share, (uint32_t)per};
+  int rc = us_tmap_encode(&tmQ, q, US_TMAP_BF16, 3, dims, strides, qbox, US_SWZ_128);
+  if (!rc) rc = us_tmap_2d(&tmK, k, US_TMAP_BF16, rows, (uint64_t)Hkv * D, (uint64_t)Hkv * D, box, 64, US_SWZ_128);
+  if (!rc) rc = us_tmap_2d(&tmV, v, US_TMAP_BF16, rows, (uint64_t)Hkv * D, (uint64_t)Hkv * D, box, 64, US_SWZ_128);
+  if (rc) return rc;
+  ScoredArgs a = {};
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.table = table;
+  a.max_pages = max_pages;
+  a.pages = (int)pages;
+  a.page = (int)page;
+  a.cu_shared = cu_shared;
+  a.lens = lens;
+  a.cu_rows = cu_rows;
+  a.shared = shared;
+  a.batch = B;
+  a.pairs = pairs;
+  a.parts = parts;
+  a.blocks_per_part = blocks_per_part;
+  a.part_o = part_o;
+  a.part_ml = part_ml;
+  a.status = us_status_ptr();
+  set_rules(a, scale, cap, slopes);
+  return start_any<1>(D, cap > 0.f, dim3(parts, pairs * Hkv, groups), tmQ, tmK, tmV, a, (cudaStream_t)stream_);
+}

@@ -276,8 +276,8 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
     (``quant_pages``); ``page_table`` int32 [B, max_pages], ``seq_lens`` int32 [B] (the new row's key included, so
     the row stands at position length - 1; 0: the row's output is zero).  Keys from max(``starts`` (int32 [B]),
     length - window) on are visible.  ``shared``: see ``SharedPrefix``; it goes with neither ``starts`` nor a window.
-    A page outside the cache counts as not visible and sets the device status, as does a length past the page table
-    (which is cut there).  Returns bf16 [B, Hq, D]."""
+    A page outside the cache is read as zeros and sets the device status, as does a length past the page table (which
+    is cut there); on the CPU both raise.  Returns bf16 [B, Hq, D]."""
     B, Hq, D = q.shape
     if kcache.dim() != 4 or kcache.shape != vcache.shape:
         raise ValueError("K and V pages have the same shape [pages, page_size, Hkv, D]")
@@ -343,12 +343,17 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
             if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.prefix_ml.numel() < rows * 2:
                 raise ValueError("the workspace is of smaller shared prefixes")
             k, v, cu = kcache, vcache, None
-            if bits != 16:       # the prefix is expanded once for all its readers; it stays in the L2 cache
-                from .quant_pages import kv_gather_quant
+            if bits != 16 or page < 8 or (_TILE % page and page % _TILE):
+                # integer pages, and pages that no tile is made of: the prefix is expanded once for all its readers
                 cu = torch.zeros(groups + 1, dtype=I32, device=q.device)
-                torch.cumsum(shared.lens, 0, out=cu[1:])
+                torch.cumsum(shared.lens, 0, dtype=I32, out=cu[1:])
                 first = page_table.index_select(0, shared.cu_rows[:-1].clamp(max=B - 1))
-                k, v = kv_gather_quant(kcache, vcache, k_scale, v_scale, first, cu, groups * shared.max_len)
+                if bits == 16:
+                    from .functional import kv_gather
+                    k, v = kv_gather(kcache, vcache, first, cu, groups * shared.max_len)
+                else:
+                    from .quant_pages import kv_gather_quant
+                    k, v = kv_gather_quant(kcache, vcache, k_scale, v_scale, first, cu, groups * shared.max_len)
             N.call("us_scored_prefix", N.ptr(q), q.stride(0), N.ptr(k), pages, N.ptr(v), page, N.ptr(cu), N.ptr(page_table),
                    page_table.shape[1], k.shape[0], B, N.ptr(seq_lens), N.ptr(shared.cu_rows), N.ptr(shared.lens), groups,
                    Hq, Hkv, D, shared.max_rows, scale, rules.cap, N.ptr(rules.slopes), N.ptr(work.prefix_o),
