@@ -6,18 +6,28 @@ F64 = torch.float64
 HALF_STEP = torch.finfo(torch.bfloat16).eps / 2
 
 
-def attend(q, k, v, scale, cap, slopes, p, see):
+def attend(q, k, v, scale, cap, slopes, p, see, steps=None):
     """q [rows, Hq, D], k / v [keys, Hkv, D], p [rows] positions, see [rows, keys] -> (out, bound), both [rows, Hq, D].
 
     bound: a weight is rounded to bf16 once (HALF_STEP of it, so HALF_STEP sum w |v| of the result), the result once
     (HALF_STEP of it).  A score errs by its FP32 sum (D + 8 roundings of sum |q k| scale), by the cap's function (2^-16
-    of the cap, the kernels' own bound) and by its FP32 size; an error e of all scores changes a normalised weight by 2 e."""
+    of the cap, the kernels' own bound) and by its FP32 size; an error e of all scores changes a normalised weight by 2 e.
+
+    steps: (K's, V's) sizes [keys, Hkv, D] of the offset under which integer codes are multiplied (the step of a code times
+    1152 for 8 bits, 72 for 4).  A score is then the sum of D / 16 + 1 products whose running sum is at most sum |q| step,
+    each off by at most 2^-22 of it (the tensor unit keeps FP32 sums and cuts off what is below): (D / 16 + 1) 2^-22
+    sum |q| step.  A result has, in each tile, four products and one correction of at most sum w step, so 5 x 2^-22 of
+    sum w step over all tiles."""
     q, k, v = q.double(), k.double(), v.double()
     share = q.shape[1] // k.shape[1]
     k, v = k.repeat_interleave(share, 1), v.repeat_interleave(share, 1)
     s = torch.einsum("qhd,khd->hqk", q, k) * scale
     err = float((torch.einsum("qhd,khd->hqk", q.abs(), k.abs()) * abs(scale))[:, see].max()) * (q.shape[2] + 8) * 2.0 ** -24 \
         if see.any() else 0.0
+    if steps is not None:
+        ko, vo = (t.double().repeat_interleave(share, 1) for t in steps)
+        if see.any():
+            err += float((torch.einsum("qhd,khd->hqk", q.abs(), ko) * abs(scale))[:, see].max()) * (q.shape[2] / 16 + 1) * 2.0 ** -22
     if cap:
         s = cap * torch.tanh(s / cap)
         err += cap * 2.0 ** -16
@@ -33,7 +43,10 @@ def attend(q, k, v, scale, cap, slopes, p, see):
     v = torch.where(see.any(0)[:, None, None], v, torch.zeros_like(v))   # what nobody sees weighs nothing
     out = torch.einsum("hqk,khd->qhd", w, v)
     mass = torch.einsum("hqk,khd->qhd", w, v.abs())
-    return out, mass * (HALF_STEP + 2 * err + 2.0 ** -20) + out.abs() * HALF_STEP + 1e-30
+    bound = mass * (HALF_STEP + 2 * err + 2.0 ** -20) + out.abs() * HALF_STEP + 1e-30
+    if steps is not None:
+        bound += torch.einsum("hqk,khd->qhd", w, vo) * 5 * 2.0 ** -22
+    return out, bound
 
 
 def unpack(code, scale):
@@ -75,7 +88,12 @@ def decode(q, kc, vc, table, lens, scale, cap=0.0, slopes=None, window=0, starts
         lo = max(n - window if window else 0, int(starts[b]) if starts is not None else 0)
         # keys that are not visible weigh nothing whatever they hold
         k, v = (torch.where((j >= lo)[:, None, None], t, torch.zeros_like(t)) for t in (k, v))
-        o, e = attend(q[b:b + 1], k, v, scale, cap, slopes, torch.tensor([n - 1], device=q.device), (j >= lo)[None])
+        steps = None
+        if ks is not None:
+            offset = 1152.0 if kc.shape[3] == q.shape[2] else 72.0
+            steps = tuple(torch.where((j >= lo)[:, None, None], t, torch.zeros_like(t)) for t in (
+                offset * sc[pages].transpose(1, 2).double().flatten(0, 1)[:n].repeat_interleave(64, -1) for sc in (ks, vs)))
+        o, e = attend(q[b:b + 1], k, v, scale, cap, slopes, torch.tensor([n - 1], device=q.device), (j >= lo)[None], steps)
         outs.append(o[0])
         bounds.append(e[0])
     return torch.stack(outs), torch.stack(bounds)

@@ -7,33 +7,41 @@
 //
 // Bound by the bytes of the keys, so everything serves the stream of loads:
 //
-// * All keys of the launch form one list of tiles ordered by (sequence, key head, tile), cut into one range per SM:
-//   no SM idles behind a long sequence.  A range that starts or ends inside a (sequence, key head) pair leaves that
-//   pair's unnormalised output, maximum and sum in the CTA's slot (0: its first pair, 1: its last); the CTA whose
-//   arrival completes a pair's count folds the slots and puts the count back to zero.
-// * Each of eight warps has its own KW keys of every tile and its own ring of stages, which it fills itself
-//   with 16-byte asynchronous copies: page ids of a tile are one load per lane, a tile ahead of its copies, and no
-//   warp waits for another until a pair ends.  The ring runs on across pairs.
+// * All keys of the launch form one list of tiles ordered by (sequence, key head, tile), cut into one range per warp: no
+//   SM idles behind a long sequence, and no warp waits for another before its range is done.  A warp fills its own
+//   ring of stages (the K rows or the V rows of a tile) with 16-byte asynchronous copies, on across pairs; page ids of
+//   a tile are one load per lane, a tile ahead of its copies.
+// * A pair (sequence, key head) inside one range is written by its warp.  Others leave unnormalised outputs, maxima and
+//   sums: of the pair that a range ends in, in the warp's ring, which is free by then; of one that it only begins in, in the
+//   warp's slot in memory.  At the end all warps of a CTA fold the parts of its pairs, sixteen channels of a pair at a
+//   time, and pairs that go on in other CTAs once more through the CTAs' slots, by the CTA whose arrival completes a
+//   pair's count and puts it back to zero.  (Warps that split every tile between them and met at each pair's end spent a
+//   quarter of the time there.)  Both rounds are one short loop: every instruction of this end is fetched cold, by all
+//   SMs at once, and an unrolled form of it took 15 us where this one takes some 4.
 // * Keys stand on the M side of m16n8k16 products (S^T = K Q^T, O^T = V^T P^T), the query heads of a key head on the
 //   N side: groups of up to 8 heads pay for 8 columns, not for 16 rows, and the softmax has its maximum and sum
 //   per column, three shuffles each.  P^T becomes the B operand by an 8 x 8 transpose in registers (movmatrix).
-// * Integer codes become bf16 exactly (8 bits: (0x4300 | low 7 bits) - (0x4300 | sign bit) = 128 + l - 128 (1 + sign);
-//   4 bits: (0x4300 | u) - 136), three or two and a half instructions per two codes, and never carry a scale: a key's
-//   scales multiply its scores, a value's its probabilities.  Which channel stands in which k slot is free as long as
-//   Q agrees, so bytes and nibbles are taken out of the words as they lie; for V the free order is the order of the
-//   output rows.
+// * Integer codes are multiplied as FP16 numbers 1024 + u or 64 + u, u the code plus 128 or 8, which bit operations form
+//   (a byte in the last bits of 1024, a nibble four bits up in those of 64).  The offset is taken out by products as
+//   well: -offset x Q starts the sums of K, ones x P^T gives the sums that V's outputs have too much, tile by tile.
+//   One and a half (8 bits) or one and three quarters (4 bits) instructions two codes.  (Nibbles in the last bits of
+//   1024 take half an instruction less, but an offset of 344 times their size eats as much of FP32's sums.)  Scales
+//   never touch the codes: a key's
+//   multiply its scores, a value's its probabilities.  Which channel stands in which k slot is free as long as Q
+//   agrees, so bytes and nibbles are taken out of the words as they lie; for V the free order is that of the output.
 //
-// Statistics and outputs are FP32; P (with a value's scale) is rounded to bf16 for its product, at most 2^-9 of each
-// weight.  Keys that are not visible are never loaded (zeros in their place), so nothing in them reaches the result.
+// Statistics and outputs are FP32.  P is rounded once for its product: to bf16 (2^-8 of a weight at most), or, over
+// integer pages, with its value's scale to FP16 (2^-11).  There the weights are held as p s 2^(14 - E), E the exponent
+// of the largest value scale so far: 15 bits above 1 and 24 below, so a value 2^10 times its neighbours' costs them
+// nothing.  Q is divided by the power of two of its largest channel to be FP16 exactly (channels under 2^-14 of that lose
+// bits).  Keys that are not visible are never loaded (zeros in their place): nothing in them reaches the result.
+#include <type_traits>
 #include "include/us_common.cuh"
 #include "include/us_mma.cuh"
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-constexpr int kMaxSeqs = 1024;
-constexpr int kPitch = 68;                  // floats per head in the merge buffer: 8 rows x 4 heads on 32 banks
+constexpr int kMaxSeqs = 704;               // of a launch: what the ring leaves of shared memory
 
 struct DecodeArgs {
   const __nv_bfloat16* q;
@@ -41,7 +49,8 @@ struct DecodeArgs {
   const __nv_bfloat16 *ks, *vs;             // scales of integer pages
   const int *table, *lens, *starts;
   __nv_bfloat16* out;
-  float *part_o, *part_ml;                  // [CTAs][2][16][D], [CTAs][2][16][2]
+  // parts: of warps, one each, then of CTAs, two each (kPart floats a part, see there)
+  float* part;
   int* counters;                            // [B * pairs per sequence], zero between launches
   const float* slopes;
   long long ldq, ldo;
@@ -53,6 +62,7 @@ struct DecodeArgs {
   const float *pre_o, *pre_ml;
   int groups, pairs, parts, blocks_per_part;
   unsigned int* status;
+  uint32_t magic;                           // see bytes_even, nibbles
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -62,7 +72,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {   // 8 x 8 matrix of 16-bit values across the warp
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool there) {
@@ -71,18 +81,41 @@ __device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool there)
 __device__ __forceinline__ void cp4z(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("sub.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
+// c[16 x 8] += a[16 x 16] b[16 x 8] in bf16 or FP16.  Not volatile: products of unlike sums may pass one another.
+__device__ __forceinline__ void mma_b(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t bytes_even(uint32_t x) {   // bytes 0 and 2 as bf16
-  return sub_bf2((x & 0x007f007fu) | 0x43004300u, (x & 0x00800080u) | 0x43004300u);
+__device__ __forceinline__ void mma_h(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t bytes_odd(uint32_t x) { return bytes_even(x >> 8); }
-template <int N>
-__device__ __forceinline__ uint32_t nibbles(uint32_t x) {      // nibbles N and N + 4 as bf16
-  return sub_bf2(((x >> (4 * N)) & 0x000f000fu) | 0x43004300u, 0x43084308u);
+__device__ __forceinline__ uint32_t pack_h(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Bytes 0 and 2, or 1 and 3, of a word of codes plus 128 as 1024 + u; nibbles 0 and 4 of a word of codes plus 8 as 64 + u,
+// for the others the word is shifted.  `magic` (0x64646464, 0x54005400) comes as a kernel argument: as a constant it was
+// moved into a register anew before most of its uses, a third of all instructions.
+__device__ __forceinline__ uint32_t bytes_even(uint32_t x, uint32_t magic) { return __byte_perm(x, magic, 0x4240); }
+__device__ __forceinline__ uint32_t bytes_odd(uint32_t x, uint32_t magic) { return __byte_perm(x, magic, 0x4341); }
+__device__ __forceinline__ uint32_t nibbles(uint32_t x, uint32_t magic) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xEA;" : "=r"(y) : "r"(x), "r"(magic));     // (x & mask) | magic
+  return y;
+}
+constexpr uint32_t kOne = 0x3C003C00u;          // FP16 pairs: 1, -1152 = -(1024 + 128), -72 = -(64 + 8)
+constexpr uint32_t kMinus1152 = 0xE480E480u, kMinus72 = 0xD480D480u;
+__device__ __forceinline__ float power_of_two(int field) {     // 2^(field - 127), field clamped to what a float has
+  return __uint_as_float((uint32_t)min(max(field, 0), 254) << 23);
 }
 
 // A position in the tile list.
@@ -90,16 +123,19 @@ struct Walk {
   int b, hc, t, tiles;
 };
 
-template <int D, int FMT>                   // FMT: bits of a code (16: bf16)
+template <int D, int FMT, int NT>           // FMT: bits of a code (16: bf16)
 struct Shape {
+  // Integer codes take more instructions a byte, and with two warps a scheduler each waits for itself: sixteen warps of
+  // 128 registers where one head tile leaves room for that.
+  static constexpr int kWarps = FMT != 16 && NT == 1 ? 16 : 8;
   static constexpr int kRow = D * FMT / 8;                          // bytes of a cached row
-  static constexpr int kKeys = kRow >= 256 ? 16 : 32;               // keys of a warp's stage
-  static constexpr int kScales = FMT == 16 ? 0 : kKeys * 4;         // bytes of a plane's scales
-  static constexpr int kStage = 2 * kKeys * kRow + 2 * kScales;
-  static constexpr int kRoom = 196608 / kWarps;                     // ring bytes of a warp
-  static constexpr int kStages = kRoom / kStage > 6 ? 6 : kRoom / kStage;
-  static constexpr int kTile = kWarps * kKeys;
+  static constexpr int kKeys = FMT == 16 && kRow <= 128 && NT == 1 ? 64 : 32;   // keys of a warp's part of a tile
+  static constexpr int kScales = FMT == 16 ? 0 : kKeys * 4;
+  static constexpr int kStage = kKeys * kRow + kScales;             // K or V rows of it
+  static constexpr int kRoom = (FMT == 16 ? 196608 : 202752) / kWarps;    // ring bytes of a warp
+  static constexpr int kStages = kRoom / kStage > 8 ? 8 : kRoom / kStage;
   static constexpr int kPieces = kRow / 16;                         // 16-byte pieces of a row
+  static_assert(kStages >= 3, "ring");
 };
 
 template <int PIECES>
@@ -109,26 +145,30 @@ __device__ __forceinline__ int swizzle(int row, int piece) {        // eight row
   else return piece ^ ((row >> 2) & 1);
 }
 
-constexpr int kMergeFloats = kWarps * 8 * kPitch;                   // [warp][8 heads][64 channels + 4]
+// A part of a pair's result (see kPart): where it is, and which pair's, by its first tile.
+struct Part {
+  const float* at;                          // null: none
+  int begin, end, b, hc;
+};
 
-template <int D, int FMT>
+template <int D, int FMT, int NT>
 constexpr size_t shared_bytes() {
-  using S = Shape<D, FMT>;
-  return (size_t)kWarps * S::kStages * S::kStage + kMergeFloats * 4 + (kWarps * 32 + 32) * 4 + (3 * kMaxSeqs + 4) * 4;
+  using S = Shape<D, FMT, NT>;
+  return (size_t)S::kWarps * S::kStages * S::kStage + 32 * sizeof(Part) + 16 + (3 * kMaxSeqs + 4) * 4;   // rings; parts; flags; sequences
 }
 
 template <int D, int FMT, int NT>           // NT: 8-column head tiles (query heads of a key head in one pass: 8 NT)
-__global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const DecodeArgs a) {
-  using S = Shape<D, FMT>;
-  constexpr int KW = S::kKeys, MT = KW / 16, KS = D / 16, G = D / 64;
+__global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_decode_kernel(const DecodeArgs a) {
+  using S = Shape<D, FMT, NT>;
+  constexpr int kWarps = S::kWarps, kThreads = kWarps * 32;
+  constexpr int KW = S::kKeys, MT = KW / 16, KS = D / 16, G = D / 64, KL = KW / 32;
   US_PDL_PROLOGUE();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem + (size_t)warp * S::kStages * S::kStage;
-  float* buf = (float*)(smem + (size_t)kWarps * S::kStages * S::kStage);
-  float* ml = buf + kMergeFloats;           // [warp][16 heads][2]
-  int* flag = (int*)(ml + kWarps * 32);     // [0]: this CTA completes the pair
-  int* pre = flag + 32;                     // tiles before sequence b
+  Part* parts = (Part*)(smem + (size_t)kWarps * S::kStages * S::kStage);  // [warp][2]: begun before its range, ended by it
+  int* flag = (int*)(parts + 32);           // [2] CTAs of its first, last pair if this CTA completes it (else 0), [2] first of them
+  int* pre = flag + 4;                      // tiles before sequence b
   int* first = pre + kMaxSeqs + 4;          // visible keys of sequence b: [first, end)
   int* end = first + kMaxSeqs;
 
@@ -154,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const Decode
     lo = min(lo, hi);
     first[b] = lo;
     end[b] = hi;
-    pre[b + 1] = max(1, (hi - lo + S::kTile - 1) / S::kTile);       // a pair without keys still has its zeros to write
+    pre[b + 1] = max(1, (hi - lo + KW - 1) / KW);       // a pair without keys still has its zeros to write
   }
   if (tid == 0) pre[0] = 0;
   __syncthreads();
@@ -177,29 +217,37 @@ __global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const Decode
   }
   __syncthreads();
   const int total = Hc * pre[B];
-  const int n_cta = min((int)gridDim.x, total), cta = blockIdx.x;
-  if (cta >= n_cta) return;
-  auto range = [&](int c) { return (int)(((long long)c * total) / n_cta); };
-  auto owner = [&](int g) {
-    int c = (int)(((long long)g * n_cta) / total);
-    while (c + 1 < n_cta && range(c + 1) <= g) ++c;
-    while (c > 0 && range(c) > g) --c;
-    return c;
+  // one range of the list a warp; where there are fewer tiles than warps, every CTA has as many warps at work
+  const int ctas = gridDim.x, cta = blockIdx.x;
+  const int active = min(kWarps, (total + ctas - 1) / ctas), workers = min(total, ctas * active);
+  const unsigned long long pace = ((unsigned long long)total << 32) / (unsigned)workers;
+  auto start_of = [&](int k) -> int { return k >= workers ? total : (int)((pace * (unsigned)k) >> 32); };
+  auto worker_of = [&](int g) -> int {
+    int k = min((int)((float)g * ((float)workers / (float)total)), workers - 1);
+    while (k + 1 < workers && start_of(k + 1) <= g) ++k;
+    while (k > 0 && start_of(k) > g) --k;
+    return k;
   };
-  const int g0 = range(cta), g1 = range(cta + 1);
-  Walk load;
-  {
+  const int me0 = cta * active, me1 = min(me0 + active, workers), me = me0 + warp;     // this CTA's ranges, this warp's
+  if (me0 >= workers) return;
+  const bool works = warp < active && me < workers;
+  const int g0 = works ? start_of(me) : total, g1 = works ? start_of(me + 1) : total;
+  // the pair that tile g is in
+  auto find = [&](int g) -> Walk {
+    Walk w;
     int lo = 0, hi = B - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (Hc * pre[mid] <= g0) lo = mid; else hi = mid - 1;
+      if (Hc * pre[mid] <= g) lo = mid; else hi = mid - 1;
     }
-    load.b = lo;
-    load.tiles = pre[lo + 1] - pre[lo];
-    const int r = g0 - Hc * pre[lo];
-    load.hc = r / load.tiles;
-    load.t = r - load.hc * load.tiles;
-  }
+    w.b = lo;
+    w.tiles = pre[lo + 1] - pre[lo];
+    const int r = g - Hc * pre[lo];
+    w.hc = r / w.tiles;
+    w.t = r - w.hc * w.tiles;
+    return w;
+  };
+  Walk load = find(min(g0, total - 1));
   Walk cur = load;
   auto advance = [&](Walk& w) {
     if (++w.t < w.tiles) return;
@@ -210,91 +258,167 @@ __global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const Decode
     if (w.b < B) w.tiles = pre[w.b + 1] - pre[w.b];
   };
 
-  // ---- loads: this warp's keys of a tile into one of its stages ----
-  // the slot (page * page size + offset) of lane's key in the tile at w, -1 where there is none
-  auto slot_of = [&](const Walk& w) -> int {
-    const int j = first[w.b] + w.t * S::kTile + warp * KW + lane;
-    if (lane >= KW || j >= end[w.b]) return -1;
-    const int pi = a.shift >= 0 ? j >> a.shift : j / a.page;
-    const int pg = __ldg(a.table + (long long)w.b * a.max_pages + pi);
-    if ((unsigned)pg >= (unsigned)a.pages) {
-      us_dev_fail(a.status, US_DEV_BOUNDS);
-      return -1;
-    }
-    return pg * a.page + (j - pi * a.page);
-  };
-  int loaded = g0;                          // tiles up to here have been asked for
-  int slot_next = slot_of(load);
-  auto issue = [&](int stage) {
-    if (loaded < g1) {
-      const int slot = slot_next, hk = load.hc / a.chunks;
-      uint8_t* st = ring + stage * S::kStage;
-      const uint32_t kd = (uint32_t)__cvta_generic_to_shared(st), vd = kd + KW * S::kRow;
-      constexpr int kRows = 32 / S::kPieces;       // rows that one instruction of the warp brings
-      const int piece = lane % S::kPieces;
+  // ---- loads: this warp's keys of a tile, K rows into one stage, V rows into the next ----
+  // Place of a key in the cache in units of 16 bytes; kNone where there is nothing to load.
+  constexpr uint32_t kNone = 0xffffffffu;
+  const uint32_t per_slot = (uint32_t)a.Hkv * S::kPieces;
+  auto place_of = [&](const Walk& w, uint32_t (&at)[KL], uint32_t (&spot)[KL]) {    // of key head 0; spot: of its scales
 #pragma unroll
-      for (int i = 0; i < KW / kRows; ++i) {
-        const int r = i * kRows + lane / S::kPieces;
-        const int sl = __shfl_sync(0xffffffffu, slot, r);
-        const long long off = sl < 0 ? 0 : ((long long)sl * a.Hkv + hk) * S::kRow + piece * 16;
-        const uint32_t to = r * S::kRow + swizzle<S::kPieces>(r, piece) * 16;
-        cp16z(kd + to, a.kc + off, sl >= 0);
-        cp16z(vd + to, a.vc + off, sl >= 0);
-      }
-      if constexpr (FMT != 16) {            // 4 bytes of scales a key: two groups, or one beside its neighbour's
-        if (lane < KW) {
-          const int pg = slot < 0 ? 0 : a.shift >= 0 ? slot >> a.shift : slot / a.page;
-          const long long at = (((long long)pg * a.Hkv + hk) * a.page + (slot < 0 ? 0 : slot - pg * a.page)) * G;
-          const uint32_t sd = kd + 2 * KW * S::kRow + lane * 4;
-          cp4z(sd, a.ks + (at & ~1LL), slot >= 0);
-          cp4z(sd + KW * 4, a.vs + (at & ~1LL), slot >= 0);
+    for (int i = 0; i < KL; ++i) {
+      const int j = first[w.b] + w.t * KW + i * 32 + lane;
+      at[i] = kNone;
+      spot[i] = 0;
+      if (j < end[w.b]) {
+        const int pi = a.shift >= 0 ? j >> a.shift : j / a.page;
+        const int pg = __ldg(a.table + (long long)w.b * a.max_pages + pi);
+        if ((unsigned)pg < (unsigned)a.pages) {
+          const uint32_t base = (uint32_t)(pg * a.page), off = (uint32_t)(j - pi * a.page);
+          at[i] = (base + off) * per_slot;
+          if constexpr (FMT != 16) spot[i] = base * (uint32_t)a.Hkv + off;
+        } else {
+          us_dev_fail(a.status, US_DEV_BOUNDS);
         }
       }
-      ++loaded;
-      if (loaded < g1) {
-        advance(load);
-        slot_next = slot_of(load);
+    }
+  };
+  int loaded = g0;                          // tiles whose K rows have been asked for
+  uint32_t next_place[KL], next_spot[KL], place[KL], spot[KL];
+  bool full_now = false, more = true;
+  if (works) place_of(load, next_place, next_spot);
+  // the next stage's copies: V_ROWS: of the tile whose K rows went last; else of the next tile
+  auto issue = [&](auto v_rows, uint32_t to) {
+    constexpr bool kV = decltype(v_rows)::value;
+    if constexpr (!kV) {
+      more = loaded < g1;
+      if (more) {
+        const uint32_t hk = (uint32_t)(a.chunks == 1 ? load.hc : load.hc / a.chunks);
+        bool full = true;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          const bool there = next_place[i] != kNone;
+          full &= there;
+          place[i] = there ? next_place[i] + hk * S::kPieces : kNone;
+          if constexpr (FMT != 16) spot[i] = next_spot[i] + hk * (uint32_t)a.page;
+        }
+        full_now = __all_sync(0xffffffffu, full);
+        ++loaded;
+        if (loaded < g1) {
+          advance(load);
+          place_of(load, next_place, next_spot);
+        }
+      }
+    }
+    if (more) {
+      constexpr int kRows = 32 / S::kPieces;       // rows that one instruction of the warp brings
+      const int piece = lane % S::kPieces, r0 = lane / S::kPieces;
+      const uint8_t* base = (kV ? a.vc : a.kc) + piece * 16;
+      if (full_now) {
+#pragma unroll
+        for (int i = 0; i < KW / kRows; ++i) {
+          const int r = i * kRows + r0;
+          const uint32_t at = __shfl_sync(0xffffffffu, place[i * kRows / 32], r & 31);
+          us::cp16(to + r * S::kRow + swizzle<S::kPieces>(r, piece) * 16, base + (unsigned long long)at * 16);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < KW / kRows; ++i) {
+          const int r = i * kRows + r0;
+          const uint32_t at = __shfl_sync(0xffffffffu, place[i * kRows / 32], r & 31);
+          cp16z(to + r * S::kRow + swizzle<S::kPieces>(r, piece) * 16, base + (at == kNone ? 0ull : (unsigned long long)at * 16), at != kNone);
+        }
+      }
+      if constexpr (FMT != 16) {            // 4 bytes of scales a key: two groups, or one beside its neighbour's
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          const bool there = place[i] != kNone;
+          const uint32_t word = there ? (G == 2 ? spot[i] : spot[i] >> 1) : 0;
+          cp4z(to + KW * S::kRow + (i * 32 + lane) * 4, (const uint8_t*)(kV ? a.vs : a.ks) + (unsigned long long)word * 4, there);
+        }
       }
     }
     us::cp_commit();
   };
 
   const int c4 = lane & 3, r8 = lane >> 2;
+  const uint32_t magic = a.magic;
+  // where this lane's rows of the 8 x 8 matrices of a piece are in a stage (bf16: K's and V's differ in their order)
+  constexpr int kLoads = FMT == 16 ? KS : S::kPieces / 2;
+  uint32_t k_lane[kLoads], v_lane[FMT == 16 ? KS : 1];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    k_lane[i] = (lane & 15) * S::kRow + swizzle<S::kPieces>(lane & 15, 2 * i + (lane >> 4)) * 16;
+    if constexpr (FMT == 16) {
+      const int row = (lane & 7) + (lane >> 4) * 8;
+      v_lane[i] = row * S::kRow + swizzle<S::kPieces>(row, 2 * i + ((lane >> 3) & 1)) * 16;
+    }
+  }
   uint32_t qf[NT][KS][2];
-  float m[NT][2], l[NT][2], bias[NT][2], o[KS][NT][4];
+  float m[NT][2], l[NT][2], bias[NT][2], factor[NT][2], o[KS][NT][4], offset[G][NT][2];
+  int top_scale = 0;                         // exponent field of the largest value scale so far (integer pages)
   auto begin_pair = [&]() {
-    const int hk = cur.hc / a.chunks, chunk = cur.hc - hk * a.chunks;
-    const int share = a.Hq / a.Hkv;
+    const int share = a.Hq / a.Hkv, hk = a.chunks == 1 ? cur.hc : cur.hc / a.chunks, chunk = cur.hc - hk * a.chunks;
+    top_scale = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int gi = chunk * 16 + nt * 8 + r8;
       const __nv_bfloat16* row = a.q + (long long)cur.b * a.ldq + (long long)(hk * share + gi) * D;
       const bool there = gi < share;
+      float back = 1.f;                      // what the head's scores are multiplied by
 #pragma unroll
       for (int k = 0; k < KS; ++k) qf[nt][k][0] = qf[nt][k][1] = 0;
-      if (there) {
-        if constexpr (FMT == 16) {
+      if constexpr (FMT == 16) {
+        if (there) {
 #pragma unroll
           for (int k = 0; k < KS; ++k) {
             qf[nt][k][0] = *reinterpret_cast<const uint32_t*>(row + k * 16 + c4 * 2);
             qf[nt][k][1] = *reinterpret_cast<const uint32_t*>(row + k * 16 + c4 * 2 + 8);
           }
-        } else if constexpr (FMT == 8) {
+        }
+      } else {
+        // bf16 pairs of the slots, then FP16 under the power of two of the head's largest channel
+        if (there) {
+          if constexpr (FMT == 8) {
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            const uint2 w = *reinterpret_cast<const uint2*>(row + k * 16 + c4 * 4);
-            qf[nt][k][0] = __byte_perm(w.x, w.y, 0x5410);
-            qf[nt][k][1] = __byte_perm(w.x, w.y, 0x7632);
-          }
-        } else {
+            for (int k = 0; k < KS; ++k) {
+              const uint2 w = *reinterpret_cast<const uint2*>(row + k * 16 + c4 * 4);
+              qf[nt][k][0] = __byte_perm(w.x, w.y, 0x5410);
+              qf[nt][k][1] = __byte_perm(w.x, w.y, 0x7632);
+            }
+          } else {
 #pragma unroll
-          for (int k = 0; k < KS; k += 2) {
-            const uint4 w = *reinterpret_cast<const uint4*>(row + k * 16 + c4 * 8);
-            qf[nt][k][0] = __byte_perm(w.x, w.z, 0x5410);
-            qf[nt][k][1] = __byte_perm(w.x, w.z, 0x7632);
-            qf[nt][k + 1][0] = __byte_perm(w.y, w.w, 0x5410);
-            qf[nt][k + 1][1] = __byte_perm(w.y, w.w, 0x7632);
+            for (int k = 0; k < KS; k += 2) {
+              const uint4 w = *reinterpret_cast<const uint4*>(row + k * 16 + c4 * 8);
+              qf[nt][k][0] = __byte_perm(w.x, w.z, 0x5410);
+              qf[nt][k][1] = __byte_perm(w.x, w.z, 0x7632);
+              qf[nt][k + 1][0] = __byte_perm(w.y, w.w, 0x5410);
+              qf[nt][k + 1][1] = __byte_perm(w.y, w.w, 0x7632);
+            }
           }
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) most = __vmaxu2(most, __vmaxu2(qf[nt][k][0] & 0x7fff7fffu, qf[nt][k][1] & 0x7fff7fffu));
+        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = (int)(max(most & 0xffffu, most >> 16) >> 7);
+        const bool scaled = e > 0 && e < 254;
+        const float down = scaled ? power_of_two(254 - e) : 1.f;
+        back = scaled ? power_of_two(e) : 1.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t w = qf[nt][k][i];
+            qf[nt][k][i] = pack_h(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
+          }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          constexpr uint32_t kOff = FMT == 8 ? kMinus1152 : kMinus72;
+#pragma unroll
+          for (int k = 4 * g; k < 4 * g + 4; ++k) mma_h(acc, kOff, kOff, kOff, kOff, qf[nt][k][0], qf[nt][k][1]);
+          offset[g][nt][0] = acc[0];
+          offset[g][nt][1] = acc[1];
         }
       }
 #pragma unroll
@@ -303,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const Decode
         m[nt][e] = -INFINITY;
         l[nt][e] = 0.f;
         bias[nt][e] = a.slopes && h < share ? a.slopes[hk * share + h] * 1.4426950408889634f : 0.f;
+        factor[nt][e] = (a.cap_log2 > 0.f ? a.scale_cap : a.scale_log2) * (FMT == 16 ? 1.f : __shfl_sync(0xffffffffu, back, (c4 * 2 + e) * 4));
       }
 #pragma unroll
       for (int i = 0; i < KS; ++i)
@@ -311,119 +436,147 @@ __global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const Decode
     }
   };
 
-  // ---- one stage: S^T = K Q^T, the softmax's step, O^T += V^T P^T ----
-  auto consume = [&](int stage) {
-    const int j0 = first[cur.b] + cur.t * S::kTile + warp * KW, hi = end[cur.b];
+  // a key's scales out of a stage: two, or (64 channels) the one whose half its parity says, the page size being even
+  auto scales = [&](const uint32_t* st, int key, int j0, float (&f)[G]) {
+    const uint32_t w = st[key];
+    if constexpr (G == 2) {
+      f[0] = __uint_as_float(w << 16);
+      f[1] = __uint_as_float(w & 0xffff0000u);
+    } else {
+      f[0] = __uint_as_float((j0 + key) & 1 ? w & 0xffff0000u : w << 16);
+    }
+  };
+
+  float s[MT][NT][4];                        // scores of a tile, then its weights
+  float alpha[NT][2];                        // what the outputs so far are multiplied by
+  bool grown = false;
+  // ---- K rows of a stage: S^T = K Q^T and the softmax's step ----
+  auto consume_k = [&](const uint8_t* st) {
+    const int j0 = first[cur.b] + cur.t * KW, hi = end[cur.b];
     if (j0 >= hi) return;
-    const uint8_t* st = ring + stage * S::kStage;
-    const uint32_t kd = (uint32_t)__cvta_generic_to_shared(st), vd = kd + KW * S::kRow;
-    const uint32_t* sk = reinterpret_cast<const uint32_t*>(st + 2 * KW * S::kRow);
-    const uint32_t* sv = sk + KW;
-    // a key's two scales (64 channels: its one, which is the half that its parity says, the page size being even)
-    auto scales = [&](const uint32_t* s, int key, float (&f)[G]) {
-      const uint32_t w = s[key];
-      if constexpr (G == 2) {
-        f[0] = __uint_as_float(w << 16);
-        f[1] = __uint_as_float(w & 0xffff0000u);
-      } else {
-        f[0] = __uint_as_float((j0 + key) & 1 ? w & 0xffff0000u : w << 16);
-      }
-    };
-    float s[MT][NT][4];
+    const uint32_t kd = (uint32_t)__cvta_generic_to_shared(st);
+    const uint32_t* sk = reinterpret_cast<const uint32_t*>(st + KW * S::kRow);
+    // a piece of channels at a time over all keys: MT sums that do not wait for one another
+    if constexpr (FMT == 16) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float acc[G][NT][4];
-#pragma unroll
-      for (int g = 0; g < G; ++g)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[g][nt][e] = 0.f;
-      const int row = mt * 16 + (lane & 15);
-      if constexpr (FMT == 16) {
+          for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
+      for (int k = 0; k < KS; ++k) {
+        const uint32_t from = kd + k_lane[k];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
           uint32_t f[4];
-          us::ldsm4(f, kd + row * S::kRow + swizzle<S::kPieces>(row, 2 * k + (lane >> 4)) * 16);
+          us::ldsm4(f, from + mt * 16 * S::kRow);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_b(s[mt][nt], f[0], f[1], f[2], f[3], qf[nt][k][0], qf[nt][k][1]);
+        }
+      }
+    } else {
+      float acc[MT][G][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            us::mma16816(acc[0][nt], f[0], f[1], f[2], f[3], qf[nt][k][0], qf[nt][k][1]);
-        }
-      } else {
 #pragma unroll
-        for (int i = 0; i < S::kPieces / 2; ++i) {
+            for (int e = 0; e < 4; ++e) acc[mt][g][nt][e] = offset[g][nt][e & 1];
+#pragma unroll
+      for (int i = 0; i < S::kPieces / 2; ++i) {
+        const uint32_t from = kd + k_lane[i];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
           uint32_t f[4];
-          us::ldsm4(f, kd + row * S::kRow + swizzle<S::kPieces>(row, 2 * i + (lane >> 4)) * 16);
+          us::ldsm4(f, from + mt * 16 * S::kRow);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t x = f[2 * half], y = f[2 * half + 1];   // keys 0 - 7 and 8 - 15
+            uint32_t x = f[2 * half], y = f[2 * half + 1];   // keys 0 - 7 and 8 - 15
             const int piece = 2 * i + half;
             if constexpr (FMT == 8) {
-              const uint32_t a0 = bytes_even(x), a1 = bytes_even(y), a2 = bytes_odd(x), a3 = bytes_odd(y);
+              x ^= 0x80808080u;
+              y ^= 0x80808080u;
+              const uint32_t a0 = bytes_even(x, magic), a1 = bytes_even(y, magic), a2 = bytes_odd(x, magic), a3 = bytes_odd(y, magic);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                us::mma16816(acc[piece / 4][nt], a0, a1, a2, a3, qf[nt][piece][0], qf[nt][piece][1]);
+              for (int nt = 0; nt < NT; ++nt) mma_h(acc[mt][piece / 4][nt], a0, a1, a2, a3, qf[nt][piece][0], qf[nt][piece][1]);
             } else {
-              const uint32_t a0 = nibbles<0>(x), a1 = nibbles<0>(y), a2 = nibbles<1>(x), a3 = nibbles<1>(y);
-              const uint32_t b0 = nibbles<2>(x), b1 = nibbles<2>(y), b2 = nibbles<3>(x), b3 = nibbles<3>(y);
+              const uint32_t a0 = nibbles(x << 4, magic), a1 = nibbles(y << 4, magic), a2 = nibbles(x, magic), a3 = nibbles(y, magic);
+              const uint32_t b0 = nibbles(x >> 4, magic), b1 = nibbles(y >> 4, magic), b2 = nibbles(x >> 8, magic), b3 = nibbles(y >> 8, magic);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                us::mma16816(acc[piece / 2][nt], a0, a1, a2, a3, qf[nt][2 * piece][0], qf[nt][2 * piece][1]);
-                us::mma16816(acc[piece / 2][nt], b0, b1, b2, b3, qf[nt][2 * piece + 1][0], qf[nt][2 * piece + 1][1]);
+                mma_h(acc[mt][piece / 2][nt], a0, a1, a2, a3, qf[nt][2 * piece][0], qf[nt][2 * piece][1]);
+                mma_h(acc[mt][piece / 2][nt], b0, b1, b2, b3, qf[nt][2 * piece + 1][0], qf[nt][2 * piece + 1][1]);
               }
             }
           }
         }
       }
-      if constexpr (FMT == 16) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][nt][e] = acc[0][nt][e];
-      } else {
+      for (int mt = 0; mt < MT; ++mt) {
         float f0[G], f1[G];
-        scales(sk, mt * 16 + r8, f0);
-        scales(sk, mt * 16 + r8 + 8, f1);
+        scales(sk, mt * 16 + r8, j0, f0);
+        scales(sk, mt * 16 + r8 + 8, j0, f1);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x = acc[0][nt][e] * (e < 2 ? f0[0] : f1[0]);
-            if constexpr (G == 2) x = fmaf(acc[1][nt][e], e < 2 ? f0[1] : f1[1], x);
+            float x = acc[mt][0][nt][e] * (e < 2 ? f0[0] : f1[0]);
+            if constexpr (G == 2) x = fmaf(acc[mt][1][nt][e], e < 2 ? f0[1] : f1[1], x);
             s[mt][nt][e] = x;
           }
       }
     }
     // scores in units of log2(e)
-    const int away0 = a.lens[cur.b] - 1 - j0;
-    float top[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      top[nt][0] = top[nt][1] = -INFINITY;
+    if (a.cap_log2 > 0.f) {                  // tanh y = 1 - 2 / (1 + e^(2 y)): off by some 2^-22 of the cap
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = mt * 16 + r8 + (e >> 1) * 8;
-          float x = s[mt][nt][e];
-          if (a.cap_log2 > 0.f) {           // tanh y = 1 - 2 / (1 + e^(2 y)): off by some 2^-23 of the cap
-            x = fmaf(-2.f * a.cap_log2, __frcp_rn(1.f + ex2(x * a.scale_cap)), a.cap_log2);
-          } else {
-            x *= a.scale_log2;
-          }
-          x = fmaf(-bias[nt][e & 1], (float)(away0 - key), x);
-          if (j0 + key >= hi) x = -INFINITY;
-          s[mt][nt][e] = x;
-          top[nt][e & 1] = fmaxf(top[nt][e & 1], x);
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[mt][nt][e] = fmaf(-2.f * a.cap_log2, rcp(1.f + ex2(s[mt][nt][e] * factor[nt][e & 1])), a.cap_log2);
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[mt][nt][e] *= factor[nt][e & 1];
+    }
+    if (a.slopes) {
+      const int away0 = a.lens[cur.b] - 1 - j0 - r8;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float away = (float)(away0 - mt * 16 - h * 8);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[mt][nt][2 * h + e] = fmaf(-bias[nt][e], away, s[mt][nt][2 * h + e]);
         }
     }
-    bool grown = false;
-    float alpha[NT][2];
+    if (j0 + KW > hi) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j0 + mt * 16 + r8 + (e >> 1) * 8 >= hi) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[mt][nt][e] = -INFINITY;
+          }
+    }
+    grown = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float t = top[nt][e];
+        float t = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+#pragma unroll
+        for (int mt = 1; mt < MT; ++mt) t = fmaxf(t, fmaxf(s[mt][nt][e], s[mt][nt][e + 2]));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
@@ -431,80 +584,131 @@ __global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const Decode
         alpha[nt][e] = t == -INFINITY ? 1.f : ex2(m[nt][e] - t);
         grown |= t > m[nt][e];
         m[nt][e] = t;
-      }
-    if (__any_sync(0xffffffffu, grown)) {
+        const float base = t == -INFINITY ? 0.f : t;      // no score above -inf so far: weights of zero
+        float sum = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        l[nt][0] *= alpha[nt][0];
-        l[nt][1] *= alpha[nt][1];
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float p = ex2(s[mt][nt][e + 2 * h] - base);
+            s[mt][nt][e + 2 * h] = p;
+            sum += p;
+          }
+        l[nt][e] = fmaf(l[nt][e], alpha[nt][e], sum);
+      }
+    grown = __any_sync(0xffffffffu, grown);
+  };
+  // ---- V rows of a stage: O^T += V^T P^T ----
+  auto consume_v = [&](const uint8_t* st) {
+    const int j0 = first[cur.b] + cur.t * KW;
+    if (j0 >= end[cur.b]) return;
+    const uint32_t vd = (uint32_t)__cvta_generic_to_shared(st);
+    const uint32_t* sv = reinterpret_cast<const uint32_t*>(st + KW * S::kRow);
+    float lift = 1.f;                        // 2^(14 - E)
+    float shrink = 1.f;
+    if constexpr (FMT != 16) {
+      uint32_t big = 0;                      // scales are not negative: as integers they are in order
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        float f[G];
+        scales(sv, i * 32 + lane, j0, f);
+#pragma unroll
+        for (int g = 0; g < G; ++g) big = max(big, __float_as_uint(f[g]) & 0x7fffffffu);
+      }
+      const int e = max(top_scale, (int)(__reduce_max_sync(0xffffffffu, big) >> 23));
+      shrink = power_of_two(127 - (e - top_scale));
+      top_scale = e;
+      lift = power_of_two(268 - e);
+    }
+    // the weights as the second operand of the products
+    constexpr int GP = FMT == 16 ? 1 : G;
+    uint32_t pb[MT][GP][NT][2];
+    if constexpr (FMT == 16) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          pb[mt][0][nt][0] = transposed(us::pack_bf(s[mt][nt][0], s[mt][nt][1]));
+          pb[mt][0][nt][1] = transposed(us::pack_bf(s[mt][nt][2], s[mt][nt][3]));
+        }
+      if (grown) {
 #pragma unroll
         for (int i = 0; i < KS; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][nt][e] *= alpha[nt][e & 1];
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][nt][e] *= alpha[nt][e & 1];
       }
-    }
+    } else {
+      float sums[G][NT][4];                  // of the rounded weights
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      uint32_t pb[G][NT][2];
-      float f0[G], f1[G];
-      if constexpr (FMT != 16) {
-        scales(sv, mt * 16 + r8, f0);
-        scales(sv, mt * 16 + r8 + 8, f1);
-      }
+      for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = s[mt][nt][e];
-          p[e] = x == -INFINITY ? 0.f : ex2(x - m[nt][e & 1]);
-          l[nt][e & 1] += p[e];
-        }
+          for (int e = 0; e < 4; ++e) sums[g][nt][e] = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float f0[G], f1[G];
+        scales(sv, mt * 16 + r8, j0, f0);
+        scales(sv, mt * 16 + r8 + 8, j0, f1);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          if constexpr (FMT == 16) {
-            if (g == 0) {
-              pb[0][nt][0] = transposed(us::pack_bf(p[0], p[1]));
-              pb[0][nt][1] = transposed(us::pack_bf(p[2], p[3]));
-            }
-          } else {
-            pb[g][nt][0] = transposed(us::pack_bf(p[0] * f0[g], p[1] * f0[g]));
-            pb[g][nt][1] = transposed(us::pack_bf(p[2] * f1[g], p[3] * f1[g]));
+          f0[g] *= lift;
+          f1[g] *= lift;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            pb[mt][g][nt][0] = transposed(pack_h(s[mt][nt][0] * f0[g], s[mt][nt][1] * f0[g]));
+            pb[mt][g][nt][1] = transposed(pack_h(s[mt][nt][2] * f1[g], s[mt][nt][3] * f1[g]));
+            mma_h(sums[g][nt], kOne, kOne, kOne, kOne, pb[mt][g][nt][0], pb[mt][g][nt][1]);
           }
         }
       }
-      if constexpr (FMT == 16) {
-        const int row = mt * 16 + (lane & 7) + (lane >> 4) * 8;
+      // the outputs so far under the new maximum, and less what this tile's offsets will add
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          uint32_t f[4];
-          us::ldsm4t(f, vd + row * S::kRow + swizzle<S::kPieces>(row, 2 * i + ((lane >> 3) & 1)) * 16);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            us::mma16816(o[i][nt], f[0], f[1], f[2], f[3], pb[0][nt][0], pb[0][nt][1]);
+        for (int e = 0; e < 2; ++e) {
+          const float f = alpha[nt][e] * shrink;
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const float less = sums[g][nt][e] * (FMT == 4 ? -72.f : -1152.f);
+#pragma unroll
+            for (int i = 4 * g; i < 4 * g + 4; ++i) {
+              o[i][nt][e] = fmaf(o[i][nt][e], f, less);
+              o[i][nt][e + 2] = fmaf(o[i][nt][e + 2], f, less);
+            }
+          }
         }
-      } else {
-        const int row = mt * 16 + (lane & 15);
+    }
 #pragma unroll
-        for (int i = 0; i < S::kPieces / 2; ++i) {
-          uint32_t f[4];
-          us::ldsm4t(f, vd + row * S::kRow + swizzle<S::kPieces>(row, 2 * i + (lane >> 4)) * 16);
+    for (int i = 0; i < kLoads; ++i) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t f[4];
+        if constexpr (FMT == 16) {
+          us::ldsm4t(f, vd + v_lane[i] + mt * 16 * S::kRow);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_b(o[i][nt], f[0], f[1], f[2], f[3], pb[mt][0][nt][0], pb[mt][0][nt][1]);
+        } else {
+          us::ldsm4t(f, vd + k_lane[i] + mt * 16 * S::kRow);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t x = f[2 * half], y = f[2 * half + 1];   // keys 0 - 7 and 8 - 15
+            uint32_t x = f[2 * half], y = f[2 * half + 1];   // keys 0 - 7 and 8 - 15
             const int piece = 2 * i + half;
             if constexpr (FMT == 8) {
-              const uint32_t a0 = bytes_even(x), a1 = bytes_odd(x), a2 = bytes_even(y), a3 = bytes_odd(y);
+              x ^= 0x80808080u;
+              y ^= 0x80808080u;
+              const uint32_t a0 = bytes_even(x, magic), a1 = bytes_odd(x, magic), a2 = bytes_even(y, magic), a3 = bytes_odd(y, magic);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                us::mma16816(o[piece][nt], a0, a1, a2, a3, pb[piece / 4][nt][0], pb[piece / 4][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) mma_h(o[piece][nt], a0, a1, a2, a3, pb[mt][piece / 4][nt][0], pb[mt][piece / 4][nt][1]);
             } else {
-              const uint32_t a0 = nibbles<0>(x), a1 = nibbles<1>(x), a2 = nibbles<0>(y), a3 = nibbles<1>(y);
-              const uint32_t b0 = nibbles<2>(x), b1 = nibbles<3>(x), b2 = nibbles<2>(y), b3 = nibbles<3>(y);
+              const uint32_t a0 = nibbles(x << 4, magic), a1 = nibbles(x, magic), a2 = nibbles(y << 4, magic), a3 = nibbles(y, magic);
+              const uint32_t b0 = nibbles(x >> 4, magic), b1 = nibbles(x >> 8, magic), b2 = nibbles(y >> 4, magic), b3 = nibbles(y >> 8, magic);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                us::mma16816(o[2 * piece][nt], a0, a1, a2, a3, pb[piece / 2][nt][0], pb[piece / 2][nt][1]);
-                us::mma16816(o[2 * piece + 1][nt], b0, b1, b2, b3, pb[piece / 2][nt][0], pb[piece / 2][nt][1]);
+                mma_h(o[2 * piece][nt], a0, a1, a2, a3, pb[mt][piece / 2][nt][0], pb[mt][piece / 2][nt][1]);
+                mma_h(o[2 * piece + 1][nt], b0, b1, b2, b3, pb[mt][piece / 2][nt][0], pb[mt][piece / 2][nt][1]);
               }
             }
           }
@@ -519,174 +723,355 @@ __global__ void __launch_bounds__(kThreads, 1) scored_decode_kernel(const Decode
     else return (t >> 1) * 32 + r8 * 4 + (t & 1) * 2 + half;
   };
 
-  // folds the partial results of head `gi` of pair (b, hc), channels d and d + 1, that other launches and CTAs left:
-  // slots of CTAs [c0, c1] and the parts of the shared prefix, beside (M, L, x, y)
-  auto fold = [&](int b, int hc, int gi, int d, int c0, int c1, int begin, float M, float L, float x, float y) {
-    const int hk = hc / a.chunks, chunk = hc - hk * a.chunks, share = a.Hq / a.Hkv;
-    int np = 0;
-    long long at = 0;
-    if (a.groups > 0 && b < a.cu_rows[a.groups]) {
-      int g = 0, h = a.groups - 1;
-      while (g < h) {
-        const int mid = (g + h + 1) >> 1;
-        if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
-      }
-      const int blocks = (a.shared[g] + 127) >> 7;
-      np = min((blocks + a.blocks_per_part - 1) / a.blocks_per_part, a.parts);
-      const int per = 128 / share, r = b - a.cu_rows[g];       // sequences of a 128-row tile of the prefix kernel
-      if (blocks > a.parts * a.blocks_per_part || r >= a.pairs * 2 * per) {   // a group larger than the host was told
-        us_dev_fail(a.status, US_DEV_BOUNDS);
-        if (r >= a.pairs * 2 * per) np = 0;
-      }
-      const int tile = r / per, in_tile = (r - tile * per) * share + chunk * 16 + gi;
-      at = ((((long long)g * a.pairs + (tile >> 1)) * a.Hkv + hk) * a.parts) * 256 + (tile & 1) * 128 + in_tile;
+  // the shared prefix's parts of a pair: how many, and the row of the first of them (head 0); the next ones are 256 on
+  auto prefix_parts = [&](int b, int hk, int chunk, long long& at) -> int {
+    if (a.groups == 0 || b >= a.cu_rows[a.groups]) return 0;
+    int g = 0, h = a.groups - 1;
+    while (g < h) {
+      const int mid = (g + h + 1) >> 1;
+      if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
     }
-    auto slot = [&](int c) { return ((long long)c * 2 + (range(c) >= begin ? 0 : 1)) * 16 + gi; };
-    float top = M;
-    for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(a.part_ml + slot(c) * 2));
-    for (int i = 0; i < np; ++i) top = fmaxf(top, __ldcg(a.pre_ml + (at + (long long)i * 256) * 2));
-    float w = M == -INFINITY ? 0.f : ex2(M - top);
-    L *= w;
-    x *= w;
-    y *= w;
-    auto add = [&](const float* mls, const float* os) {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(mls));
-      const float u = v.x == -INFINITY ? 0.f : ex2(v.x - top);
-      const float2 p = __ldcg(reinterpret_cast<const float2*>(os));
-      L = fmaf(u, v.y, L);
-      if (u != 0.f) {          // a part of weight zero may hold anything
-        x = fmaf(u, p.x, x);
-        y = fmaf(u, p.y, y);
-      }
-    };
-    for (int c = c0; c <= c1; ++c) add(a.part_ml + slot(c) * 2, a.part_o + slot(c) * D + d);
-    for (int i = 0; i < np; ++i) add(a.pre_ml + (at + (long long)i * 256) * 2, a.pre_o + (at + (long long)i * 256) * D + d);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    *reinterpret_cast<uint32_t*>(a.out + (long long)b * a.ldo + (long long)(hk * share + chunk * 16 + gi) * D + d) =
-        us::pack_bf(x * inv, y * inv);
+    const int blocks = (a.shared[g] + 127) >> 7, share = a.Hq / a.Hkv;
+    int np = min((blocks + a.blocks_per_part - 1) / a.blocks_per_part, a.parts);
+    const int per = 128 / share, r = b - a.cu_rows[g];       // sequences of a 128-row tile of the prefix kernel
+    if (blocks > a.parts * a.blocks_per_part || r >= a.pairs * 2 * per) {   // a group larger than the host was told
+      us_dev_fail(a.status, US_DEV_BOUNDS);
+      if (r >= a.pairs * 2 * per) np = 0;
+    }
+    const int tile = r / per, in_tile = (r - tile * per) * share + chunk * 16;
+    at = ((((long long)g * a.pairs + (tile >> 1)) * a.Hkv + hk) * a.parts) * 256 + (tile & 1) * 128 + in_tile;
+    return np;
   };
-
-#pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) issue(i);
-  int stage = 0, segment = 0, i = g0;
-  while (i < g1) {
-    begin_pair();
-    const int n = min(cur.tiles - cur.t, g1 - i);
-    const bool whole = cur.t == 0 && n == cur.tiles;
-    for (int t = 0; t < n; ++t, ++i, ++cur.t) {
-      us::cp_wait<S::kStages - 2>();
-      __syncwarp();
-      consume(stage);
-      __syncwarp();
-      issue(stage == 0 ? S::kStages - 1 : stage - 1);    // the stage that the tile before this one has left
-      stage = stage + 1 == S::kStages ? 0 : stage + 1;
-    }
-    // ---- the pair (or this CTA's part of it) ends: the warps' results become one ----
-    const int hk = cur.hc / a.chunks, chunk = cur.hc - hk * a.chunks, share = a.Hq / a.Hkv;
+  // Folds the shared prefix's parts into N accumulator tiles from t0 on (unnormalised, under maximum M with sum L) and
+  // writes them.
+  auto finish = [&](auto tiles, int t0, float (*acc)[NT][4], int b, int hc, float (&M)[NT][2], float (&L)[NT][2]) {
+    constexpr int N = decltype(tiles)::value;
+    const int share = a.Hq / a.Hkv, hk = a.chunks == 1 ? hc : hc / a.chunks, chunk = hc - hk * a.chunks;
     const int heads = min(8 * NT, share - chunk * 16);
+    long long at = 0;
+    const int np = prefix_parts(b, hk, chunk, at);
+    constexpr int kAtOnce = N == 1 ? 4 : 1;  // parts whose loads are in flight together
+    for (int i0 = 0; i0 < np; i0 += kAtOnce) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int h = min(nt * 8 + c4 * 2 + e, heads - 1);
+          float2 v[kAtOnce];
+          float p[kAtOnce][N][2];
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) {
+            const long long row = at + h + (long long)min(i0 + i, np - 1) * 256;
+            v[i] = __ldcg(reinterpret_cast<const float2*>(a.pre_ml + row * 2));
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) p[i][t][half] = __ldcg(a.pre_o + row * D + channel(t0 + t, half));
+          }
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) {
+            if (i0 + i >= np || v[i].x == -INFINITY) continue;       // a part of weight zero may hold anything
+            const float top = fmaxf(M[nt][e], v[i].x), f = M[nt][e] == -INFINITY ? 0.f : ex2(M[nt][e] - top), w = ex2(v[i].x - top);
+            M[nt][e] = top;
+            L[nt][e] = L[nt][e] * f + v[i].y * w;
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) acc[t][nt][e + 2 * half] = fmaf(acc[t][nt][e + 2 * half], f, w * p[i][t][half]);
+          }
+        }
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float t = l[nt][e];
-        t += __shfl_xor_sync(0xffffffffu, t, 4);
-        t += __shfl_xor_sync(0xffffffffu, t, 8);
-        t += __shfl_xor_sync(0xffffffffu, t, 16);
-        if (r8 == 0) {
-          const int h = nt * 8 + c4 * 2 + e;
-          ml[(warp * 16 + h) * 2] = m[nt][e];
-          ml[(warp * 16 + h) * 2 + 1] = t;
+        const int h = nt * 8 + c4 * 2 + e;
+        if (h >= heads) continue;
+        const float inv = L[nt][e] == 0.f ? 0.f : 1.f / L[nt][e];
+        __nv_bfloat16* to = a.out + (long long)b * a.ldo + (long long)(hk * share + chunk * 16 + h) * D;
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) to[channel(t0 + t, half)] = us::f2bf(acc[t][nt][e + 2 * half] * inv);
+      }
+  };
+  // A part: outputs in the order of the accumulators [NT][D / 16][32 lanes][4], then maxima and sums [NT * 8][2].
+  constexpr int kPart = NT * (KS * 128 + 16);
+  static_assert(2 * kPart * 4 <= S::kStages * S::kStage, "two parts have room in a ring");
+  auto store_tile = [&](float* part, int t, const float (&x)[NT][4]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      *reinterpret_cast<float4*>(part + ((nt * KS + t) * 32 + lane) * 4) = make_float4(x[nt][0], x[nt][1], x[nt][2], x[nt][3]);
+  };
+  auto store_sums = [&](float* part, const float (&M)[NT][2], const float (&L)[NT][2]) {
+    if (r8 == 0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        *reinterpret_cast<float4*>(part + NT * KS * 128 + (nt * 8 + c4 * 2) * 2) = make_float4(M[nt][0], L[nt][0], M[nt][1], L[nt][1]);
+    }
+  };
+  auto ring_of = [&](int w) { return (float*)(smem + (size_t)w * S::kStages * S::kStage); };
+  // a value under maximum x into one under M
+  auto join = [&](float x, float& M, float& f, float& w) {
+    const float top = fmaxf(M, x);
+    f = M == -INFINITY ? 0.f : ex2(M - top);
+    w = ex2(x - top);
+    M = top;
+  };
+  // accumulator tile t of up to four parts into acc under maxima M with sums L (a maximum of -inf: no key has a weight)
+  auto add_parts = [&](const float* (&at)[4], int t, float (&acc)[1][NT][4], float (&M)[NT][2], float (&L)[NT][2]) {
+    float4 v[4][NT], p[4][NT];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        v[k][nt] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+        if (at[k]) {
+          v[k][nt] = *reinterpret_cast<const float4*>(at[k] + NT * KS * 128 + nt * 16 + c4 * 4);
+          p[k][nt] = *reinterpret_cast<const float4*>(at[k] + ((nt * KS + t) * 32 + lane) * 4);
         }
       }
-    __syncthreads();
-    const long long slot0 = ((long long)cta * 2 + (segment == 0 ? 0 : 1)) * 16;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f, w;
+        if (v[k][nt].x != -INFINITY) {
+          join(v[k][nt].x, M[nt][0], f, w);
+          L[nt][0] = fmaf(w, v[k][nt].y, L[nt][0] * f);
+          acc[0][nt][0] = fmaf(w, p[k][nt].x, acc[0][nt][0] * f);
+          acc[0][nt][2] = fmaf(w, p[k][nt].z, acc[0][nt][2] * f);
+        }
+        if (v[k][nt].z != -INFINITY) {
+          join(v[k][nt].z, M[nt][1], f, w);
+          L[nt][1] = fmaf(w, v[k][nt].w, L[nt][1] * f);
+          acc[0][nt][1] = fmaf(w, p[k][nt].y, acc[0][nt][1] * f);
+          acc[0][nt][3] = fmaf(w, p[k][nt].w, acc[0][nt][3] * f);
+        }
+      }
+  };
+  // a whole part
+  auto add_part = [&](const float* part, float (*acc)[NT][4], float (&M)[NT][2], float (&L)[NT][2]) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float w[2];
+      const float4 v = *reinterpret_cast<const float4*>(part + NT * KS * 128 + nt * 16 + c4 * 4);
+      float4 p[KS];
+#pragma unroll
+      for (int t = 0; t < KS; ++t) p[t] = *reinterpret_cast<const float4*>(part + ((nt * KS + t) * 32 + lane) * 4);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int h = nt * 8 + c4 * 2 + e;
-        float top = ml[h * 2];
+        const float x = e ? v.z : v.x;
+        if (x == -INFINITY) continue;
+        float f, w;
+        join(x, M[nt][e], f, w);
+        L[nt][e] = fmaf(w, e ? v.w : v.y, L[nt][e] * f);
 #pragma unroll
-        for (int k = 1; k < kWarps; ++k) top = fmaxf(top, ml[(k * 16 + h) * 2]);
-        w[e] = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - top);
-      }
-#pragma unroll
-      for (int g = 0; g < G; ++g) {          // 64 channels of eight heads at a time
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const int t = g * 4 + i4;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            buf[(warp * 8 + c4 * 2 + (e & 1)) * kPitch + channel(t, e >> 1) - g * 64] = w[e & 1] == 0.f ? 0.f : o[t][nt][e] * w[e & 1];
+        for (int t = 0; t < KS; ++t) {
+          acc[t][nt][e] = fmaf(w, e ? p[t].y : p[t].x, acc[t][nt][e] * f);
+          acc[t][nt][e + 2] = fmaf(w, e ? p[t].w : p[t].z, acc[t][nt][e + 2] * f);
         }
-        __syncthreads();
-        const int h8 = tid >> 5, d = (tid & 31) * 2, h = nt * 8 + h8;
-        if (h < heads) {
-          float top = ml[h * 2];
-#pragma unroll
-          for (int k = 1; k < kWarps; ++k) top = fmaxf(top, ml[(k * 16 + h) * 2]);
-          float x = 0.f, y = 0.f, L = 0.f;
-#pragma unroll
-          for (int k = 0; k < kWarps; ++k) {
-            const float2 v = *reinterpret_cast<const float2*>(buf + (k * 8 + h8) * kPitch + d);
-            x += v.x;
-            y += v.y;
-            const float mk = ml[(k * 16 + h) * 2];
-            L += mk == -INFINITY ? 0.f : ml[(k * 16 + h) * 2 + 1] * ex2(mk - top);
-          }
-          if (whole) {
-            fold(cur.b, cur.hc, h, g * 64 + d, 1, 0, 0, top, L, x, y);
-          } else {
-            *reinterpret_cast<float2*>(a.part_o + (slot0 + h) * D + g * 64 + d) = make_float2(x, y);
-            if (g == 0 && (tid & 31) == 0)
-              *reinterpret_cast<float2*>(a.part_ml + (slot0 + h) * 2) = make_float2(top, L);
-          }
-        }
-        __syncthreads();
       }
     }
-    if (!whole) {
-      __threadfence();
-      __syncthreads();
-      const int begin = Hc * pre[cur.b] + cur.hc * cur.tiles;
-      const int c0 = owner(begin), c1 = owner(begin + cur.tiles - 1);
-      if (tid == 0) {
-        int* count = a.counters + cur.b * Hc + cur.hc;
-        const int last = atomicAdd(count, 1) == c1 - c0;
-        if (last) *count = 0;
-        flag[0] = last;
-      }
-      __syncthreads();
-      if (flag[0]) {
-        __threadfence();
-        for (int e = tid; e < heads * (D / 2); e += kThreads)
-          fold(cur.b, cur.hc, e / (D / 2), (e % (D / 2)) * 2, c0, c1, begin, -INFINITY, 0.f, 0.f, 0.f);
-      }
-      __syncthreads();
+  };
+
+  // ---- this warp's range ----
+  constexpr int NS = S::kStages;
+  using KRows = std::false_type;
+  using VRows = std::true_type;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  if (tid < 32) parts[tid].at = nullptr;
+  __syncthreads();
+  if (works) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if (i & 1) issue(VRows{}, ring_at + i * S::kStage);
+      else issue(KRows{}, ring_at + i * S::kStage);
     }
-    ++segment;
-    --cur.t;                                 // the loop above left it one past the pair's last tile
-    advance(cur);
+    int stage = 0, i = g0, done = 0;
+    const int paced = total / workers, present = me1 - me0;
+    auto step = [&]() { stage = stage + 1 == NS ? 0 : stage + 1; };
+    while (i < g1) {
+      begin_pair();
+      const int n = min(cur.tiles - cur.t, g1 - i);
+      const bool from_start = cur.t == 0, to_end = cur.t + n == cur.tiles;
+      for (int t = 0; t < n; ++t, ++i, ++cur.t) {
+        us::cp_wait<NS - 1>();
+        __syncwarp();
+        consume_k(ring + stage * S::kStage);
+        __syncwarp();
+        // the freed stage gets what comes NS stages later: K rows if NS is even, else V rows
+        if constexpr (NS % 2 == 0) issue(KRows{}, ring_at + stage * S::kStage);
+        else issue(VRows{}, ring_at + stage * S::kStage);
+        step();
+        us::cp_wait<NS - 1>();
+        __syncwarp();
+        consume_v(ring + stage * S::kStage);
+        __syncwarp();
+        if constexpr (NS % 2 == 0) issue(VRows{}, ring_at + stage * S::kStage);
+        else issue(KRows{}, ring_at + stage * S::kStage);
+        step();
+        // bf16: in step (every range has at least `paced` tiles), or the scheduler's favourites are done a tenth earlier
+        // than the rest, whose loads alone do not fill the memory (64 x 4240 keys: 105 -> 102 us).  Integer pages
+        // are bound by instructions, and waiting costs them 8 us there.
+        if (FMT == 16 && ++done < paced && (done & 3) == 0) asm volatile("bar.sync 1, %0;" ::"r"(present * 32) : "memory");
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
+          l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
+          l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
+        }
+      if constexpr (FMT != 16) {
+        const float unit = power_of_two(top_scale - 14);
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][nt][e] *= unit;
+      }
+      if (from_start && to_end) {
+        finish(std::integral_constant<int, KS>{}, 0, o, cur.b, cur.hc, m, l);
+      } else {
+        const bool last = i == g1;           // every stage has been read, and no copy is under way
+        float* part = last ? ring_of(warp) : a.part + (long long)me * kPart;
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < KS; ++t) store_tile(part, t, o[t]);
+        store_sums(part, m, l);
+        if (lane == 0) parts[2 * warp + last] = Part{part, i - cur.t, i - cur.t + cur.tiles, cur.b, cur.hc};
+      }
+      --cur.t;                               // the loop above left it one past the pair's last tile
+      advance(cur);
+    }
+  }
+
+  // ---- pairs in several ranges: first this CTA's parts of them, then those that it completes, of all CTAs ----
+  const int G0 = start_of(me0), G1 = start_of(me1);
+  float* cta_parts = a.part + (long long)ctas * kWarps * kPart;       // of CTA c: 2 c (its first pair), 2 c + 1 (its last)
+  Part cut[2];                               // the pair that began before this CTA, the one that goes on behind it
+  cut[0].at = cut[1].at = nullptr;
+  for (int round = 0;; ++round) {
+    __syncthreads();
+    const Part mine = parts[lane];
+    uint32_t left = __ballot_sync(0xffffffffu, mine.at != nullptr);
+    int item = warp;                         // of KS accumulator tiles a pair, one a warp in turn
+    while (left) {
+      const Part pair = parts[__ffs(left) - 1];
+      const uint32_t run = __ballot_sync(0xffffffffu, mine.at != nullptr && mine.begin == pair.begin);
+      left &= ~run;
+      const bool here = round == 1 || (pair.begin >= G0 && pair.end <= G1);
+      if (!here) cut[pair.begin < G0 ? 0 : 1] = pair;
+      for (; item < KS; item += kWarps) {
+        float acc[1][NT][4], M[NT][2], L[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[0][nt][e] = 0.f;
+            M[nt][e & 1] = -INFINITY;
+            L[nt][e & 1] = 0.f;
+          }
+#pragma unroll 1
+        for (uint32_t u = run; u;) {         // four parts in flight
+          const float* at[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            at[k] = u ? parts[__ffs(u) - 1].at : nullptr;
+            u &= u - 1;
+          }
+          add_parts(at, item, acc, M, L);
+        }
+        if (here) {
+          finish(std::integral_constant<int, 1>{}, item, acc, pair.b, pair.hc, M, L);
+        } else {
+          float* part = cta_parts + ((long long)cta * 2 + (pair.begin < G0 ? 0 : 1)) * kPart;
+          store_tile(part, item, acc[0]);
+          if (item == 0) store_sums(part, M, L);
+        }
+      }
+      item -= KS;
+    }
+    if (round == 1 || (!cut[0].at && !cut[1].at)) return;
+    __threadfence();
+    __syncthreads();
+    if (tid < 2) {
+      const Part p = tid ? cut[1] : cut[0];
+      int n = 0;
+      if (p.at) {
+        const int c0 = worker_of(p.begin) / active, c1 = worker_of(p.end - 1) / active;
+        int* count = a.counters + p.b * Hc + p.hc;
+        if (atomicAdd(count, 1) == c1 - c0) {
+          *count = 0;
+          n = c1 - c0 + 1;
+        }
+        flag[2 + tid] = c0;
+      }
+      flag[tid] = n;
+    }
+    __syncthreads();
+    const int n0 = flag[0], n1 = flag[1];
+    if (n0 + n1 == 0) return;
+    __threadfence();
+    auto part_of = [&](int c, int begin) { return cta_parts + ((long long)c * 2 + (start_of(c * active) > begin ? 0 : 1)) * kPart; };
+    if (n0 + n1 <= 8) {
+      if (warp == 0) {
+        const int x = lane < n0 ? 0 : 1;
+        Part p = x ? cut[1] : cut[0];
+        p.at = lane < n0 + n1 ? part_of(flag[2 + x] + lane - (x ? n0 : 0), p.begin) : nullptr;
+        parts[lane] = p;
+      }
+      continue;
+    }
+    // parts of more CTAs: every warp first sums its share of them into its ring (a part's loads take a microsecond)
+    if (tid < 32) parts[tid].at = nullptr;
+    __syncthreads();
+#pragma unroll 1
+    for (int x = 0; x < 2; ++x) {
+      const int n = x ? n1 : n0;
+      if (warp >= n) continue;
+      Part p = x ? cut[1] : cut[0];
+      float* part = ring_of(warp) + x * kPart;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          m[nt][e & 1] = -INFINITY;
+          l[nt][e & 1] = 0.f;
+#pragma unroll
+          for (int t = 0; t < KS; ++t) o[t][nt][e] = 0.f;
+        }
+#pragma unroll 1
+      for (int k = warp; k < n; k += kWarps) add_part(part_of(flag[2 + x] + k, p.begin), o, m, l);
+#pragma unroll
+      for (int t = 0; t < KS; ++t) store_tile(part, t, o[t]);
+      store_sums(part, m, l);
+      p.at = part;
+      if (lane == 0) parts[2 * warp + x] = p;
+    }
   }
 }
 
 template <int D, int FMT, int NT>
 int launch(const DecodeArgs& a, int ctas, cudaStream_t stream) {
-  const size_t bytes = shared_bytes<D, FMT>();
-  static_assert(shared_bytes<D, FMT>() <= 232448, "shared memory");
+  const size_t bytes = shared_bytes<D, FMT, NT>();
+  static_assert(shared_bytes<D, FMT, NT>() <= 232448, "shared memory");
   US_CUDA_CHECK((us::allow_shared<scored_decode_kernel<D, FMT, NT>>((int)bytes)));
-  US_CUDA_CHECK(us::launch_pdl(scored_decode_kernel<D, FMT, NT>, dim3(ctas), dim3(kThreads), bytes, stream, a));
+  US_CUDA_CHECK(us::launch_pdl(scored_decode_kernel<D, FMT, NT>, dim3(ctas), dim3(Shape<D, FMT, NT>::kWarps * 32), bytes, stream, a));
   return US_OK;
 }
 
 }  // namespace
 
-// Bytes of the partial results of a launch on the current device (its counters: B * Hkv * ceil(Hq / Hkv / 16) int32).
+// Bytes of the partial results of a launch on the current device: a part for each of the 8 warps (of 16 heads) or 16 warps
+// (of 8), two for each CTA.  (Its counters: B * Hkv * ceil(Hq / Hkv / 16) int32.)
 US_API long long us_scored_decode_scratch(int D) {
   int sms = 0;
   if (us::sm_count(&sms) != cudaSuccess) return -1;
-  return (long long)sms * 2 * 16 * (D + 2) * (long long)sizeof(float);
+  const long long two = (8 + 2) * 2, one = (16 + 2) * 1;
+  return (long long)sms * (two > one ? two : one) * (D * 8 + 16) * (long long)sizeof(float);
 }
 
 // q [B, Hq, D] bf16 (row pitch ldq); pages [pages, page, Hkv, D] bf16 or integer codes with scales (bits 8, 4; 16: bf16);
@@ -704,6 +1089,7 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   US_REQUIRE(q && kc && vc && table && lens && out && scratch && counters && max_pages >= 1 && pages >= 1 && page >= 1);
   US_REQUIRE(bits == 16 || ((bits == 8 || bits == 4) && ks && vs && page % 2 == 0 && (((uintptr_t)ks | (uintptr_t)vs) % 4) == 0));
   US_REQUIRE((long long)pages * page <= 0x7fffffffLL && window >= 0 && cap >= 0.f);
+  if ((long long)pages * page * Hkv * (D * bits / 128) >= 0xffffffffLL) return US_ERR_LIMIT;   // places are 32 bits of 16 bytes
   US_REQUIRE((ldq % 8) == 0 && (ldo % 2) == 0 && (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) % 16) == 0 &&
              ((uintptr_t)out % 4) == 0);
   const int share = Hq / Hkv;
@@ -721,8 +1107,7 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   a.out = (__nv_bfloat16*)out;
   int sms = 0;
   US_CUDA_CHECK(us::sm_count(&sms));
-  a.part_o = (float*)scratch;
-  a.part_ml = (float*)scratch + (long long)sms * 2 * 16 * D;
+  a.part = (float*)scratch;
   a.counters = counters;
   a.slopes = slopes;
   a.ldq = ldq;
@@ -749,6 +1134,7 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   a.parts = parts;
   a.blocks_per_part = blocks_per_part;
   a.status = us_status_ptr();
+  a.magic = bits == 8 ? 0x64646464u : 0x54005400u;
   cudaStream_t stream = (cudaStream_t)stream_;
 #define US_SCORED(DD, F)                                                                   \
   if (D == DD && bits == F) return share <= 8 ? launch<DD, F, 1>(a, sms, stream) : launch<DD, F, 2>(a, sms, stream)

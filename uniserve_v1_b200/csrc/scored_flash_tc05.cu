@@ -40,7 +40,7 @@ constexpr int kHalf = 128 * 128;              // bytes of 64 columns of a tile
 constexpr float kRescaleThreshold = 8.f;      // log2 units
 constexpr int kMaxBlocks = 8192;              // key blocks of a sequence
 constexpr int kWords = kMaxBlocks / 32;
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;                 // two warpgroups of softmax rows; loads, products and two idle warps
 constexpr float kPolyReach = 0.75f;           // of the cap
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -239,7 +239,10 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
   }
 
-  if (taken_a + taken_b > 0) {
+  // 384 threads are launched with 168 registers each (64,512); a row of scores wants more, the other roles less
+  // (256 x 208 + 128 x 80 = 63,488)
+  if (taken_a + taken_b > 0 && warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == kTmaWarp) {
       // ---------------------------------------------------------------- loads --
       // The whole warp walks; lane 0 loads whole tiles, or every lane its page of a tile.
@@ -378,8 +381,11 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         us_dev_fail(a.status, US_DEV_TIMEOUT_FULL);
         *abort_flag = 1;
       }
-    } else {
+    }
+  } else if (taken_a + taken_b > 0) {
+    {
       // -------------------------------------------------------------- softmax --
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
       const int x = warp >> 2, r = (warp & 3) * 32 + lane;
       const uint32_t lane_addr = ((uint32_t)((warp & 3) * 32) << 16);
       const uint32_t s_tmem = tmem_base + (uint32_t)x * kBN + lane_addr;

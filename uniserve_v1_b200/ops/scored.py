@@ -33,7 +33,7 @@ N.register_signatures({
     "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
 })
 
-MAX_SEQS = 1024            # sequences of one decode launch; larger batches go in slices
+MAX_SEQS = 704             # sequences of one decode launch; larger batches go in slices
 MAX_KEYS = 1 << 20         # keys of a prompt's sequence
 _TILE = 128                # rows of a tile, keys of a block of the prompt kernel
 
