@@ -26,6 +26,7 @@
 // A shared prefix: rows of a tile are (sequence, query head of the key head) pairs of one group, the keys come through
 // the page list of the group's first row (or packed), split into `parts` of the blocks; unnormalised outputs, maxima and
 // sums go to the workspace.  Every wait is bounded.
+#include <type_traits>
 #include "include/us_common.cuh"
 #include "include/us_flash.cuh"
 #include "include/us_tc05.cuh"
@@ -54,6 +55,7 @@ struct ScoredArgs {
   const float* slopes;
   float scale_log2;
   float poly[4], reach, scale_cap, cap_log2;  // cap: x = s (p0 + p1 s^2 + ...) where |s| <= reach
+  float base;                                 // what stands for every row's maximum under a small cap
   // shared prefixes
   const int *table, *lens, *cu_rows, *shared, *cu_shared;
   int max_pages, pages, page, batch, pairs, parts, blocks_per_part;
@@ -89,20 +91,21 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return hi <= lo ? 0u : (0xffffffffu >> (32 - (hi - lo))) << lo;
 }
 
-// The blocks that a CTA walks, in order.
+// The blocks that a CTA walks, the last first: under a distance bias a row's largest scores are beside it, and a maximum
+// that is found first makes no output be scaled again.
 struct Blocks {
   const uint32_t* bits;     // [kWords] of tile A, then of tile B
-  int word, words;
+  int word;
   uint32_t left;
-  __device__ __forceinline__ Blocks(const uint32_t* b, int n) : bits(b), word(0), words(n), left(n > 0 ? b[0] | b[kWords] : 0) {}
+  __device__ __forceinline__ Blocks(const uint32_t* b, int words) : bits(b), word(words - 1), left(words > 0 ? b[words - 1] | b[kWords + words - 1] : 0) {}
   // the next block, and whether the tiles take part in it; -1 at the end
   __device__ __forceinline__ int next(bool& a, bool& b) {
     while (left == 0) {
-      if (++word >= words) return -1;
+      if (--word < 0) return -1;
       left = bits[word] | bits[kWords + word];
     }
-    const int i = __ffs(left) - 1;
-    left &= left - 1;
+    const int i = 31 - __clz(left);
+    left ^= 1u << i;
     a = (bits[word] >> i) & 1u;
     b = (bits[kWords + word] >> i) & 1u;
     return word * 32 + i;
@@ -110,7 +113,8 @@ struct Blocks {
 };
 
 // MODE 0: prompts.  1: shared prefixes.
-template <int kD, bool CAP, bool BIAS, int MODE, uint32_t EMU>
+// FIXED: no running maximum (see set_rules).  EMU: which of every eight exponential pairs go to the polynomial.
+template <int kD, bool CAP, bool BIAS, bool FIXED, int MODE, uint32_t EMU>
 __global__ void __launch_bounds__(kThreads, 1)
 scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const ScoredArgs a) {
@@ -122,11 +126,11 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   int seq, h = 0, hk, q0, q_start = 0, q_len, k_start, kv_len, shift = 0, per = kBM, pre = 0, part = 0;
   long long prow0 = 0;
   if constexpr (MODE == 0) {
-    seq = blockIdx.z;
-    h = blockIdx.y;
+    seq = blockIdx.y;
+    h = blockIdx.x;
     hk = h / share;
-    // under a causal mask the last rows walk the most blocks: they start first
-    q0 = (a.causal ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x) * 2 * kBM;
+    // under a causal mask the last rows walk the most blocks: those of all heads and sequences start first
+    q0 = (a.causal ? (int)gridDim.z - 1 - (int)blockIdx.z : (int)blockIdx.z) * 2 * kBM;
     q_start = a.cu_q[seq];
     q_len = min(a.cu_q[seq + 1], a.Tq) - q_start;
     k_start = a.cu_k[seq];
@@ -174,7 +178,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint32_t* bits = tmem_slot + 4;      // [2][kWords]
 
   if (tid == 0) {
-    tc::mbar_init(q_full, 1);
+    tc::mbar_init(q_full, 2);          // Q, and the first block's K
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&kv_full[i], 1);
       tc::mbar_init(&kv_empty[i], 1);
@@ -185,6 +189,16 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
     *abort_flag = 0;
     tc::mbar_fence_init();
+    // Q is on its way while the blocks are looked up
+    tc::mbar_expect_tx(q_full, MODE == 0 ? 2 * kTile : 2 * kHalves * per * share * 128);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int hf = 0; hf < kHalves; ++hf) {
+        uint8_t* to = sQ + x * kTile + hf * kHalf;
+        if constexpr (MODE == 0) tc::tma_load_2d(to, &tmQ, q_full, h * kD + 64 * hf, q_start + q0 + x * kBM);
+        else tc::tma_load_3d(to, &tmQ, q_full, 64 * hf, hk * share, q_start + q0 + x * per);
+      }
   }
   if (warp == kMmaWarp) {
     tc::tmem_alloc(tmem_slot, 512);
@@ -241,7 +255,12 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 
   // 384 threads are launched with 168 registers each (64,512); a row of scores wants more, the other roles less
   // (256 x 208 + 128 x 80 = 63,488)
-  if (taken_a + taken_b > 0 && warp >= 8) {
+  if (taken_a + taken_b == 0) {        // nothing is seen: Q has to have landed before the CTA ends
+    if (tid == 0) {
+      tc::mbar_arrive(q_full);
+      if (!tc::mbar_wait(q_full, 0, abort_flag)) us_dev_fail(a.status, US_DEV_TIMEOUT_FULL);
+    }
+  } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == kTmaWarp) {
       // ---------------------------------------------------------------- loads --
@@ -272,21 +291,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       bool ta, tb;
       int j = walk.next(ta, tb);
       int row = row_of(j);
-      const uint32_t q_bytes = MODE == 0 ? 2 * kTile : 2 * kHalves * per * share * 128;
-      if (lane == 0) {
-        tc::tma_prefetch_desc(&tmQ);
-        tc::tma_prefetch_desc(&tmK);
-        tc::tma_prefetch_desc(&tmV);
-        tc::mbar_expect_tx(q_full, q_bytes + kTile);
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int hf = 0; hf < kHalves; ++hf) {
-            uint8_t* to = sQ + x * kTile + hf * kHalf;
-            if constexpr (MODE == 0) tc::tma_load_2d(to, &tmQ, q_full, h * kD + 64 * hf, q_start + q0 + x * kBM);
-            else tc::tma_load_3d(to, &tmQ, q_full, 64 * hf, hk * share, q_start + q0 + x * per);
-          }
-      }
+      if (lane == 0) tc::mbar_expect_tx(q_full, kTile);
       __syncwarp();
       load_tile(sK, &tmK, q_full, row);
       for (int e = 0; j >= 0; ++e) {
@@ -382,7 +387,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         *abort_flag = 1;
       }
     }
-  } else if (taken_a + taken_b > 0) {
+  } else {
     {
       // -------------------------------------------------------------- softmax --
       asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -427,34 +432,38 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         c2 = pack2(a.poly[2], a.poly[2]);
         c3 = pack2(a.poly[3], a.poly[3]);
       }
-      float m_used = -INFINITY, l_sum = 0.f;
+      // FIXED: what is taken for the maximum.  A row before the first key (p < 0, no causal mask) has all keys at least -p
+      // away: that much bias is common to all.
+      const float base = FIXED ? a.base - (BIAS && p < 0 ? sl * (float)-p : 0.f) : 0.f;
+      float m_used = FIXED ? base : -INFINITY, m_next = m_used, l_sum = 0.f;
       Blocks walk(bits, words);
       int n = 0;
       bool ok = true;
       while (ok) {
-        bool mine, other;
+        bool mine;
         int j;
         do {
           bool ta, tb;
           j = walk.next(ta, tb);
           mine = x ? tb : ta;
         } while (j >= 0 && !mine);
-        (void)other;
         if (j < 0) break;
         if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_full[x], (uint32_t)n & 1u, abort_flag))) { ok = false; break; }
         tc::tc_fence_after_sync();
         uint32_t v[kBN];
+        auto fetch = [&]() {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+          for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+        };
+        fetch();
         const int kbase = (jb + j) * kBN;
         // what of the block is visible to the row
-        const bool whole = (lo <= kbase && hi >= kbase + kBN) || pr >= kbase + kBN;
-        bool mixed = false;
+        bool whole = (lo <= kbase && hi >= kbase + kBN) || pr >= kbase + kBN;
         if (MODE == 0 && ranges) {
           const int2 d = ranges[j];
-          mixed = d.x != doc || d.y != doc;
+          whole &= d.x == doc && d.y == doc;
         }
-        const bool masked = __any_sync(0xffffffffu, !whole || mixed);
+        const bool masked = __any_sync(0xffffffffu, !whole);
         uint32_t see[4];
         if (masked) {
 #pragma unroll
@@ -480,89 +489,11 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
           }
         }
-        tc::tmem_ld_wait();
-        // v: raw scores, or with a cap or a bias scores in units of log2(e)
-        const int delta = p - kbase;
-        if (CAP || BIAS) {
-          bool poly = true;
-          if (CAP) {
-            float big[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 32; i += 2)
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                big[c] = max3_abs(big[c], __uint_as_float(v[32 * c + i]), __uint_as_float(v[32 * c + i + 1]));
-            // (a comparison that a NaN fails: such a block takes the other form, which passes it on)
-            poly = __all_sync(0xffffffffu, fabsf(fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]))) <= a.reach);
-            if (!poly) {
-#pragma unroll
-              for (int i = 0; i < kBN; ++i)   // tanh y = 1 - 2 / (1 + e^(2 y))
-                v[i] = __float_as_uint(fmaf(-2.f * a.cap_log2, rcpf(1.f + ex2f(__uint_as_float(v[i]) * a.scale_cap)), a.cap_log2));
-            }
-          }
-          if (BIAS && __any_sync(0xffffffffu, delta > 0 && delta < kBN - 1)) {
-            // keys on both sides of some row
-#pragma unroll
-            for (int i = 0; i < kBN; ++i) {
-              const float bias = -sl * fabsf((float)(delta - i));
-              const float s = __uint_as_float(v[i]);
-              if (CAP && poly) {
-                const float w = s * s;
-                v[i] = __float_as_uint(fmaf(s, fmaf(fmaf(fmaf(a.poly[3], w, a.poly[2]), w, a.poly[1]), w, a.poly[0]), bias));
-              } else {
-                v[i] = __float_as_uint(CAP ? s + bias : fmaf(s, a.scale_log2, bias));
-              }
-            }
-          } else if (BIAS || poly) {
-            const float step = delta > 0 ? sl : -sl, at = -sl * fabsf((float)delta);
-            unsigned long long b2[4];
-            const unsigned long long st2 = pack2(2.f * step, 2.f * step);
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              b2[c] = BIAS ? pack2(fmaf(step, 32.f * c, at), fmaf(step, 32.f * c + 1.f, at)) : 0ull;
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint32_t& e0 = v[32 * c + i];
-                uint32_t& e1 = v[32 * c + i + 1];
-                const unsigned long long s2 = pack2(__uint_as_float(e0), __uint_as_float(e1));
-                unsigned long long y;
-                if (CAP && poly) {
-                  const unsigned long long w = mul2(s2, s2);
-                  y = fma2(fma2(fma2(c3, w, c2), w, c1), w, c0);
-                  y = BIAS ? fma2(s2, y, b2[c]) : mul2(s2, y);
-                } else {
-                  y = CAP ? add2(s2, b2[c]) : fma2(s2, sc2, b2[c]);
-                }
-                if (BIAS) b2[c] = add2(b2[c], st2);
-                float y0, y1;
-                unpack2(y, y0, y1);
-                e0 = __float_as_uint(y0);
-                e1 = __float_as_uint(y1);
-              }
-            }
-          }
-        }
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((see[c] >> i) & 1u)) v[32 * c + i] = 0xff800000u;
-        }
-        float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 32; i += 2)
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            mxs[c] = max3(mxs[c], __uint_as_float(v[32 * c + i]), __uint_as_float(v[32 * c + i + 1]));
-        const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
-        const float m_new = fmaxf(m_used, (CAP || BIAS) ? mx : mx * a.scale_log2);
-        if (__any_sync(0xffffffffu, m_new - m_used > kRescaleThreshold || (m_used == -INFINITY && m_new > -INFINITY))) {
+        // O_X under another maximum.  It is still: this block's S was issued after the last block's product, by the same
+        // thread.
+        auto rescale = [&](float m_new) {
           const float alpha = m_used == -INFINITY ? 0.f : ex2f(m_used - m_new);
           if (n > 0) {
-            // O_X is still: this block's S was issued after the last block's product, by the same thread
 #pragma unroll 1
             for (int c = 0; c < kD; c += 32) {
               uint32_t w[32];
@@ -575,16 +506,30 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           }
           l_sum *= alpha;
           m_used = m_new;
+        };
+        tc::tmem_ld_wait();
+        if (!FIXED && __any_sync(0xffffffffu, m_next - m_used > kRescaleThreshold)) rescale(m_next);
+        const int delta = p - kbase;
+        // Whether the row's scores are cap's polynomial's.  (A comparison that a NaN fails: such a block takes the other
+        // form, which passes it on.)
+        bool poly = true;
+        if (CAP) {
+          float big[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              big[c] = max3_abs(big[c], __uint_as_float(v[32 * c + i]), __uint_as_float(v[32 * c + i + 1]));
+          poly = __all_sync(0xffffffffu, fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) <= a.reach);
         }
-        const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-        const unsigned long long nm2 = pack2(neg_m, neg_m);
+        // Keys on both sides of some row: magnitudes.  (Keys behind a row that it does not see need none: a causal row's bias
+        // is a line.)
+        const bool sides = BIAS && __any_sync(0xffffffffu, max(hi, pr) > p + 1 && delta > 0 && delta < kBN - 1);
         unsigned long long ls[4] = {0ull, 0ull, 0ull, 0ull};
         uint32_t pk[kBN / 2];
-        auto exp_pair = [&](uint32_t s0, uint32_t s1, unsigned long long& l, bool poly) -> uint32_t {
-          const unsigned long long s2 = pack2(__uint_as_float(s0), __uint_as_float(s1));
-          float t0, t1, p0, p1;
-          unpack2((CAP || BIAS) ? add2(s2, nm2) : fma2(s2, sc2, nm2), t0, t1);
-          if (poly) {
+        auto weigh = [&](float t0, float t1, unsigned long long& l, bool emulate) -> uint32_t {
+          float p0, p1;
+          if (emulate) {
             ex2_poly2(t0, t1, p0, p1);
           } else {
             p0 = ex2f(t0);
@@ -594,18 +539,94 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           const __nv_bfloat162 t = __floats2bfloat162_rn(p0, p1);
           return *reinterpret_cast<const uint32_t*>(&t);
         };
-        if (EMU != 0 && !masked) {
+        // One pass from scores to weights, so that the FMA pipe's polynomials and the special-function unit's exponentials
+        // run side by side.  Without a fixed base the maximum is that of the blocks before: bf16 and FP32 have room for
+        // what exceeds it, and the next block starts from this one's.
+        bool through = false;
+        auto pass = [&](auto with_mask) {
+          constexpr bool MASK = decltype(with_mask)::value;
+          const float less = FIXED ? -base : m_used == -INFINITY ? 0.f : -m_used;
+          const float step = delta > 0 ? sl : -sl, at = BIAS ? fmaf(-sl, fabsf((float)delta), less) : less;
+          unsigned long long b2[4];
+          const unsigned long long st2 = pack2(2.f * step, 2.f * step);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2)
+          for (int c = 0; c < 4; ++c) b2[c] = BIAS ? pack2(fmaf(step, 32.f * c, at), fmaf(step, 32.f * c + 1.f, at)) : pack2(at, at);
+          float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              pk[16 * c + (i >> 1)] = exp_pair(v[32 * c + i], v[32 * c + i + 1], ls[c], (EMU >> (((i >> 1) & 1) * 4 + c)) & 1u);
-        } else {
+          for (int i = 0; i < 32; i += 2) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2)
+            for (int c = 0; c < 4; ++c) {
+              const unsigned long long s2 = pack2(__uint_as_float(v[32 * c + i]), __uint_as_float(v[32 * c + i + 1]));
+              unsigned long long y;
+              if (CAP) {
+                const unsigned long long w = mul2(s2, s2);
+                y = fma2(s2, fma2(fma2(fma2(c3, w, c2), w, c1), w, c0), b2[c]);
+              } else {
+                y = fma2(s2, sc2, b2[c]);
+              }
+              if (BIAS) b2[c] = add2(b2[c], st2);
+              float t0, t1;
+              unpack2(y, t0, t1);
+              if (MASK) {
+                if (!((see[c] >> i) & 1u)) t0 = -INFINITY;
+                if (!((see[c] >> (i + 1)) & 1u)) t1 = -INFINITY;
+              }
+              if (!FIXED) mxs[c] = max3(mxs[c], t0, t1);
+              pk[16 * c + (i >> 1)] = weigh(t0, t1, ls[c], !MASK && ((EMU >> (((i >> 1) & 1) * 4 + c)) & 1u));
+            }
+          }
+          if (!FIXED) {
+            const float over = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));     // of the maximum so far
+            through = __all_sync(0xffffffffu, over <= 64.f);
+            m_next = fmaxf(m_used, m_used + over);
+          } else {
+            through = true;
+          }
+        };
+        if ((FIXED || (!CAP && n > 0 && __all_sync(0xffffffffu, m_used > -INFINITY))) && poly && !sides) {
+          if (masked) pass(std::true_type{});
+          else pass(std::false_type{});
+        }
+        if (!through) {
+          // the general form: scores in units of log2(e) less the base, masks, the maximum, weights
+          if (!FIXED && !CAP && n > 0) {     // (the scores were weighed and are wanted again)
+            fetch();
+            tc::tmem_ld_wait();
+          }
+          const float at = (float)delta;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              pk[16 * c + (i >> 1)] = exp_pair(v[32 * c + i], v[32 * c + i + 1], ls[c], false);
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float s = __uint_as_float(v[32 * c + i]);
+              if (CAP) {                     // tanh y = 1 - 2 / (1 + e^(2 y))
+                s = fmaf(-2.f * a.cap_log2, rcpf(1.f + ex2f(s * a.scale_cap)), a.cap_log2 - base);
+              } else {
+                s *= a.scale_log2;
+              }
+              if (BIAS) s = fmaf(-sl, fabsf(at - (float)(32 * c + i)), s);
+              if (masked && !((see[c] >> i) & 1u)) s = -INFINITY;
+              v[32 * c + i] = __float_as_uint(s);
+            }
+          if (!FIXED) {
+            float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                mxs[c] = max3(mxs[c], __uint_as_float(v[32 * c + i]), __uint_as_float(v[32 * c + i + 1]));
+            const float m_new = fmaxf(m_used, fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])));
+            if (__any_sync(0xffffffffu, m_new > m_used)) rescale(m_new);
+            m_next = m_used;
+          }
+          const float less = FIXED || m_used == -INFINITY ? 0.f : m_used;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            ls[c] = 0ull;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              pk[16 * c + (i >> 1)] = weigh(__uint_as_float(v[32 * c + i]) - less, __uint_as_float(v[32 * c + i + 1]) - less, ls[c], false);
+          }
         }
         {
           float s0, s1;
@@ -699,28 +720,35 @@ void set_rules(ScoredArgs& a, float scale, float cap, const float* slopes) {
     a.reach = mag > 1e-4 && mag < 1e4 ? (float)(kPolyReach / mag) : -1.f;
     a.scale_cap = (float)(2.0 * k * kLog2e);
     a.cap_log2 = cap * kLog2e;
+    a.base = a.cap_log2 > 40.f ? a.cap_log2 - 40.f : 0.f;      // weights in [2^(-cap_log2 - base), 2^40]
   }
 }
+// Caps under which weights need no maximum: the smallest one is above 2^-121.
+bool small_cap(const ScoredArgs& a) { return a.cap_log2 + a.base <= 120.f; }
 
-template <int D, bool CAP, bool BIAS, int MODE>
+template <int D, bool CAP, bool BIAS, bool FIXED, int MODE>
 int start(dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ScoredArgs& a, cudaStream_t stream) {
-  // 64-wide heads have half the tensor work per exponential: a quarter of them on the FMA pipe (flash_attn2_tc05.cu)
-  constexpr uint32_t kEmu = D == 64 && !CAP ? 0x21u : 0u;
+  // Exponentials on the FMA pipe: an eighth (no cap: 187 -> 179 us at 4096 causal rows x 32 heads), a quarter for 64-wide
+  // heads, which have half the tensor work per exponential (275 -> 253 us); with a cap that pipe has enough to do (none:
+  // 189 us, an eighth: 193).
+  constexpr uint32_t kEmu = CAP ? 0u : D == 64 ? 0x21u : 0x01u;
   const size_t bytes = shared_bytes(D);
-  US_CUDA_CHECK((us::allow_shared<scored_flash_kernel<D, CAP, BIAS, MODE, kEmu>>((int)bytes)));
-  US_CUDA_CHECK(us::launch_pdl(scored_flash_kernel<D, CAP, BIAS, MODE, kEmu>, grid, dim3(kThreads), bytes, stream, q, k, v, a));
+  US_CUDA_CHECK((us::allow_shared<scored_flash_kernel<D, CAP, BIAS, FIXED, MODE, kEmu>>((int)bytes)));
+  US_CUDA_CHECK(us::launch_pdl(scored_flash_kernel<D, CAP, BIAS, FIXED, MODE, kEmu>, grid, dim3(kThreads), bytes, stream, q, k, v, a));
   return US_OK;
+}
+template <int D, int MODE>
+int start_any(bool cap, dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ScoredArgs& a,
+              cudaStream_t stream) {
+  const bool bias = a.slopes != nullptr;
+  if (!cap) return bias ? start<D, false, true, false, MODE>(grid, q, k, v, a, stream) : start<D, false, false, false, MODE>(grid, q, k, v, a, stream);
+  if (small_cap(a)) return bias ? start<D, true, true, true, MODE>(grid, q, k, v, a, stream) : start<D, true, false, true, MODE>(grid, q, k, v, a, stream);
+  return bias ? start<D, true, true, false, MODE>(grid, q, k, v, a, stream) : start<D, true, false, false, MODE>(grid, q, k, v, a, stream);
 }
 template <int MODE>
 int start_any(int D, bool cap, dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ScoredArgs& a,
               cudaStream_t stream) {
-  const bool bias = a.slopes != nullptr;
-  if (D == 128) {
-    if (cap) return bias ? start<128, true, true, MODE>(grid, q, k, v, a, stream) : start<128, true, false, MODE>(grid, q, k, v, a, stream);
-    return bias ? start<128, false, true, MODE>(grid, q, k, v, a, stream) : start<128, false, false, MODE>(grid, q, k, v, a, stream);
-  }
-  if (cap) return bias ? start<64, true, true, MODE>(grid, q, k, v, a, stream) : start<64, true, false, MODE>(grid, q, k, v, a, stream);
-  return bias ? start<64, false, true, MODE>(grid, q, k, v, a, stream) : start<64, false, false, MODE>(grid, q, k, v, a, stream);
+  return D == 128 ? start_any<128, MODE>(cap, grid, q, k, v, a, stream) : start_any<64, MODE>(cap, grid, q, k, v, a, stream);
 }
 
 }  // namespace
@@ -731,7 +759,7 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
                            long long ldo, const int* cu_q, const int* cu_k, int n, int Tq, int Tk, int Hq, int Hkv, int D,
                            int max_q, int max_k, float scale, float cap, const float* slopes, int causal, int window,
                            const int* docs, const int* prefix, void* ranges, void* stream_) {
-  US_REQUIRE(q && k && v && out && cu_q && cu_k && n >= 1 && n <= 65535 && Tq >= 1 && Tk >= 1 && max_q >= 1 && max_k >= 0);
+  US_REQUIRE(q && k && v && out && cu_q && cu_k && n >= 1 && n <= 65535 && Tq >= 1 && Tk >= 1 && max_q >= 1 && max_q <= 65535 * 2 * kBM && max_k >= 0);
   US_REQUIRE((D == 64 || D == 128) && Hkv >= 1 && Hq >= 1 && Hq <= 65535 && Hq % Hkv == 0 && window >= 0 && cap >= 0.f);
   US_REQUIRE(((ldq | ldk | ldv | ldo) % 8) == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16) == 0);
   US_REQUIRE(!docs || ranges);
@@ -760,7 +788,7 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   set_rules(a, scale, cap, slopes);
   if (docs && max_k > 0)
     US_CUDA_CHECK(us::launch_pdl(doc_ranges_kernel, dim3(((max_k + kBN - 1) / kBN + 3) / 4, n), dim3(128), 0, stream, docs, cu_k, Tk, (int2*)ranges));
-  return start_any<0>(D, cap > 0.f, dim3((max_q + 2 * kBM - 1) / (2 * kBM), Hq, n), tmQ, tmK, tmV, a, stream);
+  return start_any<0>(D, cap > 0.f, dim3(Hq, n, (max_q + 2 * kBM - 1) / (2 * kBM)), tmQ, tmK, tmV, a, stream);
 }
 
 // The part that the shared prefixes of a decode batch have in its attention (scored_decode.cu): rows
