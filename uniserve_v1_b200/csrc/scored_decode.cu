@@ -56,11 +56,11 @@ struct DecodeArgs {
   long long ldq, ldo;
   int B, Hq, Hkv, chunks, max_pages, pages, page, shift, window;
   float scale_log2, scale_cap, cap_log2;    // cap_log2 == 0: no cap; scale_cap = 2 scale log2(e) / cap
-  // shared prefixes: rows [cu_rows[g], cu_rows[g + 1]) share their first shared[g] keys, whose partial results are
-  // pre_o / pre_ml [group][tile pair][key head][part][256][D or 2]
+  // shared prefixes: rows [cu_rows[g], cu_rows[g + 1]) share their first shared[g] keys, which are not this launch's; its
+  // results then go unnormalised to own_o [B][Hq][D], own_ml [B][Hq][2] for scored_merge_kernel
   const int *cu_rows, *shared;
-  const float *pre_o, *pre_ml;
-  int groups, pairs, parts, blocks_per_part;
+  float *own_o, *own_ml;
+  int groups;
   unsigned int* status;
   uint32_t magic;                           // see bytes_even, nibbles
 };
@@ -162,7 +162,9 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
   using S = Shape<D, FMT, NT>;
   constexpr int kWarps = S::kWarps, kThreads = kWarps * 32;
   constexpr int KW = S::kKeys, MT = KW / 16, KS = D / 16, G = D / 64, KL = KW / 32;
-  US_PDL_PROLOGUE();
+  // beside the launch of the shared prefixes, which waited for what both read before it let this one start
+  if (a.groups > 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  else US_PDL_PROLOGUE();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem + (size_t)warp * S::kStages * S::kStage;
@@ -723,72 +725,29 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
     else return (t >> 1) * 32 + r8 * 4 + (t & 1) * 2 + half;
   };
 
-  // the shared prefix's parts of a pair: how many, and the row of the first of them (head 0); the next ones are 256 on
-  auto prefix_parts = [&](int b, int hk, int chunk, long long& at) -> int {
-    if (a.groups == 0 || b >= a.cu_rows[a.groups]) return 0;
-    int g = 0, h = a.groups - 1;
-    while (g < h) {
-      const int mid = (g + h + 1) >> 1;
-      if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
-    }
-    const int blocks = (a.shared[g] + 127) >> 7, share = a.Hq / a.Hkv;
-    int np = min((blocks + a.blocks_per_part - 1) / a.blocks_per_part, a.parts);
-    const int per = 128 / share, r = b - a.cu_rows[g];       // sequences of a 128-row tile of the prefix kernel
-    if (blocks > a.parts * a.blocks_per_part || r >= a.pairs * 2 * per) {   // a group larger than the host was told
-      us_dev_fail(a.status, US_DEV_BOUNDS);
-      if (r >= a.pairs * 2 * per) np = 0;
-    }
-    const int tile = r / per, in_tile = (r - tile * per) * share + chunk * 16;
-    at = ((((long long)g * a.pairs + (tile >> 1)) * a.Hkv + hk) * a.parts) * 256 + (tile & 1) * 128 + in_tile;
-    return np;
-  };
-  // Folds the shared prefix's parts into N accumulator tiles from t0 on (unnormalised, under maximum M with sum L) and
-  // writes them.
-  auto finish = [&](auto tiles, int t0, float (*acc)[NT][4], int b, int hc, float (&M)[NT][2], float (&L)[NT][2]) {
+  // writes N accumulator tiles from t0 on (unnormalised, under maximum M with sum L)
+  auto finish = [&](auto tiles, int t0, float (*acc)[NT][4], int b, int hc, const float (&M)[NT][2], const float (&L)[NT][2]) {
     constexpr int N = decltype(tiles)::value;
     const int share = a.Hq / a.Hkv, hk = a.chunks == 1 ? hc : hc / a.chunks, chunk = hc - hk * a.chunks;
     const int heads = min(8 * NT, share - chunk * 16);
-    long long at = 0;
-    const int np = prefix_parts(b, hk, chunk, at);
-    constexpr int kAtOnce = N == 1 ? 4 : 1;  // parts whose loads are in flight together
-    for (int i0 = 0; i0 < np; i0 += kAtOnce) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int h = min(nt * 8 + c4 * 2 + e, heads - 1);
-          float2 v[kAtOnce];
-          float p[kAtOnce][N][2];
-#pragma unroll
-          for (int i = 0; i < kAtOnce; ++i) {
-            const long long row = at + h + (long long)min(i0 + i, np - 1) * 256;
-            v[i] = __ldcg(reinterpret_cast<const float2*>(a.pre_ml + row * 2));
-#pragma unroll
-            for (int t = 0; t < N; ++t)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) p[i][t][half] = __ldcg(a.pre_o + row * D + channel(t0 + t, half));
-          }
-#pragma unroll
-          for (int i = 0; i < kAtOnce; ++i) {
-            if (i0 + i >= np || v[i].x == -INFINITY) continue;       // a part of weight zero may hold anything
-            const float top = fmaxf(M[nt][e], v[i].x), f = M[nt][e] == -INFINITY ? 0.f : ex2(M[nt][e] - top), w = ex2(v[i].x - top);
-            M[nt][e] = top;
-            L[nt][e] = L[nt][e] * f + v[i].y * w;
-#pragma unroll
-            for (int t = 0; t < N; ++t)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) acc[t][nt][e + 2 * half] = fmaf(acc[t][nt][e + 2 * half], f, w * p[i][t][half]);
-          }
-        }
-    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int h = nt * 8 + c4 * 2 + e;
         if (h >= heads) continue;
+        const int head = hk * share + chunk * 16 + h;
+        if (a.groups > 0) {
+          const long long row = (long long)b * a.Hq + head;
+#pragma unroll
+          for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) a.own_o[row * D + channel(t0 + t, half)] = acc[t][nt][e + 2 * half];
+          if (t0 == 0 && r8 == 0) *reinterpret_cast<float2*>(a.own_ml + row * 2) = make_float2(M[nt][e], L[nt][e]);
+          continue;
+        }
         const float inv = L[nt][e] == 0.f ? 0.f : 1.f / L[nt][e];
-        __nv_bfloat16* to = a.out + (long long)b * a.ldo + (long long)(hk * share + chunk * 16 + h) * D;
+        __nv_bfloat16* to = a.out + (long long)b * a.ldo + (long long)head * D;
 #pragma unroll
         for (int t = 0; t < N; ++t)
 #pragma unroll
@@ -1054,6 +1013,75 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
   }
 }
 
+// Rows of a batch with shared prefixes: what the decode launch left of a row and the parts of its group's prefix.
+struct MergeArgs {
+  const float *own_o, *own_ml, *pre_o, *pre_ml;     // pre: [group][tile pair][key head][part][256 rows][D and 2]
+  const int *cu_rows, *shared;
+  __nv_bfloat16* out;
+  long long ldo;
+  int B, Hq, Hkv, groups, pairs, parts, blocks_per_part;
+  unsigned int* status;
+};
+
+// A warp a row (sequence, query head): 4 or 2 channels a lane, all parts' loads in flight together.  Bound by latency: 64
+// rows of 32 heads with 9 parts are 10 MB out of the L2 cache.
+template <int D>
+__global__ void __launch_bounds__(256) scored_merge_kernel(const MergeArgs a) {
+  constexpr int kC = D / 32;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.B * a.Hq) return;
+  const int b = row / a.Hq, head = row - b * a.Hq, share = a.Hq / a.Hkv, hk = head / share;
+  float acc[kC];
+#pragma unroll
+  for (int c = 0; c < kC; ++c) acc[c] = a.own_o[(long long)row * D + lane * kC + c];
+  float M = a.own_ml[row * 2], L = a.own_ml[row * 2 + 1];
+  if (M == -INFINITY) {          // no key of it has a weight
+    L = 0.f;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) acc[c] = 0.f;
+  }
+  if (b < a.cu_rows[a.groups]) {
+    int g = 0, h = a.groups - 1;
+    while (g < h) {
+      const int mid = (g + h + 1) >> 1;
+      if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
+    }
+    const int blocks = (a.shared[g] + 127) >> 7;
+    int np = min((blocks + a.blocks_per_part - 1) / a.blocks_per_part, a.parts);
+    const int per = 128 / share, r = b - a.cu_rows[g];       // sequences of a 128-row tile of the prefix kernel
+    if (blocks > a.parts * a.blocks_per_part || r >= a.pairs * 2 * per) {   // a group larger than the host was told
+      us_dev_fail(a.status, US_DEV_BOUNDS);
+      if (r >= a.pairs * 2 * per) np = 0;
+    }
+    const int tile = r / per, in_tile = (r - tile * per) * share + head - hk * share;
+    const long long at = ((((long long)g * a.pairs + (tile >> 1)) * a.Hkv + hk) * a.parts) * 256 + (tile & 1) * 128 + in_tile;
+    for (int i0 = 0; i0 < np; i0 += 8) {
+      float2 v[8];
+      float p[8][kC];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long long from = at + (long long)min(i0 + i, np - 1) * 256;
+        v[i] = *reinterpret_cast<const float2*>(a.pre_ml + from * 2);
+#pragma unroll
+        for (int c = 0; c < kC; ++c) p[i][c] = a.pre_o[from * D + lane * kC + c];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= np || v[i].x == -INFINITY || v[i].y == 0.f) continue;   // a part of weight zero may hold anything
+        const float top = fmaxf(M, v[i].x), f = M == -INFINITY ? 0.f : ex2(M - top), w = ex2(v[i].x - top);
+        M = top;
+        L = fmaf(w, v[i].y, L * f);
+#pragma unroll
+        for (int c = 0; c < kC; ++c) acc[c] = fmaf(w, p[i][c], acc[c] * f);
+      }
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  __nv_bfloat16* to = a.out + (long long)b * a.ldo + (long long)head * D + lane * kC;
+#pragma unroll
+  for (int c = 0; c < kC; c += 2) *reinterpret_cast<uint32_t*>(to + c) = us::pack_bf(acc[c] * inv, acc[c + 1] * inv);
+}
+
 template <int D, int FMT, int NT>
 int launch(const DecodeArgs& a, int ctas, cudaStream_t stream) {
   const size_t bytes = shared_bytes<D, FMT, NT>();
@@ -1077,13 +1105,14 @@ US_API long long us_scored_decode_scratch(int D) {
 // q [B, Hq, D] bf16 (row pitch ldq); pages [pages, page, Hkv, D] bf16 or integer codes with scales (bits 8, 4; 16: bf16);
 // table [B, max_pages], lens [B], starts [B] or null.  scratch, counters: see above; counters are zero before the first
 // call and left zero; calls that share them are ordered on the device.  groups > 0: the keys below shared[g] of rows
-// [cu_rows[g], cu_rows[g + 1]) are in pre_o / pre_ml (us_scored_flash), whose layout the last arguments give.
+// [cu_rows[g], cu_rows[g + 1]) are in pre_o / pre_ml by us_scored_prefix, the launch before this one on the stream, and
+// own_o, own_ml ([B][Hq][D and 2] floats) take the rest until both are joined.
 US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const void* vc, const void* ks, const void* vs,
                             const int* table, int max_pages, const int* lens, const int* starts, void* out, long long ldo,
                             void* scratch, int* counters, int B, int Hq, int Hkv, int D, int bits, int pages, int page,
                             int window, float scale, float cap, const float* slopes, int groups, const int* cu_rows,
-                            const int* shared, const float* pre_o, const float* pre_ml, int pairs, int parts,
-                            int blocks_per_part, void* stream_) {
+                            const int* shared, const float* pre_o, const float* pre_ml, float* own_o, float* own_ml, int pairs,
+                            int parts, int blocks_per_part, void* stream_) {
   US_REQUIRE(B >= 0 && B <= kMaxSeqs && (D == 64 || D == 128) && Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0);
   if (B == 0) return US_OK;
   US_REQUIRE(q && kc && vc && table && lens && out && scratch && counters && max_pages >= 1 && pages >= 1 && page >= 1);
@@ -1093,7 +1122,7 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   US_REQUIRE((ldq % 8) == 0 && (ldo % 2) == 0 && (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) % 16) == 0 &&
              ((uintptr_t)out % 4) == 0);
   const int share = Hq / Hkv;
-  if (groups > 0) US_REQUIRE(cu_rows && shared && pre_o && pre_ml && pairs >= 1 && parts >= 1 && blocks_per_part >= 1 && share <= 128 &&
+  if (groups > 0) US_REQUIRE(cu_rows && shared && pre_o && pre_ml && own_o && own_ml && pairs >= 1 && parts >= 1 && blocks_per_part >= 1 && share <= 128 &&
                              window == 0 && !starts);
   DecodeArgs a = {};
   a.q = (const __nv_bfloat16*)q;
@@ -1128,16 +1157,14 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   a.groups = groups;
   a.cu_rows = cu_rows;
   a.shared = shared;
-  a.pre_o = pre_o;
-  a.pre_ml = pre_ml;
-  a.pairs = pairs;
-  a.parts = parts;
-  a.blocks_per_part = blocks_per_part;
+  a.own_o = own_o;
+  a.own_ml = own_ml;
   a.status = us_status_ptr();
   a.magic = bits == 8 ? 0x64646464u : 0x54005400u;
   cudaStream_t stream = (cudaStream_t)stream_;
+  int rc = US_ERR_UNSUPPORTED;
 #define US_SCORED(DD, F)                                                                   \
-  if (D == DD && bits == F) return share <= 8 ? launch<DD, F, 1>(a, sms, stream) : launch<DD, F, 2>(a, sms, stream)
+  if (D == DD && bits == F) rc = share <= 8 ? launch<DD, F, 1>(a, sms, stream) : launch<DD, F, 2>(a, sms, stream)
   US_SCORED(64, 16);
   US_SCORED(64, 8);
   US_SCORED(64, 4);
@@ -1145,5 +1172,28 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   US_SCORED(128, 8);
   US_SCORED(128, 4);
 #undef US_SCORED
-  return US_ERR_UNSUPPORTED;
+  if (rc || groups == 0) return rc;
+  MergeArgs m;
+  m.own_o = own_o;
+  m.own_ml = own_ml;
+  m.pre_o = pre_o;
+  m.pre_ml = pre_ml;
+  m.cu_rows = cu_rows;
+  m.shared = shared;
+  m.out = (__nv_bfloat16*)out;
+  m.ldo = ldo;
+  m.B = B;
+  m.Hq = Hq;
+  m.Hkv = Hkv;
+  m.groups = groups;
+  m.pairs = pairs;
+  m.parts = parts;
+  m.blocks_per_part = blocks_per_part;
+  m.status = a.status;
+  // plain stream order: both launches before it are complete (the decode launch does not wait for the prefix's)
+  const int rows = B * Hq;
+  if (D == 64) scored_merge_kernel<64><<<(rows + 7) / 8, 256, 0, stream>>>(m);
+  else scored_merge_kernel<128><<<(rows + 7) / 8, 256, 0, stream>>>(m);
+  US_LAUNCH_CHECK();
+  return US_OK;
 }

@@ -118,7 +118,12 @@ template <int kD, bool CAP, bool BIAS, bool FIXED, int MODE, uint32_t EMU>
 __global__ void __launch_bounds__(kThreads, 1)
 scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const ScoredArgs a) {
-  US_PDL_PROLOGUE();
+  if (MODE == 0) {
+    US_PDL_PROLOGUE();
+  } else {       // the launch behind this one (scored_decode.cu) does not wait: it may start once what both read is there
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  }
   constexpr int kHalves = kD / 64, kTile = kHalves * kHalf;
   constexpr int kTmaWarp = 8, kMmaWarp = 9;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;

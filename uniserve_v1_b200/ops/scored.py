@@ -28,7 +28,7 @@ BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 N.register_signatures({
     "us_scored_decode_scratch": (L, [I]),
     "us_scored_decode": (I, [P, L, P, P, P, P, P, I, P, P, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, P, P, P, P,
-                             I, I, I, P]),
+                             P, P, I, I, I, P]),
     "us_scored_flash": (I, [P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, I, P, P, P, P]),
     "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
 })
@@ -227,6 +227,8 @@ class DecodeWork:
     counters: torch.Tensor                       # zero between calls
     prefix_o: Optional[torch.Tensor] = None      # partial results of shared prefixes
     prefix_ml: Optional[torch.Tensor] = None
+    own_o: Optional[torch.Tensor] = None         # and of the rest of each row
+    own_ml: Optional[torch.Tensor] = None
 
 
 def _chunks(Hq, Hkv):
@@ -266,6 +268,8 @@ def decode_work(B, Hq, Hkv, D, device, shared: Optional[SharedPrefix] = None) ->
             rows = shared.groups * pairs * Hkv * parts * 2 * _TILE
             w.prefix_o = torch.empty(rows * D, dtype=F32, device=device)
             w.prefix_ml = torch.empty(rows * 2, dtype=F32, device=device)
+            w.own_o = torch.empty(B * Hq * D, dtype=F32, device=device)
+            w.own_ml = torch.empty(B * Hq * 2, dtype=F32, device=device)
     return w
 
 
@@ -335,12 +339,13 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
                 work.scratch.numel() * 4 < N.kernels().us_scored_decode_scratch(D):
             raise ValueError("the workspace is of a smaller batch, fewer heads, or another device")
         groups = 0
-        pre = (None,) * 4 + (1, 1, 1)
+        pre = (None,) * 6 + (1, 1, 1)
         if B and shared is not None:
             pairs, parts, each = _prefix_plan(shared, Hq, Hkv, _sm_count(q.device))
             groups = shared.groups
             rows = groups * pairs * Hkv * parts * 2 * _TILE
-            if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.prefix_ml.numel() < rows * 2:
+            if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.prefix_ml.numel() < rows * 2 or \
+                    work.own_o.numel() < B * Hq * D:
                 raise ValueError("the workspace is of smaller shared prefixes")
             k, v, cu = kcache, vcache, None
             if bits != 16 or page < 8 or (_TILE % page and page % _TILE):
@@ -358,12 +363,13 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
                    page_table.shape[1], k.shape[0], B, N.ptr(seq_lens), N.ptr(shared.cu_rows), N.ptr(shared.lens), groups,
                    Hq, Hkv, D, shared.max_rows, scale, rules.cap, N.ptr(rules.slopes), N.ptr(work.prefix_o),
                    N.ptr(work.prefix_ml), pairs, parts, each, N.stream())
-            pre = (N.ptr(shared.cu_rows), N.ptr(shared.lens), N.ptr(work.prefix_o), N.ptr(work.prefix_ml), pairs, parts, each)
+            pre = (N.ptr(shared.cu_rows), N.ptr(shared.lens), N.ptr(work.prefix_o), N.ptr(work.prefix_ml),
+                   N.ptr(work.own_o), N.ptr(work.own_ml), pairs, parts, each)
         if B:
             N.call("us_scored_decode", N.ptr(q), q.stride(0), N.ptr(kcache), N.ptr(vcache), N.ptr(k_scale), N.ptr(v_scale),
                    N.ptr(page_table), page_table.shape[1], N.ptr(seq_lens), N.ptr(starts), N.ptr(to), to.stride(0),
                    N.ptr(work.scratch), N.ptr(work.counters), B, Hq, Hkv, D, bits, pages, page, rules.window, scale,
-                   rules.cap, N.ptr(rules.slopes), groups, *pre, N.stream())
+                   rules.cap, N.ptr(rules.slopes), groups, *pre, N.stream(), launches=2 if groups else 1)
         if out is not None and to is not out:
             return out.copy_(to)
         return to
