@@ -70,9 +70,10 @@ def cached(kc, ks, pages, count):
     return rows.reshape(-1, *rows.shape[2:])[:count]
 
 
-def decode(q, kc, vc, table, lens, scale, cap=0.0, slopes=None, window=0, starts=None, ks=None, vs=None, rounded=None):
-    """Row by row -> (out, bound) [B, Hq, D].  The first `rounded[b]` keys and values of a row are those of the cache
-    rounded to bf16 (an expanded prefix)."""
+def decode(q, kc, vc, table, lens, scale, cap=0.0, slopes=None, window=0, starts=None, ks=None, vs=None, expanded=None):
+    """Row by row -> (out, bound) [B, Hq, D].  The first `expanded[b]` keys and values of a row (a shared prefix of integer
+    pages) are the cache's rounded to FP16 under a power of two (2^e to 2^(e + 1) holds the prefix's largest scale of the
+    head, so products of codes are in reach): its definition of those values."""
     outs, bounds = [], []
     page = kc.shape[1]
     for b, n in enumerate(lens.tolist()):
@@ -83,8 +84,14 @@ def decode(q, kc, vc, table, lens, scale, cap=0.0, slopes=None, window=0, starts
         pages = table[b, :-(-n // page)].long()
         k, v = cached(kc, ks, pages, n), cached(vc, vs, pages, n)
         j = torch.arange(n, device=q.device)
-        if rounded is not None:
-            k, v = (torch.cat([t[:rounded[b]].bfloat16().double(), t[rounded[b]:]]) for t in (k, v))
+        if expanded is not None and expanded[b]:
+            m, at = min(expanded[b], n), table[b, :-(-expanded[b] // page)].long()
+            kv = []
+            for t, sc in ((k, ks), (v, vs)):
+                top = sc[at].transpose(1, 2).flatten(0, 1)[:expanded[b]].double().amax((0, 2))
+                down = torch.exp2(torch.floor(torch.log2(top)))[None, :, None]
+                kv.append(torch.cat([(t[:m] / down).half().double() * down, t[m:]]))
+            k, v = kv
         lo = max(n - window if window else 0, int(starts[b]) if starts is not None else 0)
         # keys that are not visible weigh nothing whatever they hold
         k, v = (torch.where((j >= lo)[:, None, None], t, torch.zeros_like(t)) for t in (k, v))

@@ -156,8 +156,8 @@ def test_shared_prefixes(case):
     rules = S.ScoreRules(cap, sl)
     got = S.decode_attention(q, kc, vc, table, n, scale, rules, k_scale=ks, v_scale=vs, shared=sh)
     N.raise_on_device_error()
-    rounded = [p for r, p in zip(case[0], case[1]) for _ in range(r)] + [0] * case[2] if ks is not None else None
-    O.check(got, *O.decode(q, kc, vc, table, n, scale, cap, sl, ks=ks, vs=vs, rounded=rounded))
+    prefixes = [p for r, p in zip(case[0], case[1]) for _ in range(r)] + [0] * case[2]
+    O.check(got, *O.decode(q, kc, vc, table, n, scale, cap, sl, ks=ks, vs=vs, expanded=prefixes if ks is not None else None))
     apart = S.decode_attention(q, kc, vc, table, n, scale, rules, k_scale=ks, v_scale=vs)
     O.check(apart, *O.decode(q, kc, vc, table, n, scale, cap, sl, ks=ks, vs=vs))
 

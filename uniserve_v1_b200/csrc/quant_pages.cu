@@ -8,7 +8,11 @@
 // magnitude is under m 2^-100 is stored as zeros (its reciprocal would overflow), a group that holds an
 // infinity or a NaN gets a NaN scale and reads back as NaN.
 //
-// Both are bound by memory.  Writing: a thread has 8 channels of K and of V (two 16-byte loads in flight),
+// A prefix that many sequences share is expanded for the tensor unit (scored_flash_tc05.cu) as FP16: code * s / 2^e with e
+// the exponent of the largest scale of the prefix and head, at most 254 and rounded by 2^-11 (bf16 would round
+// every key by 2^-8 again, which a capped model's scores of some tens turn into percents of a weight).
+//
+// Writing and reading are bound by memory.  Writing: a thread has 8 channels of K and of V (two 16-byte loads in flight),
 // eight threads a group.  Reading: a block has 16 rows, their places in the pages are looked up once, and a
 // thread expands 16 channels at a time (16- or 8-byte load, two 16-byte stores).
 #include "include/us_common.cuh"
@@ -189,6 +193,131 @@ __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
   }
 }
 
+struct PrefixArgs {
+  const uint8_t *kc, *vc;
+  const __nv_bfloat16 *ks, *vs;
+  const int *table, *cu_rows, *shared;
+  const __nv_bfloat16* q;
+  long long ldq;
+  __half *ko, *vo, *qo;        // [groups][max_len][heads][dim] twice, [B][Hq][dim]
+  float* q_back;               // [B * Hq]: what a row's scores are multiplied by
+  int2* exps;                  // [groups * heads]: exponent fields of the largest scale of K and of V
+  int groups, max_len, max_pages, pages, page, heads, dim, batch, Hq;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ float power_of_two(int field) { return __uint_as_float((uint32_t)min(max(field, 0), 254) << 23); }
+// slot of position `pos` of a group's prefix, or -1
+__device__ __forceinline__ long long prefix_slot(const PrefixArgs& a, int g, int pos) {
+  const int pi = pos / a.page;
+  const int pg = pi < a.max_pages ? a.table[(long long)a.cu_rows[g] * a.max_pages + pi] : -1;
+  if (pg >= 0 && pg < a.pages) return (long long)pg * a.page + (pos - pi * a.page);
+  us_dev_fail(a.status, US_DEV_BOUNDS);
+  return -1;
+}
+
+// Blocks [0, groups * heads): the largest scales of a group's head.  The others: 16 rows of Q each, divided by the power of
+// two of their largest channel.
+__global__ void __launch_bounds__(512) prefix_scales_kernel(const PrefixArgs a) {
+  US_PDL_PROLOGUE();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if ((int)blockIdx.x < a.groups * a.heads) {
+    __shared__ uint32_t most[2][16];
+    const int g = blockIdx.x / a.heads, head = blockIdx.x - g * a.heads, groups = a.dim >> 6;
+    const int len = a.cu_rows[g + 1] > a.cu_rows[g] ? min(a.shared[g], a.max_len) : 0;
+    uint32_t k = 0, v = 0;
+#pragma unroll 4
+    for (int pos = threadIdx.x; pos < len; pos += 512) {
+      const long long slot = prefix_slot(a, g, pos);
+      if (slot < 0) continue;
+      const long long p = slot / a.page, at = ((p * a.heads + head) * a.page + (slot - p * a.page)) * groups;
+      for (int i = 0; i < groups; ++i) {
+        k = max(k, (uint32_t)__bfloat16_as_ushort(a.ks[at + i]) & 0x7fffu);
+        v = max(v, (uint32_t)__bfloat16_as_ushort(a.vs[at + i]) & 0x7fffu);
+      }
+    }
+    k = __reduce_max_sync(0xffffffffu, k);
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (lane == 0) {
+      most[0][warp] = k;
+      most[1][warp] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 16; ++i) {
+        k = max(k, most[0][i]);
+        v = max(v, most[1][i]);
+      }
+      a.exps[blockIdx.x] = make_int2((int)(k >> 7), (int)(v >> 7));
+    }
+    return;
+  }
+  const int row = ((int)blockIdx.x - a.groups * a.heads) * 16 + warp;
+  if (row >= a.batch * a.Hq) return;
+  const int b = row / a.Hq;
+  const __nv_bfloat16* from = a.q + (long long)b * a.ldq + (long long)(row - b * a.Hq) * a.dim;
+  uint32_t most = 0;
+  for (int i = lane; i < a.dim; i += 32) most = max(most, (uint32_t)__bfloat16_as_ushort(from[i]) & 0x7fffu);
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int e = (int)(most >> 7);
+  const bool scaled = e > 0 && e < 254;
+  const float down = scaled ? power_of_two(254 - e) : 1.f;
+  for (int i = lane; i < a.dim; i += 32) a.qo[(long long)row * a.dim + i] = __float2half_rn(us::bf2f(from[i]) * down);
+  if (lane == 0) a.q_back[row] = scaled ? power_of_two(e) : 1.f;
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(256) prefix_expand_kernel(const PrefixArgs a) {
+  US_PDL_PROLOGUE();
+  const int g = blockIdx.y, r0 = blockIdx.x * kReadRows;
+  const int len = a.cu_rows[g + 1] > a.cu_rows[g] ? min(a.shared[g], a.max_len) : 0;
+  if (r0 >= len) return;
+  __shared__ long long src[kReadRows];
+  if (threadIdx.x < kReadRows) src[threadIdx.x] = r0 + (int)threadIdx.x < len ? prefix_slot(a, g, r0 + threadIdx.x) : -1;
+  __syncthreads();
+  const bool plane_v = blockIdx.z != 0;
+  const int per_head = a.dim >> 4, per_row = a.heads * per_head, groups = a.dim >> 6;
+  const uint8_t* cache = plane_v ? a.vc : a.kc;
+  const __nv_bfloat16* scales = plane_v ? a.vs : a.ks;
+  __half* out = (plane_v ? a.vo : a.ko) + ((long long)g * a.max_len + r0) * a.heads * a.dim;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < min(kReadRows, len - r0) * per_row; e += 256) {
+    const int i = e / per_row, rest = e - i * per_row, head = rest / per_head, ch = (rest - head * per_head) * 16;
+    uint4* to = reinterpret_cast<uint4*>(out + ((long long)i * a.heads + head) * a.dim + ch);
+    const long long slot = src[i];
+    if (slot < 0) {
+      to[0] = to[1] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const int2 top = a.exps[g * a.heads + head];
+    const long long p = slot / a.page;
+    const float sc = us::bf2f(scales[((p * a.heads + head) * a.page + (slot - p * a.page)) * groups + (ch >> 6)]) *
+                     power_of_two(254 - (plane_v ? top.y : top.x));
+    const uint8_t* c = cache + (slot * a.heads + head) * (a.dim * BITS / 8) + ch * BITS / 8;
+    uint32_t o[8];
+    if constexpr (BITS == 8) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(c);
+      const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t u = w[j >> 1] >> (16 * (j & 1));
+        const __half2 b = __floats2half2_rn(small_int(u & 255u, 128.f) * sc, small_int((u >> 8) & 255u, 128.f) * sc);
+        o[j] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    } else {
+      const uint2 raw = *reinterpret_cast<const uint2*>(c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t u = (j < 4 ? raw.x : raw.y) >> (8 * (j & 3));
+        const __half2 b = __floats2half2_rn(small_int(u & 15u, 8.f) * sc, small_int((u >> 4) & 15u, 8.f) * sc);
+        o[j] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    }
+    to[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
 
 }  // namespace
@@ -227,5 +356,25 @@ US_API int us_quant_gather(const void* kc, const void* vc, const void* ks, const
                    us_status_ptr()};
   US_CUDA_CHECK(us::launch_pdl(bits == 8 ? quant_gather_kernel<8> : quant_gather_kernel<4>,
                                dim3((total + kReadRows - 1) / kReadRows, 2), dim3(256), 0, (cudaStream_t)stream_, a));
+  return US_OK;
+}
+
+// The first min(shared[g], max_len) cached rows behind row cu_rows[g]'s page list as FP16 under the powers of two
+// `exps`, to ko / vo [groups][max_len][heads][dim], and q [batch, Hq, dim] as FP16 rows qo under the factors q_back.
+US_API int us_quant_prefix(const void* kc, const void* vc, const void* ks, const void* vs, const int* table, int max_pages,
+                           const int* cu_rows, const int* shared, int groups, int max_len, int pages, int page, int heads,
+                           int dim, int bits, const void* q, long long ldq, int batch, int Hq, void* ko, void* vo, void* qo,
+                           float* q_back, void* exps, void* stream_) {
+  US_REQUIRE(kc && vc && ks && vs && table && cu_rows && shared && q && ko && vo && qo && q_back && exps);
+  US_REQUIRE(groups >= 1 && groups <= 65535 && max_len >= 1 && pages >= 1 && page >= 1 && heads >= 1 && dim >= 64 && dim % 64 == 0 &&
+             (bits == 8 || bits == 4) && batch >= 1 && Hq >= 1 && max_pages >= 1);
+  US_REQUIRE(aligned16(kc) && aligned16(vc) && aligned16(ko) && aligned16(vo));
+  const PrefixArgs a{(const uint8_t*)kc, (const uint8_t*)vc, (const __nv_bfloat16*)ks, (const __nv_bfloat16*)vs, table, cu_rows,
+                     shared, (const __nv_bfloat16*)q, ldq, (__half*)ko, (__half*)vo, (__half*)qo, q_back, (int2*)exps, groups,
+                     max_len, max_pages, pages, page, heads, dim, batch, Hq, us_status_ptr()};
+  cudaStream_t stream = (cudaStream_t)stream_;
+  US_CUDA_CHECK(us::launch_pdl(prefix_scales_kernel, dim3(groups * heads + (batch * Hq + 15) / 16), dim3(512), 0, stream, a));
+  US_CUDA_CHECK(us::launch_pdl(bits == 8 ? prefix_expand_kernel<8> : prefix_expand_kernel<4>,
+                               dim3((max_len + kReadRows - 1) / kReadRows, groups, 2), dim3(256), 0, stream, a));
   return US_OK;
 }

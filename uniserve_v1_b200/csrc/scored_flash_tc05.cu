@@ -57,7 +57,10 @@ struct ScoredArgs {
   float poly[4], reach, scale_cap, cap_log2;  // cap: x = s (p0 + p1 s^2 + ...) where |s| <= reach
   float base;                                 // what stands for every row's maximum under a small cap
   // shared prefixes
-  const int *table, *lens, *cu_rows, *shared, *cu_shared;
+  const int *table, *lens, *cu_rows, *shared;
+  const float* q_back;                        // FP16 operands (quant_pages.cu): factors of the rows of Q,
+  const int2* exps;                           // and exponent fields of K and V [groups * Hkv]
+  int key_stride;                             // > 0: packed keys, those of group g from row g * key_stride on
   int max_pages, pages, page, batch, pairs, parts, blocks_per_part;
   float *part_o, *part_ml;
   unsigned int* status;
@@ -84,6 +87,7 @@ __device__ __forceinline__ void ex2_poly2(float t0, float t1, float& p0, float& 
   p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(u1) << 23));
 }
 
+__device__ __forceinline__ float power_of_two(int field) { return __uint_as_float((uint32_t)min(max(field, 0), 254) << 23); }
 // bits [lo, hi) of 32
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   lo = max(lo, 0);
@@ -151,9 +155,8 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     q_start = a.cu_rows[seq];                                   // sequences of the group
     q_len = min(a.cu_rows[seq + 1], a.batch) - q_start;
     q0 = pair * 2 * per;
-    k_start = a.cu_shared ? a.cu_shared[seq] : 0;
-    kv_len = a.shared[seq];
-    if (!a.cu_shared) kv_len = (int)min((long long)kv_len, (long long)a.max_pages * a.page);
+    k_start = seq * a.key_stride;
+    kv_len = (int)min((long long)a.shared[seq], a.key_stride > 0 ? (long long)a.key_stride : (long long)a.max_pages * a.page);
     prow0 = ((((long long)seq * a.pairs + pair) * a.Hkv + hk) * a.parts + part) * (2 * kBM);
   }
   if (q0 >= q_len) return;
@@ -270,7 +273,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     if (warp == kTmaWarp) {
       // ---------------------------------------------------------------- loads --
       // The whole warp walks; lane 0 loads whole tiles, or every lane its page of a tile.
-      const bool paged = MODE == 1 && a.table && !a.cu_shared;
+      const bool paged = MODE == 1 && a.key_stride == 0;
       const int rows_at_once = paged ? min(a.page, kBN) : kBN;
       const int loads = kBN / rows_at_once;
       auto row_of = [&](int j) -> int {      // first row of this lane's load of block j
@@ -323,8 +326,8 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag));
       };
-      constexpr uint32_t kIdescQK = tc::make_idesc(kBM, kBN, tc::kFmtBF16, tc::kFmtBF16, 0, 0);
-      constexpr uint32_t kIdescPV = tc::make_idesc(kBM, kD, tc::kFmtBF16, tc::kFmtBF16, 0, 1);
+      const uint32_t fmt = MODE == 1 && a.q_back ? tc::kFmtF16 : tc::kFmtBF16;
+      const uint32_t kIdescQK = tc::make_idesc(kBM, kBN, fmt, fmt, 0, 0), kIdescPV = tc::make_idesc(kBM, kD, fmt, fmt, 0, 1);
       const uint64_t dq = tc::smem_desc_kmajor_sw128(tc::smem_u32(sQ));
       const uint64_t dk = tc::smem_desc_kmajor_sw128(tc::smem_u32(sK));
       const uint64_t dv = tc::smem_desc_mnmajor_sw128(tc::smem_u32(sV), kHalf, 1024);
@@ -429,6 +432,14 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         }
         if (BIAS) sl = row_ok ? a.slopes[hk * share + r % share] * kLog2e : 0.f;
       }
+      // FP16 operands: the scores' and the outputs' factors
+      const bool half = MODE == 1 && a.q_back;
+      float row_factor = 1.f, out_factor = 1.f;
+      if (half) {
+        const int2 top = a.exps[seq * a.Hkv + hk];
+        out_factor = power_of_two(top.y);
+        if (row_ok) row_factor = a.q_back[(long long)(q_start + q0 + x * per + r / share) * a.Hq + hk * share + r % share] * power_of_two(top.x);
+      }
       const unsigned long long sc2 = pack2(a.scale_log2, a.scale_log2);
       unsigned long long c0 = 0, c1 = 0, c2 = 0, c3 = 0;
       if (CAP) {
@@ -512,7 +523,14 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           l_sum *= alpha;
           m_used = m_new;
         };
+        auto by_row = [&]() {                // FP16 operands were divided by powers of two
+          if (MODE == 1 && half) {
+#pragma unroll
+            for (int i = 0; i < kBN; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * row_factor);
+          }
+        };
         tc::tmem_ld_wait();
+        by_row();
         if (!FIXED && __any_sync(0xffffffffu, m_next - m_used > kRescaleThreshold)) rescale(m_next);
         const int delta = p - kbase;
         // Whether the row's scores are cap's polynomial's.  (A comparison that a NaN fails: such a block takes the other
@@ -541,6 +559,10 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             p1 = ex2f(t1);
           }
           l = add2(l, pack2(p0, p1));
+          if (MODE == 1 && half) {
+            const __half2 t = __floats2half2_rn(p0, p1);
+            return *reinterpret_cast<const uint32_t*>(&t);
+          }
           const __nv_bfloat162 t = __floats2bfloat162_rn(p0, p1);
           return *reinterpret_cast<const uint32_t*>(&t);
         };
@@ -582,7 +604,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           }
           if (!FIXED) {
             const float over = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));     // of the maximum so far
-            through = __all_sync(0xffffffffu, over <= 64.f);
+            through = __all_sync(0xffffffffu, over <= (MODE == 1 && half ? kRescaleThreshold : 64.f));    // FP16 ends at 2^16
             m_next = fmaxf(m_used, m_used + over);
           } else {
             through = true;
@@ -597,6 +619,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (!FIXED && !CAP && n > 0) {     // (the scores were weighed and are wanted again)
             fetch();
             tc::tmem_ld_wait();
+            by_row();
           }
           const float at = (float)delta;
 #pragma unroll
@@ -669,8 +692,9 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               } else {
 #pragma unroll
                 for (int q4 = 0; q4 < 8; ++q4)
-                  *reinterpret_cast<uint4*>(a.part_o + prow * kD + c + q4 * 4) =
-                      make_uint4(w[q4 * 4], w[q4 * 4 + 1], w[q4 * 4 + 2], w[q4 * 4 + 3]);
+                  *reinterpret_cast<float4*>(a.part_o + prow * kD + c + q4 * 4) =
+                      make_float4(__uint_as_float(w[q4 * 4]) * out_factor, __uint_as_float(w[q4 * 4 + 1]) * out_factor,
+                                  __uint_as_float(w[q4 * 4 + 2]) * out_factor, __uint_as_float(w[q4 * 4 + 3]) * out_factor);
               }
             }
           }
@@ -747,7 +771,8 @@ int start_any(bool cap, dim3 grid, const CUtensorMap& q, const CUtensorMap& k, c
               cudaStream_t stream) {
   const bool bias = a.slopes != nullptr;
   if (!cap) return bias ? start<D, false, true, false, MODE>(grid, q, k, v, a, stream) : start<D, false, false, false, MODE>(grid, q, k, v, a, stream);
-  if (small_cap(a)) return bias ? start<D, true, true, true, MODE>(grid, q, k, v, a, stream) : start<D, true, false, true, MODE>(grid, q, k, v, a, stream);
+  // (FP16 weights need a maximum: they end at 2^16)
+  if (small_cap(a) && !a.q_back) return bias ? start<D, true, true, true, MODE>(grid, q, k, v, a, stream) : start<D, true, false, true, MODE>(grid, q, k, v, a, stream);
   return bias ? start<D, true, true, false, MODE>(grid, q, k, v, a, stream) : start<D, true, false, false, MODE>(grid, q, k, v, a, stream);
 }
 template <int MODE>
@@ -798,14 +823,15 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
 
 // The part that the shared prefixes of a decode batch have in its attention (scored_decode.cu): rows
 // [cu_rows[g], cu_rows[g + 1]) of q [B, Hq, D] against the first shared[g] keys behind row cu_rows[g]'s page list in
-// k / v [pages, page, Hkv, D], or, with cu_shared [groups + 1], against packed rows k / v [key_rows, Hkv, D].
+// k / v [pages, page, Hkv, D], or, with key_stride > 0, in rows g * key_stride .. of packed k / v [key_rows, Hkv, D]; with q_back and
+// exps q, k and v are FP16 (us_quant_prefix).
 // part_o, part_ml: [groups][pairs][Hkv][parts][256][D and 2].
 US_API int us_scored_prefix(const void* q, long long ldq, const void* k, long long pages, const void* v, long long page,
-                            const int* cu_shared, const int* table, int max_pages, int key_rows, int B, const int* lens,
+                            const float* q_back, const void* exps, int key_stride, const int* table, int max_pages, int key_rows, int B, const int* lens,
                             const int* cu_rows, const int* shared, int groups, int Hq, int Hkv, int D, int max_rows, float scale,
                             float cap, const float* slopes, float* part_o, float* part_ml, int pairs, int parts,
                             int blocks_per_part, void* stream_) {
-  US_REQUIRE(q && k && v && lens && cu_rows && shared && part_o && part_ml && (cu_shared || table) && groups >= 1 && groups <= 65535 && B >= 1);
+  US_REQUIRE(q && k && v && lens && cu_rows && shared && part_o && part_ml && table && key_stride >= 0 && (!q_back || (exps && key_stride > 0)) && groups >= 1 && groups <= 65535 && B >= 1);
   US_REQUIRE((D == 64 || D == 128) && Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq / Hkv <= kBM && cap >= 0.f && max_rows >= 1);
   US_REQUIRE((ldq % 8) == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16) == 0 && pairs >= 1 && parts >= 1 &&
              blocks_per_part >= 1 && blocks_per_part <= kMaxBlocks && (long long)pairs * Hkv <= 65535);
@@ -813,7 +839,7 @@ US_API int us_scored_prefix(const void* q, long long ldq, const void* k, long lo
   US_REQUIRE((long long)pairs * 2 * per >= max_rows);
   uint64_t rows = (uint64_t)key_rows;
   uint32_t box = kBN;
-  if (!cu_shared) {
+  if (key_stride == 0) {
     US_REQUIRE(pages >= 1 && page >= 8 && (kBN % page == 0 || page % kBN == 0) && pages * page <= 0x7fffff00LL && max_pages >= 1);
     rows = (uint64_t)(pages * page);
     box = (uint32_t)(page < kBN ? page : kBN);
@@ -823,9 +849,10 @@ US_API int us_scored_prefix(const void* q, long long ldq, const void* k, long lo
   const uint64_t dims[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)B};
   const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)ldq * 2};
   const uint32_t qbox[3] = {64, (uint32_t)share, (uint32_t)per};
-  int rc = us_tmap_encode(&tmQ, q, US_TMAP_BF16, 3, dims, strides, qbox, US_SWZ_128);
-  if (!rc) rc = us_tmap_2d(&tmK, k, US_TMAP_BF16, rows, (uint64_t)Hkv * D, (uint64_t)Hkv * D, box, 64, US_SWZ_128);
-  if (!rc) rc = us_tmap_2d(&tmV, v, US_TMAP_BF16, rows, (uint64_t)Hkv * D, (uint64_t)Hkv * D, box, 64, US_SWZ_128);
+  const int type = q_back ? US_TMAP_F16 : US_TMAP_BF16;
+  int rc = us_tmap_encode(&tmQ, q, type, 3, dims, strides, qbox, US_SWZ_128);
+  if (!rc) rc = us_tmap_2d(&tmK, k, type, rows, (uint64_t)Hkv * D, (uint64_t)Hkv * D, box, 64, US_SWZ_128);
+  if (!rc) rc = us_tmap_2d(&tmV, v, type, rows, (uint64_t)Hkv * D, (uint64_t)Hkv * D, box, 64, US_SWZ_128);
   if (rc) return rc;
   ScoredArgs a = {};
   a.Hq = Hq;
@@ -834,7 +861,9 @@ US_API int us_scored_prefix(const void* q, long long ldq, const void* k, long lo
   a.max_pages = max_pages;
   a.pages = (int)pages;
   a.page = (int)page;
-  a.cu_shared = cu_shared;
+  a.q_back = q_back;
+  a.exps = (const int2*)exps;
+  a.key_stride = key_stride;
   a.lens = lens;
   a.cu_rows = cu_rows;
   a.shared = shared;

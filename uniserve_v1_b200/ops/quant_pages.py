@@ -26,6 +26,7 @@ BF16, F32 = torch.bfloat16, torch.float32
 GROUP = 64
 N.register_signatures({
     "us_quant_write": (I, [P, P, L, L, L, L, P, I, P, P, P, P, I, I, I, I, I, I, P]),
+    "us_quant_prefix": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, P, L, I, I, P, P, P, P, P, P]),
     "us_quant_gather": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, P, P, L, P]),
 })
 
@@ -147,3 +148,19 @@ def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows
                page_table.shape[1], N.ptr(cu.contiguous()), N.ptr(out_cu.contiguous() if out_cu is not None else None),
                B, total_rows, pages, page, heads, dim, bits, N.ptr(ko), N.ptr(vo), ko.stride(0), N.stream())
     return ko, vo
+
+
+def expand_prefix(kcache, vcache, k_scale, v_scale, page_table, shared, q):
+    """For ``scored.decode_attention``: the shared prefixes of a batch as FP16 rows under a power of two per group and head,
+    the queries likewise -> (q, k, v, factors of q's rows, exponents of k and v)."""
+    bits = page_bits(kcache, vcache, k_scale, v_scale)
+    pages, page, heads, _ = kcache.shape
+    B, Hq, D = q.shape
+    half, dev, G = torch.float16, q.device, shared.groups
+    k, v = (torch.empty(G * shared.max_len, heads, D, dtype=half, device=dev) for _ in range(2))
+    qh = torch.empty(B, Hq, D, dtype=half, device=dev)
+    back, exps = torch.empty(B * Hq, dtype=F32, device=dev), torch.empty(G * heads, 2, dtype=torch.int32, device=dev)
+    N.call("us_quant_prefix", N.ptr(kcache), N.ptr(vcache), N.ptr(k_scale), N.ptr(v_scale), N.ptr(page_table),
+           page_table.shape[1], N.ptr(shared.cu_rows), N.ptr(shared.lens), G, shared.max_len, pages, page, heads, D, bits, N.ptr(q),
+           q.stride(0), B, Hq, N.ptr(k), N.ptr(v), N.ptr(qh), N.ptr(back), N.ptr(exps), N.stream(), launches=2)
+    return qh, k, v, back, exps

@@ -30,7 +30,7 @@ N.register_signatures({
     "us_scored_decode": (I, [P, L, P, P, P, P, P, I, P, P, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, P, P, P, P,
                              P, P, I, I, I, P]),
     "us_scored_flash": (I, [P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, I, P, P, P, P]),
-    "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
+    "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
 })
 
 MAX_SEQS = 704             # sequences of one decode launch; larger batches go in slices
@@ -305,7 +305,7 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
         raise ValueError("starts is int32 [B]")
     if out is not None and (tuple(out.shape) != (B, Hq, D) or out.dtype != BF16):
         raise ValueError("out has the shape of q, in bfloat16")
-    if shared is not None and not shared.groups:
+    if shared is not None and (not shared.groups or shared.max_len <= 0):
         shared = None
     if shared is not None:
         if starts is not None or rules.window:
@@ -347,22 +347,24 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
             if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.prefix_ml.numel() < rows * 2 or \
                     work.own_o.numel() < B * Hq * D:
                 raise ValueError("the workspace is of smaller shared prefixes")
-            k, v, cu = kcache, vcache, None
-            if bits != 16 or page < 8 or (_TILE % page and page % _TILE):
-                # integer pages, and pages that no tile is made of: the prefix is expanded once for all its readers
+            qp, k, v, back, exps, stride = q, kcache, vcache, None, None, 0
+            if bits != 16:       # integer pages: the prefix is expanded once for all its readers, as FP16
+                from .quant_pages import expand_prefix
+                qp, k, v, back, exps = expand_prefix(kcache, vcache, k_scale, v_scale, page_table, shared, q)
+                stride = shared.max_len
+            elif page < 8 or (_TILE % page and page % _TILE):      # pages that no tile is made of
+                from .functional import kv_gather
+                stride = shared.max_len
                 cu = torch.zeros(groups + 1, dtype=I32, device=q.device)
-                torch.cumsum(shared.lens, 0, dtype=I32, out=cu[1:])
+                torch.cumsum(shared.lens.clamp(max=stride), 0, dtype=I32, out=cu[1:])
+                k, v = (torch.empty(groups * stride, Hkv, D, dtype=BF16, device=q.device) for _ in range(2))
                 first = page_table.index_select(0, shared.cu_rows[:-1].clamp(max=B - 1))
-                if bits == 16:
-                    from .functional import kv_gather
-                    k, v = kv_gather(kcache, vcache, first, cu, groups * shared.max_len)
-                else:
-                    from .quant_pages import kv_gather_quant
-                    k, v = kv_gather_quant(kcache, vcache, k_scale, v_scale, first, cu, groups * shared.max_len)
-            N.call("us_scored_prefix", N.ptr(q), q.stride(0), N.ptr(k), pages, N.ptr(v), page, N.ptr(cu), N.ptr(page_table),
-                   page_table.shape[1], k.shape[0], B, N.ptr(seq_lens), N.ptr(shared.cu_rows), N.ptr(shared.lens), groups,
-                   Hq, Hkv, D, shared.max_rows, scale, rules.cap, N.ptr(rules.slopes), N.ptr(work.prefix_o),
-                   N.ptr(work.prefix_ml), pairs, parts, each, N.stream())
+                kv_gather(kcache, vcache, first, cu, groups * stride, out=(k, v),
+                          out_cu=torch.arange(0, groups * stride, stride, dtype=I32, device=q.device))
+            N.call("us_scored_prefix", N.ptr(qp), qp.stride(0), N.ptr(k), pages, N.ptr(v), page, N.ptr(back), N.ptr(exps),
+                   stride, N.ptr(page_table), page_table.shape[1], k.shape[0], B, N.ptr(seq_lens), N.ptr(shared.cu_rows),
+                   N.ptr(shared.lens), groups, Hq, Hkv, D, shared.max_rows, scale, rules.cap, N.ptr(rules.slopes),
+                   N.ptr(work.prefix_o), N.ptr(work.prefix_ml), pairs, parts, each, N.stream())
             pre = (N.ptr(shared.cu_rows), N.ptr(shared.lens), N.ptr(work.prefix_o), N.ptr(work.prefix_ml),
                    N.ptr(work.own_o), N.ptr(work.own_ml), pairs, parts, each)
         if B:
