@@ -219,9 +219,11 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
   }
   __syncthreads();
   const int total = Hc * pre[B];
-  // one range of the list a warp; where there are fewer tiles than warps, every CTA has as many warps at work
+  // One range of the list a warp.  Where there are fewer tiles than warps, every CTA has as many warps at work, and as
+  // many that a pair of average length ends in eight CTAs' parts at most: 32 of one warp each cost a request of 1021 keys
+  // 4 us at the end.
   const int ctas = gridDim.x, cta = blockIdx.x;
-  const int active = min(kWarps, (total + ctas - 1) / ctas), workers = min(total, ctas * active);
+  const int active = min(kWarps, max((total + ctas - 1) / ctas, (pre[B] + 8 * B - 1) / (8 * B))), workers = min(total, ctas * active);
   const unsigned long long pace = ((unsigned long long)total << 32) / (unsigned)workers;
   auto start_of = [&](int k) -> int { return k >= workers ? total : (int)((pace * (unsigned)k) >> 32); };
   auto worker_of = [&](int g) -> int {

@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import native as N
-from .scored import on_device
+from .scored import current_device, device_of, launch
 
 P, I, L = N.P, N.I, N.L
 BF16, F32 = torch.bfloat16, torch.float32
@@ -43,16 +43,17 @@ def quant_planes(pages: int, page_size: int, kv_heads: int, dim: int, bits: int,
 
 def page_bits(kcache, vcache, k_scale, v_scale) -> int:
     """Bits of the codes of an integer cache, whose planes are checked against each other."""
-    if not all(t.is_contiguous() for t in (kcache, vcache, k_scale, v_scale)):
+    if not (kcache.is_contiguous() and vcache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise ValueError("the planes of an integer cache are contiguous")
     if kcache.dtype != torch.uint8 or vcache.dtype != torch.uint8 or k_scale.dtype != BF16 or v_scale.dtype != BF16:
         raise ValueError(f"an integer cache holds uint8 codes and bfloat16 scales; got {kcache.dtype}, {k_scale.dtype}")
-    if kcache.dim() != 4 or k_scale.dim() != 4 or kcache.shape != vcache.shape or k_scale.shape != v_scale.shape:
+    codes, scales = kcache.shape, k_scale.shape
+    if len(codes) != 4 or len(scales) != 4 or codes != vcache.shape or scales != v_scale.shape:
         raise ValueError("K and V planes of an integer cache have the same shape")
-    pages, page, heads, width = kcache.shape
-    dim = k_scale.shape[3] * GROUP
-    if tuple(k_scale.shape[:3]) != (pages, heads, page) or width not in (dim, dim // 2) or page % 2 or not dim:
-        raise ValueError(f"codes {tuple(kcache.shape)} and scales {tuple(k_scale.shape)} are not of one integer cache")
+    pages, page, heads, width = codes
+    dim = scales[3] * GROUP
+    if scales[0] != pages or scales[1] != heads or scales[2] != page or (width != dim and width * 2 != dim) or page % 2 or not dim:
+        raise ValueError(f"codes {tuple(codes)} and scales {tuple(scales)} are not of one integer cache")
     return 8 if width == dim else 4
 
 
@@ -90,10 +91,10 @@ def kv_write_quant(k, v, slots, kcache, vcache, k_scale, v_scale):
     bits = page_bits(kcache, vcache, k_scale, v_scale)
     pages, page, heads, _ = kcache.shape
     T, dim = k.shape[0], k_scale.shape[3] * GROUP
-    if tuple(k.shape) != (T, heads, dim) or v.shape != k.shape or k.dtype != BF16 or v.dtype != BF16:
+    if k.shape != (T, heads, dim) or v.shape != k.shape or k.dtype != BF16 or v.dtype != BF16:
         raise ValueError(f"rows of this cache are bfloat16 [T, {heads}, {dim}]; got {tuple(k.shape)} {k.dtype}, "
                          f"{tuple(v.shape)} {v.dtype}")
-    if tuple(slots.shape) != (T,) or slots.dtype not in (torch.int32, torch.int64):
+    if slots.shape != (T,) or (slots.dtype != torch.int64 and slots.dtype != torch.int32):
         raise ValueError(f"one int32 or int64 slot a row; got {tuple(slots.shape)} {slots.dtype}")
     if not k.is_cuda:
         if T and int(slots.max()) >= pages * page:
@@ -104,17 +105,20 @@ def kv_write_quant(k, v, slots, kcache, vcache, k_scale, v_scale):
             cache[at // page, at % page] = codes
             scale[at // page, :, at % page] = sc
         return
-    with on_device(k, v, slots, kcache, vcache, k_scale, v_scale):
-        k, v = (_rows16(t) for t in (k, v))
-        N.call("us_quant_write", N.ptr(k), N.ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-               N.ptr(slots.contiguous()), int(slots.dtype == torch.int64), N.ptr(kcache), N.ptr(vcache), N.ptr(k_scale),
-               N.ptr(v_scale), T, pages, page, heads, dim, bits, N.stream())
+    if device_of((k, v, slots, kcache, vcache, k_scale, v_scale)) != current_device():
+        with torch.cuda.device(k.device):
+            return kv_write_quant(k, v, slots, kcache, vcache, k_scale, v_scale)
+    k, v, slots = _rows16(k), _rows16(v), slots.contiguous()
+    a, b, _ = k.stride()
+    c, d, _ = v.stride()
+    launch("us_quant_write", 1, k.data_ptr(), v.data_ptr(), a, b, c, d, slots.data_ptr(), slots.dtype == torch.int64,
+           kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), T, pages, page, heads, dim, bits)
 
 
 def _rows16(t):
     """``t`` [rows, heads, D] with dense channels and 16-byte steps, as it is or copied."""
-    fine = t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
-    return t if fine else t.contiguous() if t.data_ptr() % 16 == 0 or not t.is_contiguous() else t.clone()
+    a, b, c = t.stride()
+    return t if c == 1 and a % 8 == 0 and b % 8 == 0 and t.data_ptr() % 16 == 0 else t.contiguous() if t.data_ptr() % 16 == 0 or not t.is_contiguous() else t.clone()
 
 
 def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows, out=None, out_cu=None):
@@ -130,11 +134,13 @@ def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows
     if out_cu is not None and (out is None or out_cu.dtype != torch.int32 or out_cu.numel() < B):
         raise ValueError("out_cu is int32 [B] and goes with an `out`")
     if out is None:
-        out = tuple(torch.empty(total_rows, heads, dim, dtype=BF16, device=kcache.device) for _ in range(2))
-    ko, vo = out
-    if any(t.dtype != BF16 or tuple(t.shape[1:]) != (heads, dim) or t.stride(2) != 1 or t.stride(1) != dim or
-           t.stride(0) % 8 for t in out) or ko.stride(0) != vo.stride(0) or (out_cu is None and min(ko.shape[0], vo.shape[0]) < total_rows):
-        raise ValueError(f"out is two bfloat16 [>= {total_rows}, {heads}, {dim}] with dense heads and one row pitch")
+        ko = torch.empty(total_rows, heads, dim, dtype=BF16, device=kcache.device)
+        vo = torch.empty_like(ko)
+    else:
+        ko, vo = out
+        if any(t.dtype != BF16 or t.shape[1:] != (heads, dim) or t.stride(2) != 1 or t.stride(1) != dim or t.stride(0) % 8
+               for t in out) or ko.stride(0) != vo.stride(0) or (out_cu is None and min(ko.shape[0], vo.shape[0]) < total_rows):
+            raise ValueError(f"out is two bfloat16 [>= {total_rows}, {heads}, {dim}] with dense heads and one row pitch")
     if not kcache.is_cuda:
         ends, starts = cu.tolist(), (out_cu if out_cu is not None else cu).tolist()
         for s in range(B):
@@ -143,10 +149,13 @@ def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows
             for cache, scale, to in ((kcache, k_scale, ko), (vcache, v_scale, vo)):
                 to[starts[s]:starts[s] + len(pos)] = dequantise(cache[at, pos % page], scale[at, :, pos % page]).to(BF16)
         return ko, vo
-    with on_device(kcache, vcache, k_scale, v_scale, page_table, cu, ko, vo, out_cu):
-        N.call("us_quant_gather", N.ptr(kcache), N.ptr(vcache), N.ptr(k_scale), N.ptr(v_scale), N.ptr(page_table),
-               page_table.shape[1], N.ptr(cu.contiguous()), N.ptr(out_cu.contiguous() if out_cu is not None else None),
-               B, total_rows, pages, page, heads, dim, bits, N.ptr(ko), N.ptr(vo), ko.stride(0), N.stream())
+    if device_of((kcache, vcache, k_scale, v_scale, page_table, cu, ko, vo, out_cu)) != current_device():
+        with torch.cuda.device(kcache.device):
+            return kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows, (ko, vo), out_cu)
+    cu, out_cu = cu.contiguous(), None if out_cu is None else out_cu.contiguous()
+    launch("us_quant_gather", 1, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+           page_table.data_ptr(), page_table.shape[1], cu.data_ptr(), None if out_cu is None else out_cu.data_ptr(), B, total_rows,
+           pages, page, heads, dim, bits, ko.data_ptr(), vo.data_ptr(), ko.stride(0))
     return ko, vo
 
 
@@ -160,7 +169,8 @@ def expand_prefix(kcache, vcache, k_scale, v_scale, page_table, shared, q):
     k, v = (torch.empty(G * shared.max_len, heads, D, dtype=half, device=dev) for _ in range(2))
     qh = torch.empty(B, Hq, D, dtype=half, device=dev)
     back, exps = torch.empty(B * Hq, dtype=F32, device=dev), torch.empty(G * heads, 2, dtype=torch.int32, device=dev)
-    N.call("us_quant_prefix", N.ptr(kcache), N.ptr(vcache), N.ptr(k_scale), N.ptr(v_scale), N.ptr(page_table),
-           page_table.shape[1], N.ptr(shared.cu_rows), N.ptr(shared.lens), G, shared.max_len, pages, page, heads, D, bits, N.ptr(q),
-           q.stride(0), B, Hq, N.ptr(k), N.ptr(v), N.ptr(qh), N.ptr(back), N.ptr(exps), N.stream(), launches=2)
+    launch("us_quant_prefix", 2, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+           page_table.data_ptr(), page_table.shape[1], shared.cu_rows.data_ptr(), shared.lens.data_ptr(), G, shared.max_len, pages,
+           page, heads, D, bits, q.data_ptr(), q.stride(0), B, Hq, k.data_ptr(), v.data_ptr(), qh.data_ptr(), back.data_ptr(),
+           exps.data_ptr())
     return qh, k, v, back, exps

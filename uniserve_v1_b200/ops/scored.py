@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -38,8 +38,7 @@ MAX_KEYS = 1 << 20         # keys of a prompt's sequence
 _TILE = 128                # rows of a tile, keys of a block of the prompt kernel
 
 
-@dataclass(frozen=True)
-class ScoreRules:
+class ScoreRules(NamedTuple):
     """What happens to a score between scale q.k and the softmax."""
     cap: float = 0.0                            # > 0: cap * tanh(score / cap)
     slopes: Optional[torch.Tensor] = None       # FP32 [Hq]: - slope * |position - key|
@@ -61,43 +60,54 @@ class SharedPrefix:
         return self.lens.shape[0]
 
 
-class on_device:
-    """The device of `tensors` (all on one; None is left out) as the current one."""
-
-    def __init__(self, *tensors):
-        at = None
-        for t in tensors:
-            if t is not None:
-                i = t.get_device()
-                if at is None:
-                    at = i
-                elif i != at:
-                    raise ValueError("the tensors of a call are on one device")
-        self.ctx = None if at == torch._C._cuda_getDevice() else torch.cuda.device(at)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *e):
-        if self.ctx is not None:
-            self.ctx.__exit__(*e)
+def device_of(tensors) -> int:
+    """The one device that all of `tensors` are on (None is left out)."""
+    at = None
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if at is None:
+                at = i
+            elif i != at:
+                raise ValueError("the tensors of a call are on one device")
+    return at
 
 
-def _check_rules(rules, Hq, dev):
-    if not (rules.cap >= 0.0 and math.isfinite(rules.cap)) or rules.window < 0:
-        raise ValueError(f"cap {rules.cap} and window {rules.window} are not negative, and finite")
-    s = rules.slopes
-    if s is not None and (s.dtype != F32 or tuple(s.shape) != (Hq,) or not s.is_contiguous() or s.device != dev):
+current_device = torch._C._cuda_getDevice
+_entry: dict = {}
+
+
+def launch(name: str, launches: int, *args) -> None:
+    """``native.call`` with device addresses as plain integers, the entry point looked up once: a decode step of one
+    request waits for Python, not for its kernels."""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(N.kernels(), name)
+    rc = fn(*args, N.stream())
+    if rc != 0:
+        N.check(rc, name)
+    N.launch_count += launches
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _check_rules(rules, Hq, at):
+    cap, s, window = rules
+    if not 0.0 <= cap < math.inf or window < 0:
+        raise ValueError(f"cap {cap} and window {window} are not negative, and finite")
+    if s is not None and (s.dtype != F32 or s.shape != (Hq,) or not s.is_contiguous() or s.get_device() != at):
         raise ValueError(f"slopes are a contiguous float32 [{Hq}] beside the queries; got {tuple(s.shape)} {s.dtype}")
 
 
 def _heads(q, k, v, what):
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
+    a, b = q.shape, k.shape
+    if len(a) != 3 or len(b) != 3 or v.shape != b or a[2] != b[2]:
         raise ValueError(f"{what}: q [rows, Hq, D], k and v [keys, Hkv, D]; got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
-    if not k.shape[1] or not q.shape[1] or q.shape[1] % k.shape[1]:
-        raise ValueError(f"{what}: {q.shape[1]} query heads over {k.shape[1]} key heads")
+    if not b[1] or not a[1] or a[1] % b[1]:
+        raise ValueError(f"{what}: {a[1]} query heads over {b[1]} key heads")
 
 
 # ----------------------------------------------------------------- prompts --
@@ -116,17 +126,19 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
     may reach any row of its own sequence that shares a block of 128 keys with one that sees it."""
     _heads(q, k, v, "prompt_attention")
     Tq, Hq, D = q.shape
-    _check_rules(rules, Hq, q.device)
+    Tk, Hkv, _ = k.shape
+    at = q.get_device()
+    _check_rules(rules, Hq, at)
     n = cu_q.numel() - 1
     if n < 0 or cu_k.numel() != n + 1 or cu_q.dtype != I32 or cu_k.dtype != I32:
         raise ValueError("cu_q and cu_k are int32 [sequences + 1]")
-    if docs is not None and (docs.dtype != I32 or docs.shape != k.shape[:1]):
+    if docs is not None and (docs.dtype != I32 or docs.shape != (Tk,)):
         raise ValueError("docs is int32, one number a key")
     if prefix is not None and (prefix.dtype != I32 or prefix.numel() != n):
         raise ValueError("prefix is int32, one length a sequence")
     if out is not None and (out.shape != q.shape or out.dtype != BF16):
         raise ValueError("out has the shape of q, in bfloat16")
-    if not q.is_cuda:
+    if at < 0:
         res = _prompt_cpu(q, k, v, cu_q, cu_k, scale, rules, causal, docs, prefix)
         if out is None:
             return res
@@ -138,40 +150,46 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
     if D % 8 or D > 128 or max_k > MAX_KEYS:
         raise ValueError(f"scored attention serves head widths that are multiples of 8 up to 128, and sequences of up to "
                          f"{MAX_KEYS} keys; got width {D}, {max_k} keys")
-    with on_device(q, k, v, cu_q, cu_k, docs, prefix, rules.slopes, out):
-        if D not in (64, 128):          # zero channels add nothing to q.k and give zero channels, cut off again
-            wide = 64 if D < 64 else 128
-            q, k, v = (torch.nn.functional.pad(t, (0, wide - D)) for t in (q, k, v))
-            got = prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules, causal, docs, prefix)[..., :D]
-            if out is None:
-                return got.contiguous()
-            keep = torch.arange(Tq, device=q.device)[:, None, None] < cu_q[-1]
-            return out.copy_(torch.where(keep, got, out))
-        q, k, v = (_dense_heads(t) for t in (q, k, v))
-        to = out if out is not None and _fits(out) else torch.empty(Tq, Hq, D, dtype=BF16, device=q.device)
-        if out is not None and to is not out:
-            to.copy_(out)
-        if n and Tq and max_q > 0:
-            if not k.shape[0]:
-                k = v = torch.zeros(1, k.shape[1], D, dtype=BF16, device=q.device)
-                docs = None
-            ranges = None
-            if docs is not None:
-                docs = docs.contiguous()
-                ranges = torch.empty(2 * (k.shape[0] // _TILE + n + 1), dtype=I32, device=q.device)
-            N.call("us_scored_flash", N.ptr(q), q.stride(0), N.ptr(k), k.stride(0), N.ptr(v), v.stride(0), N.ptr(to),
-                   to.stride(0), N.ptr(cu_q.contiguous()), N.ptr(cu_k.contiguous()), n, Tq, k.shape[0], Hq, k.shape[1], D,
-                   max_q, max_k, scale, rules.cap, N.ptr(rules.slopes), int(causal), rules.window, N.ptr(docs),
-                   N.ptr(prefix.contiguous() if prefix is not None else None), N.ptr(ranges), N.stream(),
-                   launches=1 if docs is None else 2)
-        if out is not None and to is not out:
-            out.copy_(to)
-            return out
-        return to
+    device_of((q, k, v, cu_q, cu_k, docs, prefix, out))
+    if at != current_device():
+        with torch.cuda.device(at):
+            return prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules, causal, docs, prefix, out)
+    if D != 64 and D != 128:            # zero channels add nothing to q.k and give zero channels, cut off again
+        wide = 64 if D < 64 else 128
+        q, k, v = (torch.nn.functional.pad(t, (0, wide - D)) for t in (q, k, v))
+        got = prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules, causal, docs, prefix)[..., :D]
+        if out is None:
+            return got.contiguous()
+        keep = torch.arange(Tq, device=q.device)[:, None, None] < cu_q[-1]
+        return out.copy_(torch.where(keep, got, out))
+    q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
+    to = out
+    if out is None:
+        to = torch.empty_like(q) if q.is_contiguous() else q.new_empty(Tq, Hq, D)
+    elif not _fits(out):
+        to = out.contiguous() if not out.is_contiguous() else out.clone()
+    if n and Tq and max_q > 0:
+        if not Tk:
+            k = v = torch.zeros(1, Hkv, D, dtype=BF16, device=q.device)
+            docs, Tk = None, 1
+        ranges = None
+        if docs is not None:
+            docs = docs.contiguous()
+            ranges = torch.empty(2 * (Tk // _TILE + n + 1), dtype=I32, device=q.device)
+        if not (cu_q.is_contiguous() and cu_k.is_contiguous()):
+            cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
+        prefix = None if prefix is None else prefix.contiguous()
+        launch("us_scored_flash", 1 if docs is None else 2, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0),
+               v.data_ptr(), v.stride(0), to.data_ptr(), to.stride(0), cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, Hq, Hkv, D,
+               max_q, max_k, scale, rules.cap, _at(rules.slopes), causal, rules.window, _at(docs), _at(prefix), _at(ranges))
+    if out is not None and to is not out:
+        return out.copy_(to)
+    return to
 
 
 def _fits(t):
-    return t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+    a, b, c = t.stride()
+    return c == 1 and b == t.shape[2] and a % 8 == 0 and t.data_ptr() % 16 == 0
 
 
 def _dense_heads(t):
@@ -225,6 +243,7 @@ class DecodeWork:
     ordered on the device (two captured graphs that may run side by side have one each)."""
     scratch: torch.Tensor
     counters: torch.Tensor                       # zero between calls
+    width: int                                   # channels of a head, at most
     prefix_o: Optional[torch.Tensor] = None      # partial results of shared prefixes
     prefix_ml: Optional[torch.Tensor] = None
     own_o: Optional[torch.Tensor] = None         # and of the rest of each row
@@ -249,8 +268,7 @@ def _prefix_plan(shared: SharedPrefix, Hq, Hkv, sms):
 _sms: dict = {}
 
 
-def _sm_count(device) -> int:
-    i = device.index if device.index is not None else torch.cuda.current_device()
+def _sm_count(i: int) -> int:
     if i not in _sms:
         _sms[i] = torch.cuda.get_device_properties(i).multi_processor_count
     return _sms[i]
@@ -262,9 +280,9 @@ def decode_work(B, Hq, Hkv, D, device, shared: Optional[SharedPrefix] = None) ->
     with torch.cuda.device(device):
         bytes_ = N.kernels().us_scored_decode_scratch(D)
         w = DecodeWork(torch.empty(bytes_ // 4, dtype=F32, device=device),
-                       torch.zeros(min(B, MAX_SEQS) * Hkv * _chunks(Hq, Hkv), dtype=I32, device=device))
+                       torch.zeros(min(B, MAX_SEQS) * Hkv * _chunks(Hq, Hkv), dtype=I32, device=device), D)
         if shared is not None and shared.groups:
-            pairs, parts, _ = _prefix_plan(shared, Hq, Hkv, _sm_count(device))
+            pairs, parts, _ = _prefix_plan(shared, Hq, Hkv, _sm_count(device.index if device.index is not None else current_device()))
             rows = shared.groups * pairs * Hkv * parts * 2 * _TILE
             w.prefix_o = torch.empty(rows * D, dtype=F32, device=device)
             w.prefix_ml = torch.empty(rows * 2, dtype=F32, device=device)
@@ -286,95 +304,99 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
     if kcache.dim() != 4 or kcache.shape != vcache.shape:
         raise ValueError("K and V pages have the same shape [pages, page_size, Hkv, D]")
     pages, page, Hkv, width = kcache.shape
-    bits = 16
-    if (k_scale is None) != (v_scale is None):
-        raise ValueError("integer pages come with the scales of both planes")
-    if k_scale is not None:
+    at, bits = q.get_device(), 16
+    if k_scale is not None or v_scale is not None:
+        if k_scale is None or v_scale is None:
+            raise ValueError("integer pages come with the scales of both planes")
         from .quant_pages import GROUP, page_bits
         bits = page_bits(kcache, vcache, k_scale, v_scale)
-        if k_scale.shape[3] * GROUP != D:
-            raise ValueError(f"queries of width {D} over pages of width {k_scale.shape[3] * GROUP}")
-    elif width != D or kcache.dtype != q.dtype or vcache.dtype != q.dtype:
-        raise ValueError(f"queries [.., {D}] {q.dtype} over pages [.., {width}] {kcache.dtype}")
-    if Hq % Hkv:
-        raise ValueError(f"{Hq} query heads over {Hkv} key heads")
-    _check_rules(rules, Hq, q.device)
+        width = k_scale.shape[3] * GROUP
+    elif kcache.dtype != q.dtype or vcache.dtype != q.dtype:
+        raise ValueError(f"queries {q.dtype} over pages {kcache.dtype}")
+    if width != D or Hq % Hkv:
+        raise ValueError(f"queries [.., {Hq}, {D}] over pages [.., {Hkv}, {width}]")
+    _check_rules(rules, Hq, at)
     if page_table.dim() != 2 or page_table.shape[0] < B or seq_lens.numel() < B or page_table.dtype != I32 or seq_lens.dtype != I32:
         raise ValueError("page_table is int32 [B, max_pages], seq_lens int32 [B]")
     if starts is not None and (starts.dtype != I32 or starts.numel() < B):
         raise ValueError("starts is int32 [B]")
-    if out is not None and (tuple(out.shape) != (B, Hq, D) or out.dtype != BF16):
+    if out is not None and (out.shape != q.shape or out.dtype != BF16):
         raise ValueError("out has the shape of q, in bfloat16")
-    if shared is not None and (not shared.groups or shared.max_len <= 0):
-        shared = None
     if shared is not None:
-        if starts is not None or rules.window:
+        if not shared.groups or shared.max_len <= 0:
+            shared = None
+        elif starts is not None or rules.window:
             raise ValueError("a shared prefix goes with neither starts nor a window")
-        if shared.cu_rows.dtype != I32 or shared.lens.dtype != I32 or shared.cu_rows.numel() != shared.groups + 1:
+        elif shared.cu_rows.dtype != I32 or shared.lens.dtype != I32 or shared.cu_rows.numel() != shared.groups + 1:
             raise ValueError("a shared prefix has int32 cu_rows [groups + 1] and lens [groups]")
-        if Hq // Hkv > _TILE or B > MAX_SEQS:
+        elif Hq // Hkv > _TILE or B > MAX_SEQS:
             raise ValueError(f"a shared prefix is served for up to {_TILE} query heads a key head and {MAX_SEQS} sequences")
-    if not q.is_cuda:
+    if at < 0:
         res = _decode_cpu(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k_scale, v_scale, shared)
         return res if out is None else out.copy_(res)
-    if q.dtype != BF16 or D not in (64, 128):
+    if q.dtype != BF16 or (D != 128 and D != 64):
         raise ValueError(f"scored decode attention serves bfloat16 queries of width 64 or 128; got {q.dtype}, {D}")
-    if not (page_table.is_contiguous() and seq_lens.is_contiguous() and kcache.is_contiguous() and vcache.is_contiguous()):
-        raise ValueError("pages, page table and lengths are contiguous")
+    if not (page_table.is_contiguous() and seq_lens.is_contiguous() and kcache.is_contiguous() and vcache.is_contiguous() and
+            (starts is None or starts.is_contiguous())):
+        raise ValueError("pages, page table, lengths and starts are contiguous")
+    device_of((q, kcache, vcache, k_scale, v_scale, page_table, seq_lens, starts, out,
+               shared and shared.cu_rows, shared and shared.lens, work and work.counters))
+    if at != current_device():
+        with torch.cuda.device(at):
+            return decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k_scale, v_scale, shared, work, out)
     if B > MAX_SEQS:
-        out = torch.empty(B, Hq, D, dtype=BF16, device=q.device) if out is None else out
+        out = q.new_empty(B, Hq, D) if out is None else out
         for b in range(0, B, MAX_SEQS):
             e = min(B, b + MAX_SEQS)
             decode_attention(q[b:e], kcache, vcache, page_table[b:e], seq_lens[b:e], scale, rules,
                              None if starts is None else starts[b:e], k_scale, v_scale, None, work, out[b:e])
         return out
-    with on_device(q, kcache, vcache, k_scale, v_scale, page_table, seq_lens, starts, rules.slopes, out,
-                   shared.cu_rows if shared else None, shared.lens if shared else None):
-        q = _dense_heads(q)
-        to = out if out is not None and out.stride(2) == 1 and out.stride(1) == D and out.stride(0) % 2 == 0 and \
-            out.data_ptr() % 4 == 0 else torch.empty(B, Hq, D, dtype=BF16, device=q.device)
-        if work is None:
-            work = decode_work(B, Hq, Hkv, D, q.device, shared)
-        elif work.counters.numel() < B * Hkv * _chunks(Hq, Hkv) or work.counters.device != q.device or \
-                work.scratch.numel() * 4 < N.kernels().us_scored_decode_scratch(D):
-            raise ValueError("the workspace is of a smaller batch, fewer heads, or another device")
-        groups = 0
-        pre = (None,) * 6 + (1, 1, 1)
-        if B and shared is not None:
-            pairs, parts, each = _prefix_plan(shared, Hq, Hkv, _sm_count(q.device))
-            groups = shared.groups
-            rows = groups * pairs * Hkv * parts * 2 * _TILE
-            if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.prefix_ml.numel() < rows * 2 or \
-                    work.own_o.numel() < B * Hq * D:
-                raise ValueError("the workspace is of smaller shared prefixes")
-            qp, k, v, back, exps, stride = q, kcache, vcache, None, None, 0
-            if bits != 16:       # integer pages: the prefix is expanded once for all its readers, as FP16
-                from .quant_pages import expand_prefix
-                qp, k, v, back, exps = expand_prefix(kcache, vcache, k_scale, v_scale, page_table, shared, q)
-                stride = shared.max_len
-            elif page < 8 or (_TILE % page and page % _TILE):      # pages that no tile is made of
-                from .functional import kv_gather
-                stride = shared.max_len
-                cu = torch.zeros(groups + 1, dtype=I32, device=q.device)
-                torch.cumsum(shared.lens.clamp(max=stride), 0, dtype=I32, out=cu[1:])
-                k, v = (torch.empty(groups * stride, Hkv, D, dtype=BF16, device=q.device) for _ in range(2))
-                first = page_table.index_select(0, shared.cu_rows[:-1].clamp(max=B - 1))
-                kv_gather(kcache, vcache, first, cu, groups * stride, out=(k, v),
-                          out_cu=torch.arange(0, groups * stride, stride, dtype=I32, device=q.device))
-            N.call("us_scored_prefix", N.ptr(qp), qp.stride(0), N.ptr(k), pages, N.ptr(v), page, N.ptr(back), N.ptr(exps),
-                   stride, N.ptr(page_table), page_table.shape[1], k.shape[0], B, N.ptr(seq_lens), N.ptr(shared.cu_rows),
-                   N.ptr(shared.lens), groups, Hq, Hkv, D, shared.max_rows, scale, rules.cap, N.ptr(rules.slopes),
-                   N.ptr(work.prefix_o), N.ptr(work.prefix_ml), pairs, parts, each, N.stream())
-            pre = (N.ptr(shared.cu_rows), N.ptr(shared.lens), N.ptr(work.prefix_o), N.ptr(work.prefix_ml),
-                   N.ptr(work.own_o), N.ptr(work.own_ml), pairs, parts, each)
-        if B:
-            N.call("us_scored_decode", N.ptr(q), q.stride(0), N.ptr(kcache), N.ptr(vcache), N.ptr(k_scale), N.ptr(v_scale),
-                   N.ptr(page_table), page_table.shape[1], N.ptr(seq_lens), N.ptr(starts), N.ptr(to), to.stride(0),
-                   N.ptr(work.scratch), N.ptr(work.counters), B, Hq, Hkv, D, bits, pages, page, rules.window, scale,
-                   rules.cap, N.ptr(rules.slopes), groups, *pre, N.stream(), launches=2 if groups else 1)
-        if out is not None and to is not out:
-            return out.copy_(to)
-        return to
+    q = _dense_heads(q)
+    to = out
+    if out is None or not (out.stride(2) == 1 and out.stride(1) == D and out.stride(0) % 2 == 0 and out.data_ptr() % 4 == 0):
+        to = q.new_empty(B, Hq, D)
+    if not B:
+        return to if out is None else out
+    if work is None:
+        work = decode_work(B, Hq, Hkv, D, q.device, shared)
+    elif work.counters.numel() < B * Hkv * _chunks(Hq, Hkv) or work.width < D:
+        raise ValueError("the workspace is of a smaller batch, fewer heads or narrower ones")
+    groups, pre = 0, _NO_PREFIX
+    if shared is not None:
+        pairs, parts, each = _prefix_plan(shared, Hq, Hkv, _sm_count(at))
+        groups = shared.groups
+        rows = groups * pairs * Hkv * parts * 2 * _TILE
+        if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.own_o.numel() < B * Hq * D:
+            raise ValueError("the workspace is of smaller shared prefixes")
+        qp, k, v, back, exps, stride = q, kcache, vcache, None, None, 0
+        if bits != 16:       # integer pages: the prefix is expanded once for all its readers, as FP16
+            from .quant_pages import expand_prefix
+            qp, k, v, back, exps = expand_prefix(kcache, vcache, k_scale, v_scale, page_table, shared, q)
+            stride = shared.max_len
+        elif page < 8 or (_TILE % page and page % _TILE):      # pages that no tile is made of
+            from .functional import kv_gather
+            stride = shared.max_len
+            cu = torch.zeros(groups + 1, dtype=I32, device=q.device)
+            torch.cumsum(shared.lens.clamp(max=stride), 0, dtype=I32, out=cu[1:])
+            k, v = (torch.empty(groups * stride, Hkv, D, dtype=BF16, device=q.device) for _ in range(2))
+            first = page_table.index_select(0, shared.cu_rows[:-1].clamp(max=B - 1))
+            kv_gather(kcache, vcache, first, cu, groups * stride, out=(k, v),
+                      out_cu=torch.arange(0, groups * stride, stride, dtype=I32, device=q.device))
+        cu_rows, lens, po, pm = shared.cu_rows.data_ptr(), shared.lens.data_ptr(), work.prefix_o.data_ptr(), work.prefix_ml.data_ptr()
+        launch("us_scored_prefix", 1, qp.data_ptr(), qp.stride(0), k.data_ptr(), pages, v.data_ptr(), page, _at(back), _at(exps),
+               stride, page_table.data_ptr(), page_table.shape[1], k.shape[0], B, seq_lens.data_ptr(), cu_rows, lens, groups, Hq,
+               Hkv, D, shared.max_rows, scale, rules.cap, _at(rules.slopes), po, pm, pairs, parts, each)
+        pre = (cu_rows, lens, po, pm, work.own_o.data_ptr(), work.own_ml.data_ptr(), pairs, parts, each)
+    launch("us_scored_decode", 2 if groups else 1, q.data_ptr(), q.stride(0), kcache.data_ptr(), vcache.data_ptr(), _at(k_scale),
+           _at(v_scale), page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), _at(starts), to.data_ptr(), to.stride(0),
+           work.scratch.data_ptr(), work.counters.data_ptr(), B, Hq, Hkv, D, bits, pages, page, rules.window, scale, rules.cap,
+           _at(rules.slopes), groups, *pre)
+    if out is not None and to is not out:
+        return out.copy_(to)
+    return to
+
+
+_NO_PREFIX = (None, None, None, None, None, None, 1, 1, 1)
 
 
 def _decode_cpu(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k_scale, v_scale, shared):
