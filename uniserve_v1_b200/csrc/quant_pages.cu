@@ -12,9 +12,10 @@
 // the exponent of the largest scale of the prefix and head, at most 254 and rounded by 2^-11 (bf16 would round
 // every key by 2^-8 again, which a capped model's scores of some tens turn into percents of a weight).
 //
-// Writing and reading are bound by memory.  Writing: a thread has 8 channels of K and of V (two 16-byte loads in flight),
-// eight threads a group.  Reading: a block has 16 rows, their places in the pages are looked up once, and a
-// thread expands 16 channels at a time (16- or 8-byte load, two 16-byte stores).
+// Writing and reading are bound by memory.  A thread has one column of 8 channels (16 bytes of bf16) in the rows of its
+// block, so what depends on the column is computed once, and loads of several rows are in flight; the rows' places are looked
+// up once a block.  (A division of 64 bits a piece made 12 us of 5 when 8168 rows of 4 heads were written; 16 channels a
+// thread, which leave sectors half written, 32 us of 25 when 41,000 were read.)
 #include "include/us_common.cuh"
 
 namespace {
@@ -53,64 +54,78 @@ __device__ __forceinline__ void quantise8(const uint4& raw, uint32_t (&code)[2],
     scale = us::f2bf(__fdiv_rn(most, kMost));
     inv = __frcp_rn(us::bf2f(scale));
   }
-  // 1.5 * 2^23 + c: the rounded integer in the low mantissa bits (halves to even, as the sum is rounded).
-  // The product is rounded before the sum, as in the definition: no fused multiply-add.
+  // 1.5 * 2^23 + c: the rounded integer in the low mantissa bits (halves to even, as the sum is rounded).  The product is
+  // rounded before the sum, as in the definition: no fused multiply-add.  It stays under m + 1 / 2 without a clamp: the
+  // scale is at least 1 - 2^-8 of max|x| / m, and m / (1 - 2^-8) is 127.498 or 7.03.
   uint32_t t[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float x = top >= 0x7f80u ? 0.f : __uint_as_float(i & 1 ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
-    const float y = fminf(fmaxf(__fmul_rn(x, inv), -kMost), kMost);
-    t[i] = __float_as_uint(__fadd_rn(y, 12582912.f + (BITS == 4 ? 8.f : 0.f)));
+    const float x = __uint_as_float(i & 1 ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
+    t[i] = __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f + (BITS == 4 ? 8.f : 0.f)));
   }
+  const bool fine = top < 0x7f80u;
   if constexpr (BITS == 8) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      code[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t c = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
+      code[i] = fine ? c : 0u;
+    }
   } else {
     uint32_t c = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) c |= (t[i] & 15u) << (4 * i);
-    code[0] = c;
+    code[0] = fine ? c : 0x88888888u;
     code[1] = 0;
   }
 }
 
+constexpr int kWriteRows = 8;
+
 template <int BITS>
 __global__ void __launch_bounds__(256) quant_write_kernel(const WriteArgs a) {
   US_PDL_PROLOGUE();
-  const int per_head = a.dim >> 3, per_row = a.heads * per_head;
-  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-  // the last block's idle threads repeat the last row's work up to the store: a group's eight threads stay
-  // together in the shuffles
-  const long long total = (long long)a.rows * per_row;
-  const long long at = idx < total ? idx : total - 8 + (idx & 7);
-  const int row = (int)(at / per_row), rest = (int)(at - (long long)row * per_row);
-  const int head = rest / per_head, ch = (rest - head * per_head) * 8;
-  const uint4 rk = *reinterpret_cast<const uint4*>(a.k + row * a.ldk + head * a.hsk + ch);
-  const uint4 rv = *reinterpret_cast<const uint4*>(a.v + row * a.ldv + head * a.hsv + ch);
-  const long long slot = a.wide ? ((const long long*)a.slots)[row] : (long long)((const int*)a.slots)[row];
-  uint32_t ck[2], cv[2];
-  __nv_bfloat16 sk, sv;
-  quantise8<BITS>(rk, ck, sk);
-  quantise8<BITS>(rv, cv, sv);
-  if (idx >= total || slot < 0) return;
-  if (slot >= a.capacity) {
-    us_dev_fail(a.status, US_DEV_BOUNDS);
-    return;
-  }
-  const long long byte = (slot * a.heads + head) * (a.dim * BITS / 8) + ch * BITS / 8;
-  if constexpr (BITS == 8) {
-    *reinterpret_cast<uint2*>(a.kc + byte) = make_uint2(ck[0], ck[1]);
-    *reinterpret_cast<uint2*>(a.vc + byte) = make_uint2(cv[0], cv[1]);
-  } else {
-    *reinterpret_cast<uint32_t*>(a.kc + byte) = ck[0];
-    *reinterpret_cast<uint32_t*>(a.vc + byte) = cv[0];
-  }
-  if ((ch & 63) == 0) {
-    const long long p = slot / a.page;
-    const long long s = ((p * a.heads + head) * a.page + (slot - p * a.page)) * (a.dim >> 6) + (ch >> 6);
-    a.ks[s] = sk;
-    a.vs[s] = sv;
+  const int per_row = a.heads * (a.dim >> 3), block_row = blockIdx.x * kWriteRows;
+  const int together = max(1, 256 / per_row);            // rows that the block's threads stand on
+  const int r0 = (int)threadIdx.x / per_row, c0 = (int)threadIdx.x - r0 * per_row;
+  // (eight threads of a group are on one row: rows have a multiple of eight pieces.  Threads past the last row or column
+  // take part in the shuffles on ones that are there, and write nothing.)
+  for (int first = 0; first < per_row; first += 256) {
+    const bool mine = r0 < together && first + c0 < per_row;
+    const int c = mine ? first + c0 : c0 & 7;
+    const int head = (c << 3) / a.dim, ch = (c << 3) - head * a.dim;
+    const __nv_bfloat16 *k = a.k + head * a.hsk + ch, *v = a.v + head * a.hsv + ch;
+    const uint32_t byte = head * (a.dim * BITS / 8) + ch * BITS / 8, row_bytes = a.heads * (a.dim * BITS / 8);
+    const uint32_t group = (uint32_t)head * a.page;
+#pragma unroll 2
+    for (int i = 0; i < kWriteRows; i += together) {
+      const int row = block_row + i + r0, from = min(row, a.rows - 1);
+      const uint4 rk = *reinterpret_cast<const uint4*>(k + from * a.ldk);
+      const uint4 rv = *reinterpret_cast<const uint4*>(v + from * a.ldv);
+      const long long slot = a.wide ? ((const long long*)a.slots)[from] : (long long)((const int*)a.slots)[from];
+      uint32_t ck[2], cv[2];
+      __nv_bfloat16 sk, sv;
+      quantise8<BITS>(rk, ck, sk);
+      quantise8<BITS>(rv, cv, sv);
+      if (!mine || i + r0 >= kWriteRows || row >= a.rows || slot < 0) continue;
+      if (slot >= a.capacity) {
+        us_dev_fail(a.status, US_DEV_BOUNDS);
+        continue;
+      }
+      const unsigned long long to = (unsigned long long)(uint32_t)slot * row_bytes + byte;
+      if constexpr (BITS == 8) {
+        *reinterpret_cast<uint2*>(a.kc + to) = make_uint2(ck[0], ck[1]);
+        *reinterpret_cast<uint2*>(a.vc + to) = make_uint2(cv[0], cv[1]);
+      } else {
+        *reinterpret_cast<uint32_t*>(a.kc + to) = ck[0];
+        *reinterpret_cast<uint32_t*>(a.vc + to) = cv[0];
+      }
+      if ((ch & 63) == 0) {
+        const uint32_t p = (uint32_t)slot / (uint32_t)a.page, off = (uint32_t)slot - p * (uint32_t)a.page;
+        const unsigned long long s = ((unsigned long long)p * (uint32_t)(a.heads * a.page) + group + off) * (uint32_t)(a.dim >> 6) + (ch >> 6);
+        a.ks[s] = sk;
+        a.vs[s] = sv;
+      }
+    }
   }
 }
 
@@ -126,14 +141,53 @@ struct ReadArgs {
 
 constexpr int kReadRows = 16;
 
+__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t mul_bf2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// Eight codes under a scale as bf16, two at a time: a code is a bf16 number exactly (128 + its low bits, less 128 or 256,
+// or 136), and one product of two bf16 numbers, rounded once, is the definition's value.
 template <int BITS>
+struct Code {
+  typedef uint2 type;
+};
+template <>
+struct Code<4> {
+  typedef uint32_t type;
+};
+template <int BITS>
+__device__ __forceinline__ void expand8(const typename Code<BITS>::type& raw, uint32_t scale2, uint4& out) {
+  uint32_t o[4];
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = __byte_perm(j < 2 ? raw.x : raw.y, 0, j & 1 ? 0x4342 : 0x4140);
+      o[j] = mul_bf2(sub_bf2((x & 0x007f007fu) | 0x43004300u, (x & 0x00800080u) | 0x43004300u), scale2);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t x = __byte_perm(raw, 0, 0x4440 + j) * 4097u;      // a byte's nibbles in the low bits of both halves
+      o[j] = mul_bf2(sub_bf2((x & 0x000f000fu) | 0x43004300u, 0x43084308u), scale2);
+    }
+  }
+  out = make_uint4(o[0], o[1], o[2], o[3]);
+}
+template <int BITS, int ROWS>
 __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
   US_PDL_PROLOGUE();
-  __shared__ long long src[kReadRows], dst[kReadRows];   // slot (-1: a page outside the cache), output row (-1: none)
-  const int r0 = blockIdx.x * kReadRows;
-  if (threadIdx.x < kReadRows) {
+  __shared__ long long src[ROWS], at[ROWS], dst[ROWS];   // first byte (-1: a page outside the cache), first scale of head 0,
+                                                         // first output (-1: none) of a row
+  const int r0 = blockIdx.x * ROWS;
+  if (threadIdx.x < ROWS) {
     const int r = r0 + threadIdx.x;
-    long long s = -1, d = -1;
+    long long s = -1, w = 0, d = -1;
     if (r < min(a.total, a.cu[a.B])) {
       int lo = 0, hi = a.B - 1;                 // sequence of packed row r
       while (lo < hi) {
@@ -142,54 +196,57 @@ __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
       }
       const int pos = r - a.cu[lo], pi = pos / a.page;
       const int pg = pi < a.max_pages ? a.table[(long long)lo * a.max_pages + pi] : -1;
-      d = (a.out_cu ? a.out_cu[lo] : a.cu[lo]) + pos;
-      if (pg >= 0 && pg < a.pages) s = (long long)pg * a.page + (pos - pi * a.page);
-      else us_dev_fail(a.status, US_DEV_BOUNDS);
+      d = ((a.out_cu ? a.out_cu[lo] : a.cu[lo]) + pos) * a.ldo;
+      if (pg >= 0 && pg < a.pages) {
+        s = ((long long)pg * a.page + (pos - pi * a.page)) * a.heads * (a.dim * BITS / 8);
+        w = ((long long)pg * a.heads * a.page + (pos - pi * a.page)) * (a.dim >> 6);
+      } else {
+        us_dev_fail(a.status, US_DEV_BOUNDS);
+      }
     }
     src[threadIdx.x] = s;
     dst[threadIdx.x] = d;
+    at[threadIdx.x] = w;
   }
   __syncthreads();
-  const int per_head = a.dim >> 4, per_row = a.heads * per_head, groups = a.dim >> 6;
-  const bool plane_v = blockIdx.y != 0;
-  const uint8_t* cache = plane_v ? a.vc : a.kc;
-  const __nv_bfloat16* scales = plane_v ? a.vs : a.ks;
-  __nv_bfloat16* out = plane_v ? a.vo : a.ko;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < kReadRows * per_row; e += 256) {
-    const int i = e / per_row, rest = e - i * per_row;
-    const int head = rest / per_head, ch = (rest - head * per_head) * 16;
-    const long long slot = src[i];
-    if (dst[i] < 0) continue;
-    uint4* to = reinterpret_cast<uint4*>(out + dst[i] * a.ldo + head * a.dim + ch);
-    if (slot < 0) {
-      to[0] = to[1] = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    const long long p = slot / a.page;
-    const float sc = us::bf2f(scales[((p * a.heads + head) * a.page + (slot - p * a.page)) * groups + (ch >> 6)]);
-    const uint8_t* c = cache + (slot * a.heads + head) * (a.dim * BITS / 8) + ch * BITS / 8;
-    uint32_t o[8];
-    if constexpr (BITS == 8) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(c);
-      const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
+  const int per_row = a.heads * (a.dim >> 3), groups = a.dim >> 6;
+  const int together = max(1, 256 / per_row);            // rows that the block's threads stand on
+  const int t0 = (int)threadIdx.x / per_row;
+  if (t0 >= together) return;
+  for (int c = (int)threadIdx.x - t0 * per_row; c < per_row; c += 256) {
+    const int head = (c << 3) / a.dim, ch = (c << 3) - head * a.dim;
+    const int byte = head * (a.dim * BITS / 8) + ch * BITS / 8, sc = head * a.page * groups + (ch >> 6);
+    const uint8_t *kc = a.kc + byte, *vc = a.vc + byte;
+    const unsigned short *ks = reinterpret_cast<const unsigned short*>(a.ks) + sc, *vs = reinterpret_cast<const unsigned short*>(a.vs) + sc;
+    __nv_bfloat16 *ko = a.ko + (c << 3), *vo = a.vo + (c << 3);
+    for (int i0 = t0; i0 < ROWS; i0 += 4 * together) {     // the loads of four rows, then their values
+      typename Code<BITS>::type k[4], v[4];
+      uint32_t s[4], t[4];
+      long long d[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t u = w[j >> 1] >> (16 * (j & 1));
-        const __nv_bfloat162 b = __floats2bfloat162_rn(small_int(u & 255u, 128.f) * sc, small_int((u >> 8) & 255u, 128.f) * sc);
-        o[j] = *reinterpret_cast<const uint32_t*>(&b);
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * together;
+        d[j] = i < ROWS ? dst[i] : -1;
+        const long long from = i < ROWS ? src[i] : -1, w = i < ROWS ? at[i] : 0;
+        s[j] = t[j] = 0;
+        k[j] = v[j] = typename Code<BITS>::type{};
+        if (from >= 0) {
+          k[j] = *reinterpret_cast<const typename Code<BITS>::type*>(kc + from);
+          v[j] = *reinterpret_cast<const typename Code<BITS>::type*>(vc + from);
+          s[j] = ks[w];
+          t[j] = vs[w];
+        }
       }
-    } else {
-      const uint2 raw = *reinterpret_cast<const uint2*>(c);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t u = (j < 4 ? raw.x : raw.y) >> (8 * (j & 3));
-        const __nv_bfloat162 b = __floats2bfloat162_rn(small_int(u & 15u, 8.f) * sc, small_int((u >> 4) & 15u, 8.f) * sc);
-        o[j] = *reinterpret_cast<const uint32_t*>(&b);
+      for (int j = 0; j < 4; ++j) {
+        if (d[j] < 0) continue;
+        uint4 x = make_uint4(0, 0, 0, 0), y = x;
+        expand8<BITS>(k[j], s[j] * 65537u, x);
+        expand8<BITS>(v[j], t[j] * 65537u, y);
+        *reinterpret_cast<uint4*>(ko + d[j]) = x;
+        *reinterpret_cast<uint4*>(vo + d[j]) = y;
       }
     }
-    to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    to[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -334,9 +391,8 @@ US_API int us_quant_write(const void* k, const void* v, long long ldk, long long
   const WriteArgs a{(const __nv_bfloat16*)k, (const __nv_bfloat16*)v, slots, (uint8_t*)kc, (uint8_t*)vc,
                     (__nv_bfloat16*)ks, (__nv_bfloat16*)vs, ldk, hsk, ldv, hsv, (long long)pages * page, rows, page,
                     heads, dim, wide, us_status_ptr()};
-  const long long blocks = ((long long)rows * heads * (dim / 8) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return US_ERR_LIMIT;
-  US_CUDA_CHECK(us::launch_pdl(bits == 8 ? quant_write_kernel<8> : quant_write_kernel<4>, dim3((unsigned)blocks),
+  if ((long long)pages * page > 0x7fffffffLL) return US_ERR_LIMIT;
+  US_CUDA_CHECK(us::launch_pdl(bits == 8 ? quant_write_kernel<8> : quant_write_kernel<4>, dim3((rows + kWriteRows - 1) / kWriteRows),
                                dim3(256), 0, (cudaStream_t)stream_, a));
   return US_OK;
 }
@@ -354,8 +410,12 @@ US_API int us_quant_gather(const void* kc, const void* vc, const void* ks, const
   const ReadArgs a{(const uint8_t*)kc, (const uint8_t*)vc, (const __nv_bfloat16*)ks, (const __nv_bfloat16*)vs, table, cu,
                    out_cu, (__nv_bfloat16*)ko, (__nv_bfloat16*)vo, ldo, B, max_pages, pages, page, heads, dim, total,
                    us_status_ptr()};
-  US_CUDA_CHECK(us::launch_pdl(bits == 8 ? quant_gather_kernel<8> : quant_gather_kernel<4>,
-                               dim3((total + kReadRows - 1) / kReadRows, 2), dim3(256), 0, (cudaStream_t)stream_, a));
+  // 64 rows a block share one wait for their places; few rows are spread over more blocks
+  const bool many = total >= 16384;
+  auto kernel = bits == 8 ? (many ? quant_gather_kernel<8, 64> : quant_gather_kernel<8, 16>)
+                          : (many ? quant_gather_kernel<4, 64> : quant_gather_kernel<4, 16>);
+  const int rows = many ? 64 : 16;
+  US_CUDA_CHECK(us::launch_pdl(kernel, dim3((total + rows - 1) / rows), dim3(256), 0, (cudaStream_t)stream_, a));
   return US_OK;
 }
 
