@@ -168,6 +168,13 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     if (nb <= 0) return;                                        // such a part is not read
   }
 
+  int first_known = -1;
+  if constexpr (MODE == 0) {
+    const int last = min(q0 + 2 * kBM, q_len) - 1 + shift;     // position of the last row
+    if (nb > 0 && a.causal && last >= 0 && (!a.docs || pre <= last + 1)) first_known = max(last, pre - 1) / kBN;
+    else if (nb > 0 && !a.causal && !a.docs) first_known = nb - 1;
+  }
+
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sQ = smem;                  // two tiles
@@ -197,7 +204,8 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
     *abort_flag = 0;
     tc::mbar_fence_init();
-    // Q is on its way while the blocks are looked up
+    // Q is on its way while the blocks are looked up, and so is the first block's K where it is known: the last block,
+    // or that of the last row's own key (which is of its document), or the one of the prefix's end
     tc::mbar_expect_tx(q_full, MODE == 0 ? 2 * kTile : 2 * kHalves * per * share * 128);
 #pragma unroll
     for (int x = 0; x < 2; ++x)
@@ -213,6 +221,12 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     tc::tmem_relinquish();
   }
   __syncthreads();
+  if (first_known >= 0 && tid == 0) {
+    tc::mbar_expect_tx(q_full, kTile);
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf)
+      tc::tma_load_2d(sK + hf * kHalf, &tmK, q_full, hk * kD + 64 * hf, k_start + first_known * kBN);
+  }
   // ---- which blocks the tiles see ----
   const int words = (nb + 31) / 32;
   const int2* ranges = nullptr;
@@ -265,7 +279,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   // (256 x 208 + 128 x 80 = 63,488)
   if (taken_a + taken_b == 0) {        // nothing is seen: Q has to have landed before the CTA ends
     if (tid == 0) {
-      tc::mbar_arrive(q_full);
+      if (first_known < 0) tc::mbar_arrive(q_full);
       if (!tc::mbar_wait(q_full, 0, abort_flag)) us_dev_fail(a.status, US_DEV_TIMEOUT_FULL);
     }
   } else if (warp >= 8) {
@@ -299,9 +313,13 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       bool ta, tb;
       int j = walk.next(ta, tb);
       int row = row_of(j);
-      if (lane == 0) tc::mbar_expect_tx(q_full, kTile);
-      __syncwarp();
-      load_tile(sK, &tmK, q_full, row);
+      if (first_known < 0) {
+        if (lane == 0) tc::mbar_expect_tx(q_full, kTile);
+        __syncwarp();
+        load_tile(sK, &tmK, q_full, row);
+      } else if (j != first_known && lane == 0) {      // (does not happen: see first_known)
+        us_dev_fail(a.status, US_DEV_BOUNDS);
+      }
       for (int e = 0; j >= 0; ++e) {
         const int st = e & 1;
         const int jn = walk.next(ta, tb);
@@ -464,16 +482,8 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           mine = x ? tb : ta;
         } while (j >= 0 && !mine);
         if (j < 0) break;
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_full[x], (uint32_t)n & 1u, abort_flag))) { ok = false; break; }
-        tc::tc_fence_after_sync();
-        uint32_t v[kBN];
-        auto fetch = [&]() {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
-        };
-        fetch();
         const int kbase = (jb + j) * kBN;
-        // what of the block is visible to the row
+        // what of the block is visible to the row (looked up while the scores are computed)
         bool whole = (lo <= kbase && hi >= kbase + kBN) || pr >= kbase + kBN;
         if (MODE == 0 && ranges) {
           const int2 d = ranges[j];
@@ -505,6 +515,14 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
           }
         }
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_full[x], (uint32_t)n & 1u, abort_flag))) { ok = false; break; }
+        tc::tc_fence_after_sync();
+        uint32_t v[kBN];
+        auto fetch = [&]() {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+        };
+        fetch();
         // O_X under another maximum.  It is still: this block's S was issued after the last block's product, by the same
         // thread.
         auto rescale = [&](float m_new) {
@@ -674,11 +692,13 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           const float inv = MODE == 0 ? (l_sum == 0.f ? 0.f : 1.f / l_sum) : 1.f;
           const long long prow = prow0 + x * kBM + r;
           if (MODE == 1 && row_ok) *reinterpret_cast<float2*>(a.part_ml + prow * 2) = make_float2(m_used, l_sum);
-#pragma unroll 1
+          uint32_t all[kD];
+#pragma unroll
+          for (int c = 0; c < kD; c += 32) tc::tmem_ld32(o_tmem + c, *reinterpret_cast<uint32_t(*)[32]>(all + c));
+          tc::tmem_ld_wait();
+#pragma unroll
           for (int c = 0; c < kD; c += 32) {
-            uint32_t w[32];
-            tc::tmem_ld32(o_tmem + c, w);
-            tc::tmem_ld_wait();
+            const uint32_t* w = all + c;
             if (row_ok) {
               if constexpr (MODE == 0) {
                 __nv_bfloat16* orow = a.out + (long long)(q_start + row) * a.ldo + (long long)h * kD;
