@@ -17,7 +17,7 @@
 //   time, and pairs that go on in other CTAs once more through the CTAs' slots, by the CTA whose arrival completes a
 //   pair's count and puts it back to zero.  (Warps that split every tile between them and met at each pair's end spent a
 //   quarter of the time there.)  Both rounds are one short loop: every instruction of this end is fetched cold, by all
-//   SMs at once, and an unrolled form of it took 15 us where this one takes some 4.
+//   SMs at once, and an unrolled form of it took 15 us where this one takes some 8.
 // * Keys stand on the M side of m16n8k16 products (S^T = K Q^T, O^T = V^T P^T), the query heads of a key head on the
 //   N side: groups of up to 8 heads pay for 8 columns, not for 16 rows, and the softmax has its maximum and sum
 //   per column, three shuffles each.  P^T becomes the B operand by an 8 x 8 transpose in registers (movmatrix).
@@ -126,10 +126,12 @@ struct Walk {
 template <int D, int FMT, int NT>           // FMT: bits of a code (16: bf16)
 struct Shape {
   // Integer codes take more instructions a byte, and with two warps a scheduler each waits for itself: sixteen warps of
-  // 128 registers where one head tile leaves room for that.
-  static constexpr int kWarps = FMT != 16 && NT == 1 ? 16 : 8;
+  // 128 registers, or, where a byte holds two codes, twelve of 168 with 64 keys each (32 sequences of about 8,000 keys, 8
+  // key heads of 128 channels, 4 bits: 57 us, sixteen of 32 keys 63).  Two head tiles want the registers of eight warps:
+  // twelve spill, 137 us in place of 86.
+  static constexpr int kWarps = FMT == 16 || NT == 2 ? 8 : FMT == 8 ? 16 : 12;
   static constexpr int kRow = D * FMT / 8;                          // bytes of a cached row
-  static constexpr int kKeys = FMT == 16 && kRow <= 128 && NT == 1 ? 64 : 32;   // keys of a warp's part of a tile
+  static constexpr int kKeys = NT == 1 && (FMT == 16 ? kRow <= 128 : FMT == 4) ? 64 : 32;   // keys of a warp's part of a tile
   static constexpr int kScales = FMT == 16 ? 0 : kKeys * 4;
   static constexpr int kStage = kKeys * kRow + kScales;             // K or V rows of it
   static constexpr int kRoom = (FMT == 16 ? 196608 : 202752) / kWarps;    // ring bytes of a warp
@@ -154,7 +156,7 @@ struct Part {
 template <int D, int FMT, int NT>
 constexpr size_t shared_bytes() {
   using S = Shape<D, FMT, NT>;
-  return (size_t)S::kWarps * S::kStages * S::kStage + 32 * sizeof(Part) + 16 + (3 * kMaxSeqs + 4) * 4;   // rings; parts; flags; sequences
+  return (size_t)S::kWarps * S::kRoom + 32 * sizeof(Part) + 16 + (3 * kMaxSeqs + 4) * 4;   // rings; parts; flags; sequences
 }
 
 template <int D, int FMT, int NT>           // NT: 8-column head tiles (query heads of a key head in one pass: 8 NT)
@@ -167,8 +169,8 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
   else US_PDL_PROLOGUE();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* ring = smem + (size_t)warp * S::kStages * S::kStage;
-  Part* parts = (Part*)(smem + (size_t)kWarps * S::kStages * S::kStage);  // [warp][2]: begun before its range, ended by it
+  uint8_t* ring = smem + (size_t)warp * S::kRoom;
+  Part* parts = (Part*)(smem + (size_t)kWarps * S::kRoom);  // [warp][2]: begun before its range, ended by it
   int* flag = (int*)(parts + 32);           // [2] CTAs of its first, last pair if this CTA completes it (else 0), [2] first of them
   int* pre = flag + 4;                      // tiles before sequence b
   int* first = pre + kMaxSeqs + 4;          // visible keys of sequence b: [first, end)
@@ -758,7 +760,7 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
   };
   // A part: outputs in the order of the accumulators [NT][D / 16][32 lanes][4], then maxima and sums [NT * 8][2].
   constexpr int kPart = NT * (KS * 128 + 16);
-  static_assert(2 * kPart * 4 <= S::kStages * S::kStage, "two parts have room in a ring");
+  static_assert(2 * kPart * 4 <= S::kRoom, "two parts have room in a ring");
   auto store_tile = [&](float* part, int t, const float (&x)[NT][4]) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -771,7 +773,7 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
         *reinterpret_cast<float4*>(part + NT * KS * 128 + (nt * 8 + c4 * 2) * 2) = make_float4(M[nt][0], L[nt][0], M[nt][1], L[nt][1]);
     }
   };
-  auto ring_of = [&](int w) { return (float*)(smem + (size_t)w * S::kStages * S::kStage); };
+  auto ring_of = [&](int w) { return (float*)(smem + (size_t)w * S::kRoom); };
   // a value under maximum x into one under M
   auto join = [&](float x, float& M, float& f, float& w) {
     const float top = fmaxf(M, x);
