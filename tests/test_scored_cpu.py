@@ -165,3 +165,26 @@ def test_the_cache_refuses():
                dict(out=(torch.zeros(4, 2, 64), torch.zeros(4, 2, 64))), dict(out=(rnd(3, 2, 64), rnd(3, 2, 64)))):
         with pytest.raises(ValueError):
             Q.kv_gather_quant(*planes, **{**dict(page_table=table, cu=cu([4]), total_rows=4), **kw})
+
+
+@pytest.mark.parametrize("cap", [1e-7, 1025.0, 1e30])
+def test_caps_that_single_precision_does_not_carry_are_refused(cap):
+    with pytest.raises(ValueError, match="cap"):
+        S.prompt_attention(**prompt_args(rules=S.ScoreRules(cap=cap)))
+    with pytest.raises(ValueError, match="cap"):
+        S.decode_attention(**decode_args(rules=S.ScoreRules(cap=cap)))
+
+
+def test_a_window_past_32_bits_is_refused():
+    with pytest.raises(ValueError, match="window"):
+        S.prompt_attention(**prompt_args(rules=S.ScoreRules(window=(1 << 32) + 5)))
+
+
+def test_reading_back_refuses_bad_pages_and_rows_past_the_output():
+    planes = Q.quant_planes(3, 4, 2, 64, 8, "cpu")
+    for table, out_cu in ((torch.tensor([[3]], dtype=I32), [0]), (torch.tensor([[-1]], dtype=I32), [0]), (torch.tensor([[0]], dtype=I32), [2])):
+        with pytest.raises(IndexError):
+            Q.kv_gather_quant(*planes, table, cu([4]), 4, out=(rnd(5, 2, 64), rnd(5, 2, 64)), out_cu=torch.tensor(out_cu, dtype=I32))
+    k, v = Q.kv_gather_quant(*planes, torch.zeros(0, 1, dtype=I32), cu([]), 0)
+    assert k.shape == v.shape == (0, 2, 64)
+    Q.kv_write_quant(rnd(0, 2, 64), rnd(0, 2, 64), torch.zeros(0, dtype=torch.int64), *planes)

@@ -1,0 +1,184 @@
+"""Scored attention and integer pages where calls meet: graphs, streams, workspaces, plans that say less than they hold."""
+import pytest
+import torch
+
+import scored_oracle as O
+from test_scored_decode_gpu import make, slopes
+from test_scored_flash_gpu import SHARED, cu, packed, shared_batch
+from uniserve_v1_b200.ops import native as N
+from uniserve_v1_b200.ops import quant_pages as Q
+from uniserve_v1_b200.ops import scored as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, I32 = torch.bfloat16, torch.int32
+
+
+@pytest.mark.parametrize("with_docs", [False, True])
+def test_prompts_in_a_captured_graph_of_a_padded_batch(with_docs):
+    """Captured with room for four sequences and 700 rows; replayed with other lengths, one of them empty."""
+    q, k, v, cq, ck = packed(1, [300, 130, 170, 100], [300, 130, 170, 100], 4, 2, 128)
+    docs = (torch.arange(700, device=DEV) // 90).to(I32) if with_docs else None
+    rules = S.ScoreRules(cap=30.0, slopes=slopes(4))
+    out = torch.full_like(q, 3.0)
+
+    def call():
+        S.prompt_attention(q, k, v, cq, ck, 512, 512, 0.1, rules, docs=docs, out=out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for counts in ([512, 1, 0, 60], [0, 0, 0, 0], [129, 127, 128, 300]):
+        cq.copy_(cu(counts))
+        ck.copy_(cu(counts))
+        q.mul_(-1)
+        out.fill_(3.0)
+        graph.replay()
+        n = sum(counts)
+        assert (out[n:] == 3).all()
+        if n:
+            want, bound = O.prompt(q[:n], k[:n], v[:n], cq, ck, 0.1, 30.0, rules.slopes, docs=None if docs is None else docs[:n])
+            O.check(out[:n], want, bound)
+    N.raise_on_device_error()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_two_streams_at_once(bits):
+    """Two batches on two streams, each with its workspace, prompts between them."""
+    both = [make(s, [900, 0, 77, 3000], 16, 2, 128, 16, bits) for s in (1, 2)]
+    works = [S.decode_work(4, 16, 2, 128, DEV) for _ in both]
+    p = packed(3, [400], [400], 4, 2, 64)
+    alone = S.prompt_attention(*p, 400, 400, 0.1)
+    streams = [torch.cuda.Stream() for _ in both]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            q, kc, vc, ks, vs, table, n = both[i]
+            with torch.cuda.stream(s):
+                got[i].append(S.decode_attention(q, kc, vc, table, n, 0.1, k_scale=ks, v_scale=vs, work=works[i]))
+                got[i].append(S.prompt_attention(*p, 400, 400, 0.1))
+    torch.cuda.synchronize()
+    N.raise_on_device_error()
+    for i in range(2):
+        q, kc, vc, ks, vs, table, n = both[i]
+        O.check(got[i][0], *O.decode(q, kc, vc, table, n, 0.1, ks=ks, vs=vs))
+        assert all(torch.equal(a, got[i][0]) for a in got[i][::2]) and all(torch.equal(a, alone) for a in got[i][1::2])
+
+
+def test_more_sequences_than_a_launch_takes():
+    lens = [(37 * i) % 90 for i in range(S.MAX_SEQS + 5)]
+    q, kc, vc, ks, vs, table, n = make(4, lens, 4, 2, 64, 16, 8)
+    starts = torch.tensor([i % 5 for i in lens], dtype=I32, device=DEV)
+    work = S.decode_work(len(lens), 4, 2, 64, DEV)
+    got = S.decode_attention(q, kc, vc, table, n, 0.125, starts=starts, k_scale=ks, v_scale=vs, work=work)
+    O.check(got, *O.decode(q, kc, vc, table, n, 0.125, starts=starts, ks=ks, vs=vs))
+
+
+@pytest.mark.parametrize("cap", [2.0 ** -20, 0.01, 1024.0])
+def test_the_smallest_and_largest_caps(cap):
+    q, k, v, cq, ck = packed(5, [200, 70], [200, 90], 4, 2, 64, 4.0)
+    O.check(S.prompt_attention(q, k, v, cq, ck, 200, 200, 0.125, S.ScoreRules(cap)), *O.prompt(q, k, v, cq, ck, 0.125, cap))
+    q, kc, vc, _, _, table, n = make(6, [300, 65], 8, 2, 64, 16, 16, gain=4.0)
+    O.check(S.decode_attention(q, kc, vc, table, n, 0.125, S.ScoreRules(cap)), *O.decode(q, kc, vc, table, n, 0.125, cap))
+
+
+def test_a_workspace_of_other_shapes_is_refused():
+    """Room for as many channels is not room for as many rows."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([4], [300], 0, [9] * 4, 8, 2, 64, 16, 16, 0.0, False))
+    half = S.SharedPrefix(sh.cu_rows, sh.lens, 4, 300)
+    for work in (S.decode_work(2, 8, 2, 128, DEV, half), S.decode_work(4, 8, 2, 64, DEV), S.decode_work(1, 8, 2, 64, DEV, sh)):
+        with pytest.raises(ValueError, match="workspace"):
+            S.decode_attention(q, kc, vc, table, n, scale, shared=sh, work=work)
+    wide = S.decode_work(4, 8, 2, 128, DEV, sh)
+    wide.own_ml, wide.counters = wide.own_ml[:8], torch.zeros(64, dtype=I32, device=DEV)
+    with pytest.raises(ValueError, match="workspace"):
+        S.decode_attention(q, kc, vc, table, n, scale, shared=sh, work=wide)
+
+
+@pytest.mark.parametrize("bits,page", [(8, 16), (4, 16), (16, 24)])
+def test_a_prefix_longer_than_told_sets_the_status(bits, page):
+    """120 keys where 100 were told: both end in the same block of 128."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([4], [120], 0, [9] * 4, 8, 2, 64, page, bits, 0.0, False))
+    N.raise_on_device_error()
+    S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=S.SharedPrefix(sh.cu_rows, sh.lens, 4, 100))
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_groups_past_the_batch_share_nothing(bits):
+    """A plan of more rows than the batch has."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([4], [120], 0, [9] * 4, 8, 2, 64, 16, bits, 0.0, False))
+    plan = S.SharedPrefix(torch.tensor([0, 4, 9, 12], dtype=I32, device=DEV), torch.tensor([120, 64, 64], dtype=I32, device=DEV), 5, 120)
+    got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=plan)
+    N.raise_on_device_error()
+    O.check(got, *O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[120] * 4 if bits == 8 else None))
+
+
+@pytest.mark.parametrize("bits,page", [(16, 16), (16, 24), (8, 16)])
+def test_a_page_outside_the_cache_of_a_shared_prefix(bits, page):
+    """It is read as zeros, and the status says so."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([4], [192], 0, [9] * 4, 8, 2, 64, page, bits, 0.0, False))
+    N.raise_on_device_error()
+    held = table[0, 1].long()
+    table[:, 1] = kc.shape[0] + 7
+    got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=sh)
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+    table[:, 1] = held
+    kc[held] = 0
+    vc[held] = 0
+    O.check(got, *O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[192] * 4 if bits == 8 else None))
+
+
+def test_rows_read_back_stay_inside_the_output():
+    planes = Q.quant_planes(4, 8, 2, 64, 8, DEV)
+    x = torch.randn(32, 2, 64, device=DEV).to(BF16)
+    Q.kv_write_quant(x, x, torch.arange(32, device=DEV), *planes)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=I32, device=DEV)
+    whole = Q.kv_gather_quant(*planes, table, cu([10, 10]), 20)[0]
+    N.raise_on_device_error()
+    out = [torch.full((40, 2, 64), 5.0, dtype=BF16, device=DEV) for _ in range(2)]
+    view = tuple(t[:24] for t in out)
+    Q.kv_gather_quant(*planes, table, cu([10, 10]), 20, out=view, out_cu=torch.tensor([0, 18], dtype=I32, device=DEV))
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+    for t in out:
+        assert torch.equal(t[:10], whole[:10]) and torch.equal(t[18:24], whole[10:16]) and (t[10:18] == 5).all() and (t[24:] == 5).all()
+    # rows before the first sequence's are nobody's
+    out = [torch.full((20, 2, 64), 5.0, dtype=BF16, device=DEV) for _ in range(2)]
+    Q.kv_gather_quant(*planes, table, torch.tensor([3, 13, 20], dtype=I32, device=DEV), 20, out=tuple(out))
+    N.raise_on_device_error()
+    for t in out:
+        assert (t[:3] == 5).all() and torch.equal(t[3:13], whole[:10]) and torch.equal(t[13:20], whole[10:17])
+
+
+def test_a_step_over_integer_pages():
+    """Prompts of two sequences, their rows kept as 8 bits, then single rows: written, read back and attended."""
+    lens, Hq, Hkv, D, page = [130, 61], 8, 2, 128, 16
+    q, k, v, cq, ck = packed(8, lens, lens, Hq, Hkv, D)
+    rules = S.ScoreRules(50.0)
+    O.check(S.prompt_attention(q, k, v, cq, ck, 130, 130, 0.1, rules), *O.prompt(q, k, v, cq, ck, 0.1, 50.0))
+    planes = Q.quant_planes(16, page, Hkv, D, 8, DEV)
+    table = torch.randperm(16, device=DEV).view(2, 8).to(I32)
+    lens = [100, 61]
+    rows = torch.cat([torch.arange(100), 130 + torch.arange(61)]).to(DEV)
+    pos = torch.cat([torch.arange(n) for n in lens]).to(DEV)
+    seq = torch.repeat_interleave(torch.arange(2), torch.tensor(lens)).to(DEV)
+    slots = table[seq, pos // page].long() * page + pos % page
+    Q.kv_write_quant(k[rows], v[rows], slots, *planes)
+    n = torch.tensor(lens, dtype=I32, device=DEV)
+    for step in range(3):
+        x = torch.randn(2, 3, max(Hq, Hkv), D, device=DEV).to(BF16)
+        at = n.long()
+        Q.kv_write_quant(x[:, 1, :Hkv], x[:, 2, :Hkv], table[torch.arange(2, device=DEV), at // page].long() * page + at % page, *planes)
+        n += 1
+        got = S.decode_attention(x[:, 0, :Hq], planes[0], planes[1], table, n, 0.1, rules, k_scale=planes[2], v_scale=planes[3])
+        O.check(got, *O.decode(x[:, 0, :Hq].contiguous(), planes[0], planes[1], table, n, 0.1, 50.0, ks=planes[2], vs=planes[3]))
+    N.raise_on_device_error()

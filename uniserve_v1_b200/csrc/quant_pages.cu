@@ -135,7 +135,7 @@ struct ReadArgs {
   const int *table, *cu, *out_cu;
   __nv_bfloat16 *ko, *vo;
   long long ldo;
-  int B, max_pages, pages, page, heads, dim, total;
+  int B, max_pages, pages, page, heads, dim, total, out_rows;
   unsigned int* status;
 };
 
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
   if (threadIdx.x < ROWS) {
     const int r = r0 + threadIdx.x;
     long long s = -1, w = 0, d = -1;
-    if (r < min(a.total, a.cu[a.B])) {
+    if (r >= a.cu[0] && r < min(a.total, a.cu[a.B])) {
       int lo = 0, hi = a.B - 1;                 // sequence of packed row r
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -196,7 +196,12 @@ __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
       }
       const int pos = r - a.cu[lo], pi = pos / a.page;
       const int pg = pi < a.max_pages ? a.table[(long long)lo * a.max_pages + pi] : -1;
-      d = ((a.out_cu ? a.out_cu[lo] : a.cu[lo]) + pos) * a.ldo;
+      const int to = (a.out_cu ? a.out_cu[lo] : a.cu[lo]) + pos;
+      d = to * a.ldo;
+      if (to < 0 || to >= a.out_rows) {
+        d = -1;
+        us_dev_fail(a.status, US_DEV_BOUNDS);
+      }
       if (pg >= 0 && pg < a.pages) {
         s = ((long long)pg * a.page + (pos - pi * a.page)) * a.heads * (a.dim * BITS / 8);
         w = ((long long)pg * a.heads * a.page + (pos - pi * a.page)) * (a.dim >> 6);
@@ -264,6 +269,12 @@ struct PrefixArgs {
 };
 
 __device__ __forceinline__ float power_of_two(int field) { return __uint_as_float((uint32_t)min(max(field, 0), 254) << 23); }
+// rows of a group's prefix; a longer one than the host was told ends there
+__device__ __forceinline__ int prefix_rows(const PrefixArgs& a, int g) {
+  if (a.cu_rows[g + 1] <= a.cu_rows[g] || (unsigned)a.cu_rows[g] >= (unsigned)a.batch) return 0;
+  if (a.shared[g] > a.max_len) us_dev_fail(a.status, US_DEV_BOUNDS);
+  return min(a.shared[g], a.max_len);
+}
 // slot of position `pos` of a group's prefix, or -1
 __device__ __forceinline__ long long prefix_slot(const PrefixArgs& a, int g, int pos) {
   const int pi = pos / a.page;
@@ -281,7 +292,7 @@ __global__ void __launch_bounds__(512) prefix_scales_kernel(const PrefixArgs a) 
   if ((int)blockIdx.x < a.groups * a.heads) {
     __shared__ uint32_t most[2][16];
     const int g = blockIdx.x / a.heads, head = blockIdx.x - g * a.heads, groups = a.dim >> 6;
-    const int len = a.cu_rows[g + 1] > a.cu_rows[g] ? min(a.shared[g], a.max_len) : 0;
+    const int len = prefix_rows(a, g);
     uint32_t k = 0, v = 0;
 #pragma unroll 4
     for (int pos = threadIdx.x; pos < len; pos += 512) {
@@ -327,7 +338,7 @@ template <int BITS>
 __global__ void __launch_bounds__(256) prefix_expand_kernel(const PrefixArgs a) {
   US_PDL_PROLOGUE();
   const int g = blockIdx.y, r0 = blockIdx.x * kReadRows;
-  const int len = a.cu_rows[g + 1] > a.cu_rows[g] ? min(a.shared[g], a.max_len) : 0;
+  const int len = prefix_rows(a, g);
   if (r0 >= len) return;
   __shared__ long long src[kReadRows];
   if (threadIdx.x < kReadRows) src[threadIdx.x] = r0 + (int)threadIdx.x < len ? prefix_slot(a, g, r0 + threadIdx.x) : -1;
@@ -398,17 +409,18 @@ US_API int us_quant_write(const void* k, const void* v, long long ldk, long long
 }
 
 // The first cu[s + 1] - cu[s] cached rows of every sequence as bf16 rows [total, heads, dim] (row pitch ldo), packed,
-// or from row out_cu[s] on.  Rows past cu[B] are not written; a page outside the cache is read as zeros and sets the status word.
+// or from row out_cu[s] on.  Rows past cu[B] are not written; a page outside the cache is read as zeros and sets the status word, as
+// does a row outside the out_rows of the outputs, which is not written.
 US_API int us_quant_gather(const void* kc, const void* vc, const void* ks, const void* vs, const int* table,
                            int max_pages, const int* cu, const int* out_cu, int B, int total, int pages, int page,
-                           int heads, int dim, int bits, void* ko, void* vo, long long ldo, void* stream_) {
+                           int heads, int dim, int bits, void* ko, void* vo, long long ldo, int out_rows, void* stream_) {
   US_REQUIRE(B >= 0 && total >= 0 && pages >= 1 && page >= 1 && heads >= 1 && dim >= 64 && dim % 64 == 0 &&
              (bits == 8 || bits == 4) && max_pages >= 0);
   if (B == 0 || total == 0) return US_OK;
   US_REQUIRE(kc && vc && ks && vs && table && cu && ko && vo && (ldo % 8) == 0);
   US_REQUIRE(aligned16(kc) && aligned16(vc) && aligned16(ko) && aligned16(vo));
   const ReadArgs a{(const uint8_t*)kc, (const uint8_t*)vc, (const __nv_bfloat16*)ks, (const __nv_bfloat16*)vs, table, cu,
-                   out_cu, (__nv_bfloat16*)ko, (__nv_bfloat16*)vo, ldo, B, max_pages, pages, page, heads, dim, total,
+                   out_cu, (__nv_bfloat16*)ko, (__nv_bfloat16*)vo, ldo, B, max_pages, pages, page, heads, dim, total, out_rows,
                    us_status_ptr()};
   // 64 rows a block share one wait for their places; few rows are spread over more blocks
   const bool many = total >= 16384;

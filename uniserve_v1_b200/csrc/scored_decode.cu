@@ -957,7 +957,7 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
       }
       item -= KS;
     }
-    if (round == 1 || (!cut[0].at && !cut[1].at)) return;
+    if (round == 1 || (!cut[0].at && !cut[1].at)) break;
     __threadfence();
     __syncthreads();
     if (tid < 2) {
@@ -976,7 +976,7 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
     }
     __syncthreads();
     const int n0 = flag[0], n1 = flag[1];
-    if (n0 + n1 == 0) return;
+    if (n0 + n1 == 0) break;
     __threadfence();
     auto part_of = [&](int c, int begin) { return cta_parts + ((long long)c * 2 + (start_of(c * active) > begin ? 0 : 1)) * kPart; };
     if (n0 + n1 <= 8) {
@@ -1015,6 +1015,9 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
       if (lane == 0) parts[2 * warp + x] = p;
     }
   }
+  // beside the launch of the shared prefixes: this one is complete no sooner than that one, so the one that joins them finds
+  // both (one thread's wait is enough; one of every CTA cost 64 rows behind two prefixes 4 us of 54)
+  if (a.groups > 0 && cta == 0 && tid == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Rows of a batch with shared prefixes: what the decode launch left of a row and the parts of its group's prefix.

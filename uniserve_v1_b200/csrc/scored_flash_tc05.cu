@@ -157,6 +157,13 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     q0 = pair * 2 * per;
     k_start = seq * a.key_stride;
     kv_len = (int)min((long long)a.shared[seq], a.key_stride > 0 ? (long long)a.key_stride : (long long)a.max_pages * a.page);
+    // packed keys: pages outside the cache and prefixes longer than told were left out of them
+    if (a.key_stride > 0 && part == 0 && blockIdx.y == 0 && q_len > 0) {
+      bool bad = a.shared[seq] > a.key_stride;
+      for (int pi = threadIdx.x; pi * a.page < kv_len; pi += kThreads)
+        bad |= pi >= a.max_pages || (unsigned)a.table[(long long)q_start * a.max_pages + pi] >= (unsigned)a.pages;
+      if (bad) us_dev_fail(a.status, US_DEV_BOUNDS);
+    }
     prow0 = ((((long long)seq * a.pairs + pair) * a.Hkv + hk) * a.parts + part) * (2 * kBM);
   }
   if (q0 >= q_len) return;

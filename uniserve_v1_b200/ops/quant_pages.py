@@ -27,7 +27,7 @@ GROUP = 64
 N.register_signatures({
     "us_quant_write": (I, [P, P, L, L, L, L, P, I, P, P, P, P, I, I, I, I, I, I, P]),
     "us_quant_prefix": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, P, L, I, I, P, P, P, P, P, P]),
-    "us_quant_gather": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, P, P, L, P]),
+    "us_quant_gather": (I, [P, P, P, P, P, I, P, P, I, I, I, I, I, I, I, P, P, L, I, P]),
 })
 
 
@@ -125,7 +125,9 @@ def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows
     """Cached rows of a batch as bf16 (``functional.kv_gather`` for integer pages): sequence s brings its first
     cu[s + 1] - cu[s] positions through ``page_table`` [B, max_pages] to rows [cu[s], cu[s + 1]) of the result
     ([total_rows, Hkv, D] for K and for V), or to the rows from ``out_cu[s]`` on of a larger ``out``.  cu and out_cu
-    are int32 on the device, total_rows is at least cu[B]; rows that no sequence brings are left as they were."""
+    are int32 on the device, total_rows is at least cu[B]; rows that no sequence brings are left as they were.  A page
+    outside the cache is read as zeros and sets the device status, as does a row past the end of ``out``, which is left
+    out (on the CPU both raise)."""
     bits = page_bits(kcache, vcache, k_scale, v_scale)
     pages, page, heads, _ = kcache.shape
     dim, B = k_scale.shape[3] * GROUP, page_table.shape[0]
@@ -146,6 +148,8 @@ def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows
         for s in range(B):
             pos = torch.arange(ends[s + 1] - ends[s])
             at = page_table[s, pos // page].long()
+            if len(pos) and (int(at.min()) < 0 or int(at.max()) >= pages or starts[s] + len(pos) > ko.shape[0]):
+                raise IndexError(f"sequence {s} names a page outside a cache of {pages}, or rows past the end of the output")
             for cache, scale, to in ((kcache, k_scale, ko), (vcache, v_scale, vo)):
                 to[starts[s]:starts[s] + len(pos)] = dequantise(cache[at, pos % page], scale[at, :, pos % page]).to(BF16)
         return ko, vo
@@ -155,7 +159,7 @@ def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows
     cu, out_cu = cu.contiguous(), None if out_cu is None else out_cu.contiguous()
     launch("us_quant_gather", 1, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
            page_table.data_ptr(), page_table.shape[1], cu.data_ptr(), None if out_cu is None else out_cu.data_ptr(), B, total_rows,
-           pages, page, heads, dim, bits, ko.data_ptr(), vo.data_ptr(), ko.stride(0))
+           pages, page, heads, dim, bits, ko.data_ptr(), vo.data_ptr(), ko.stride(0), min(ko.shape[0], vo.shape[0]))
     return ko, vo
 
 

@@ -15,7 +15,6 @@ where ``ScoreRules`` says so, and out_h = softmax(s) V over the keys that are vi
 On the CPU both are FP32 formulas."""
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
@@ -35,13 +34,14 @@ N.register_signatures({
 
 MAX_SEQS = 704             # sequences of one decode launch; larger batches go in slices
 MAX_KEYS = 1 << 20         # keys of a prompt's sequence
+MAX_CAP = 1024.0           # scores under a larger one lose what a tanh near 1, less 1, loses of FP32
 _TILE = 128                # rows of a tile, keys of a block of the prompt kernel
 
 
 class ScoreRules(NamedTuple):
     """What happens to a score between scale q.k and the softmax."""
-    cap: float = 0.0                            # > 0: cap * tanh(score / cap)
-    slopes: Optional[torch.Tensor] = None       # FP32 [Hq]: - slope * |position - key|
+    cap: float = 0.0                            # > 0 (2^-20 to 1024): cap * tanh(score / cap)
+    slopes: Optional[torch.Tensor] = None       # FP32 [Hq], not negative: - slope * |position - key|
     window: int = 0                             # > 0: the last `window` keys, the row's own included
 
 
@@ -95,8 +95,8 @@ def _at(t):
 
 def _check_rules(rules, Hq, at):
     cap, s, window = rules
-    if not 0.0 <= cap < math.inf or window < 0:
-        raise ValueError(f"cap {cap} and window {window} are not negative, and finite")
+    if cap and not 2.0 ** -20 <= cap <= MAX_CAP or not 0 <= window < 1 << 31:
+        raise ValueError(f"a cap is 0 (none) or in [2^-20, {MAX_CAP}], a window in [0, 2^31); got {cap}, {window}")
     if s is not None and (s.dtype != F32 or s.shape != (Hq,) or not s.is_contiguous() or s.get_device() != at):
         raise ValueError(f"slopes are a contiguous float32 [{Hq}] beside the queries; got {tuple(s.shape)} {s.dtype}")
 
@@ -366,7 +366,8 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
         pairs, parts, each = _prefix_plan(shared, Hq, Hkv, _sm_count(at))
         groups = shared.groups
         rows = groups * pairs * Hkv * parts * 2 * _TILE
-        if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.own_o.numel() < B * Hq * D:
+        if work.prefix_o is None or work.prefix_o.numel() < rows * D or work.prefix_ml.numel() < rows * 2 or \
+                work.own_o.numel() < B * Hq * D or work.own_ml.numel() < B * Hq * 2:
             raise ValueError("the workspace is of smaller shared prefixes")
         qp, k, v, back, exps, stride = q, kcache, vcache, None, None, 0
         if bits != 16:       # integer pages: the prefix is expanded once for all its readers, as FP16
@@ -377,11 +378,15 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
             from .functional import kv_gather
             stride = shared.max_len
             cu = torch.zeros(groups + 1, dtype=I32, device=q.device)
-            torch.cumsum(shared.lens.clamp(max=stride), 0, dtype=I32, out=cu[1:])
+            torch.cumsum(shared.lens.clamp(0, min(stride, page_table.shape[1] * page)), 0, dtype=I32, out=cu[1:])
             k, v = (torch.empty(groups * stride, Hkv, D, dtype=BF16, device=q.device) for _ in range(2))
-            first = page_table.index_select(0, shared.cu_rows[:-1].clamp(max=B - 1))
-            kv_gather(kcache, vcache, first, cu, groups * stride, out=(k, v),
+            first = page_table.index_select(0, shared.cu_rows[:-1].clamp(0, B - 1))
+            bad = (first < 0) | (first >= pages)       # read as zeros; the prefix launch sets the status
+            kv_gather(kcache, vcache, first.masked_fill(bad, 0), cu, groups * stride, out=(k, v),
                       out_cu=torch.arange(0, groups * stride, stride, dtype=I32, device=q.device))
+            bad = bad.repeat_interleave(page, 1)[:, :stride, None, None]
+            for t in (k, v):
+                t.view(groups, stride, Hkv, D)[:, :bad.shape[1]].masked_fill_(bad, 0)
         cu_rows, lens, po, pm = shared.cu_rows.data_ptr(), shared.lens.data_ptr(), work.prefix_o.data_ptr(), work.prefix_ml.data_ptr()
         launch("us_scored_prefix", 1, qp.data_ptr(), qp.stride(0), k.data_ptr(), pages, v.data_ptr(), page, _at(back), _at(exps),
                stride, page_table.data_ptr(), page_table.shape[1], k.shape[0], B, seq_lens.data_ptr(), cu_rows, lens, groups, Hq,
