@@ -182,3 +182,17 @@ def test_a_step_over_integer_pages():
         got = S.decode_attention(x[:, 0, :Hq], planes[0], planes[1], table, n, 0.1, rules, k_scale=planes[2], v_scale=planes[3])
         O.check(got, *O.decode(x[:, 0, :Hq].contiguous(), planes[0], planes[1], table, n, 0.1, 50.0, ks=planes[2], vs=planes[3]))
     N.raise_on_device_error()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 1, 128), (64, 1, 64), (128, 1, 64), (256, 1, 128), (20, 1, 64), (48, 2, 128), (7, 1, 128)])
+@pytest.mark.parametrize("kind", ["capped", "biased", "documents", "window", "all"])
+def test_few_new_rows_behind_histories(Hq, Hkv, D, kind):
+    """Many query heads a key head, and few rows: heads stand side by side in a tile."""
+    new, keys = [3, 1, 0, 70, 9], [700, 1, 5, 333, 1001]
+    q, k, v, cq, ck = packed(11, new, keys, Hq, Hkv, D)
+    kw = {"capped": {}, "biased": {}, "documents": dict(docs=(torch.arange(sum(keys), device=DEV) // 60).to(I32)),
+          "window": dict(prefix=torch.tensor([9, 0, 0, 130, 64], dtype=I32, device=DEV)), "all": dict(causal=False)}[kind]
+    cap, sl, window = 30.0 if kind in ("capped", "documents") else 0.0, slopes(Hq) if kind in ("biased", "all") else None, 100 if kind == "window" else 0
+    got = S.prompt_attention(q, k, v, cq, ck, 128, 1024, D ** -0.5, S.ScoreRules(cap, sl, window), **kw)
+    N.raise_on_device_error()
+    O.check(got, *O.prompt(q, k, v, cq, ck, D ** -0.5, cap, sl, window=window, **kw))

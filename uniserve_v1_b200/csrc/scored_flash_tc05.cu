@@ -3,8 +3,8 @@
 //
 //   s = scale q.k_j;  s = cap tanh(s / cap);  s -= slope |p - j|;  out = sum_j e^s v_j / sum_j e^s over visible j
 //
-// A CTA has two tiles of 128 rows and walks the 128-key blocks that any of them sees; the tensor pipe alternates
-// between the tiles, so one tile's softmax runs under the other's products.  S_X = Q_X K^T and O_X += P_X V are
+// A CTA has two tiles of 128 rows, each row one of a few query heads at one position, and walks the 128-key blocks that any
+// of them sees; the tensor pipe alternates between the tiles, so one tile's softmax runs under the other's products.  S_X = Q_X K^T and O_X += P_X V are
 // tcgen05 products with S, P and O in tensor memory (P over the first half of S), operands by TMA, one thread a row in
 // the softmax (the layout of flash_attn2_tc05.cu).  What differs:
 //
@@ -55,6 +55,7 @@ struct ScoredArgs {
   const float* slopes;
   float scale_log2;
   float poly[4], reach, scale_cap, cap_log2;  // cap: x = s (p0 + p1 s^2 + ...) where |s| <= reach
+  int pack;                                   // prompts: log2 of the query heads in a tile
   float base;                                 // what stands for every row's maximum under a small cap
   // shared prefixes
   const int *table, *lens, *cu_rows, *shared;
@@ -136,10 +137,11 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   long long prow0 = 0;
   if constexpr (MODE == 0) {
     seq = blockIdx.y;
-    h = blockIdx.x;
+    h = blockIdx.x << a.pack;                                   // the first of the tile's heads
     hk = h / share;
+    per = kBM >> a.pack;
     // under a causal mask the last rows walk the most blocks: those of all heads and sequences start first
-    q0 = (a.causal ? (int)gridDim.z - 1 - (int)blockIdx.z : (int)blockIdx.z) * 2 * kBM;
+    q0 = (a.causal ? (int)gridDim.z - 1 - (int)blockIdx.z : (int)blockIdx.z) * 2 * per;
     q_start = a.cu_q[seq];
     q_len = min(a.cu_q[seq + 1], a.Tq) - q_start;
     k_start = a.cu_k[seq];
@@ -177,7 +179,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 
   int first_known = -1;
   if constexpr (MODE == 0) {
-    const int last = min(q0 + 2 * kBM, q_len) - 1 + shift;     // position of the last row
+    const int last = min(q0 + 2 * per, q_len) - 1 + shift;     // position of the last row
     if (nb > 0 && a.causal && last >= 0 && (!a.docs || pre <= last + 1)) first_known = max(last, pre - 1) / kBN;
     else if (nb > 0 && !a.causal && !a.docs) first_known = nb - 1;
   }
@@ -219,8 +221,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
       for (int hf = 0; hf < kHalves; ++hf) {
         uint8_t* to = sQ + x * kTile + hf * kHalf;
-        if constexpr (MODE == 0) tc::tma_load_2d(to, &tmQ, q_full, h * kD + 64 * hf, q_start + q0 + x * kBM);
-        else tc::tma_load_3d(to, &tmQ, q_full, 64 * hf, hk * share, q_start + q0 + x * per);
+        tc::tma_load_3d(to, &tmQ, q_full, 64 * hf, MODE == 0 ? h : hk * share, q_start + q0 + x * per);
       }
   }
   if (warp == kMmaWarp) {
@@ -245,7 +246,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const int j = wi * 32 + lane;
     bool see = j < nb;
     if constexpr (MODE == 0) {
-      const int r0 = q0 + x * kBM, r1 = min(r0 + kBM, q_len) - 1;          // the tile's rows
+      const int r0 = q0 + x * per, r1 = min(r0 + per, q_len) - 1;          // the tile's rows
       const int pa = r0 + shift, pb = r1 + shift;                         // and their positions
       const int k0 = j * kBN, k1 = min(k0 + kBN, kv_len);
       see &= r0 < q_len;
@@ -275,9 +276,9 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   const int taken_a = taken[0], taken_b = taken[1];
 
   if (MODE == 0 && tid < 2 * kBM) {    // rows that see nothing
-    const int x = tid >> 7, qi = q0 + tid;
+    const int x = tid >> 7, qi = q0 + (tid >> a.pack), head = h + (tid & ((1 << a.pack) - 1));
     if ((x ? taken_b : taken_a) == 0 && qi < q_len) {
-      uint4* dst = reinterpret_cast<uint4*>(a.out + (long long)(q_start + qi) * a.ldo + (long long)h * kD);
+      uint4* dst = reinterpret_cast<uint4*>(a.out + (long long)(q_start + qi) * a.ldo + (long long)head * kD);
       for (int i = 0; i < kD / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
     }
   }
@@ -430,12 +431,12 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const uint32_t o_tmem = tmem_base + 256 + (uint32_t)x * kD + lane_addr;
       // the row: its position, its visible keys [lo, hi) and [0, pr), its document.  (Rows behind the last one have all that
       // of the last one, so that no warp takes another path for them: a ragged batch 219 -> 211 us.)
-      int p, lo = 0, hi, pr = 0, doc = 0, row = 0;
+      int p, lo = 0, hi, pr = 0, doc = 0;
       float sl = 0.f;
       bool row_ok;
       [[maybe_unused]] int b_row = 0, head = 0;
       if constexpr (MODE == 0) {
-        row = q0 + x * kBM + r;
+        const int row = q0 + x * per + (r >> a.pack);
         row_ok = row < q_len;
         p = min(row, q_len - 1) + shift;
         hi = a.causal ? min(kv_len, p + 1) : kv_len;
@@ -445,7 +446,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (p >= 0 && p < kv_len) doc = a.docs[k_start + p];
           else hi = pr = 0;
         }
-        if (BIAS) sl = a.slopes[h] * kLog2e;
+        if (BIAS) sl = a.slopes[h + (r & ((1 << a.pack) - 1))] * kLog2e;
       } else {
         row_ok = r < per * share && q0 + x * per + r / share < q_len;
         b_row = q_start + min(q0 + x * per + min(r / share, per - 1), q_len - 1);
@@ -705,7 +706,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           constexpr int kPer = MODE == 0 ? 32 : 16;      // channels
           const uint32_t rows_ok = __ballot_sync(0xffffffffu, row_ok);
           uint8_t* lines = sQ + x * kTile + (warp & 3) * 2048;
-          const int row0 = x * kBM + (warp & 3) * 32 + (lane >> 2);
+          const int row0 = (warp & 3) * 32 + (lane >> 2);
 #pragma unroll
           for (int c = 0; c < kD; c += kPer) {
             __syncwarp();
@@ -729,10 +730,12 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             for (int i = 0; i < 4; ++i) {
               if (!((rows_ok >> (8 * i + (lane >> 2))) & 1u)) continue;
               const uint4 w = *reinterpret_cast<const uint4*>(lines + (8 * i + (lane >> 2)) * 64 + (((lane >> 3) ^ lane) & 3) * 16);
+              const int at = row0 + 8 * i;
               if constexpr (MODE == 0)
-                *reinterpret_cast<uint4*>(a.out + (long long)(q_start + q0 + row0 + 8 * i) * a.ldo + (long long)h * kD + c + (lane & 3) * 8) = w;
+                *reinterpret_cast<uint4*>(a.out + (long long)(q_start + q0 + x * per + (at >> a.pack)) * a.ldo +
+                                          (h + (at & ((1 << a.pack) - 1))) * kD + c + (lane & 3) * 8) = w;
               else
-                *reinterpret_cast<uint4*>(a.part_o + (prow + row0 - x * kBM + 8 * i) * kD + c + (lane & 3) * 4) = w;
+                *reinterpret_cast<uint4*>(a.part_o + (prow + at) * kD + c + (lane & 3) * 4) = w;
             }
           }
         } else {
@@ -831,8 +834,18 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   US_REQUIRE(((ldq | ldk | ldv | ldo) % 8) == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16) == 0);
   US_REQUIRE(!docs || ranges);
   US_REQUIRE(max_k <= kMaxBlocks * kBN);
+  // A tile has the largest power of two of a key head's query heads that divides them, with 128 rows shared out among
+  // them.  Few new rows behind long histories fill tiles that way (11 requests of 9 rows and 64 heads over 4 behind 3,600
+  // keys: 221 us with one head a tile, 66 so; 8 of 75 rows and 32 heads: 172, 106), and fewer blocks hang over a diagonal
+  // or a document's ends (ragged batch: 214, 197; documents: 115, 111; 4096 rows: 141, 144).  Where a bias grows fast and
+  // keys follow a row, the warp's steepest head decides for all (4096 rows that see all: 268, 293).
+  int pack = 0;
+  while (pack < 7 && (Hq / Hkv) % (2 << pack) == 0 && ((long long)max_q << (pack + 1)) <= 65535LL * 2 * kBM) ++pack;
   CUtensorMap tmQ, tmK, tmV;
-  int rc = us_tmap_2d(&tmQ, q, US_TMAP_BF16, (uint64_t)Tq, (uint64_t)Hq * D, (uint64_t)ldq, kBM, 64, US_SWZ_128);
+  const uint64_t dims[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)Tq};
+  const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)ldq * 2};
+  const uint32_t box[3] = {64, 1u << pack, (uint32_t)kBM >> pack};
+  int rc = us_tmap_encode(&tmQ, q, US_TMAP_BF16, 3, dims, strides, box, US_SWZ_128);
   if (!rc) rc = us_tmap_2d(&tmK, k, US_TMAP_BF16, (uint64_t)Tk, (uint64_t)Hkv * D, (uint64_t)ldk, kBN, 64, US_SWZ_128);
   if (!rc) rc = us_tmap_2d(&tmV, v, US_TMAP_BF16, (uint64_t)Tk, (uint64_t)Hkv * D, (uint64_t)ldv, kBN, 64, US_SWZ_128);
   if (rc) return rc;
@@ -847,6 +860,7 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   a.Hq = Hq;
   a.Hkv = Hkv;
   a.causal = causal;
+  a.pack = pack;
   a.window = window;
   a.docs = docs;
   a.prefix = prefix;
@@ -855,7 +869,7 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   set_rules(a, scale, cap, slopes);
   if (docs && max_k > 0)
     US_CUDA_CHECK(us::launch_pdl(doc_ranges_kernel, dim3(((max_k + kBN - 1) / kBN + 3) / 4, n), dim3(128), 0, stream, docs, cu_k, Tk, (int2*)ranges));
-  return start_any<0>(D, cap > 0.f, dim3(Hq, n, (max_q + 2 * kBM - 1) / (2 * kBM)), tmQ, tmK, tmV, a, stream);
+  return start_any<0>(D, cap > 0.f, dim3(Hq >> pack, n, (unsigned)((((long long)max_q << pack) + 2 * kBM - 1) / (2 * kBM))), tmQ, tmK, tmV, a, stream);
 }
 
 // The part that the shared prefixes of a decode batch have in its attention (scored_decode.cu): rows

@@ -4,6 +4,8 @@
     python -m uniserve_v1_b200.tools.opbench gemm --rows 37710 --m 5376 --k 5376
     python -m uniserve_v1_b200.tools.opbench gated --rows 37710 --m 14336 --k 5376
     python -m uniserve_v1_b200.tools.opbench decode --batch 64 --ctx 1024
+    python -m uniserve_v1_b200.tools.opbench scored --rows 4096 --q-heads 32 --causal --cap 50
+    python -m uniserve_v1_b200.tools.opbench scored-decode --batch 64 --ctx 1024 --kv int4 --cap 50
 
 Timing: CUDA events on the launching stream, warm-up first, a buffer larger than
 L2 is written between timed iterations.  Fractions are "of measured": the
@@ -54,7 +56,7 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("op", choices=["prefill", "delta", "flash", "gemm", "gated", "decode", "moe", "fused-norm",
                                    "ulysses", "tp", "moe-fp8", "gemm-fp8", "gemm-fp8t", "ep",
-                                   "rank-decode"])
+                                   "rank-decode", "scored", "scored-decode"])
     ap.add_argument("--tp", type=int, default=8, help="rank-decode: ranks of the emulated layout")
     ap.add_argument("--layers", type=int, default=8)
     ap.add_argument("--splits", type=int, default=0, help="decode: KV splits (0 = heuristic)")
@@ -73,7 +75,10 @@ def main():
     ap.add_argument("--causal", action="store_true")
     ap.add_argument("--head-dim", type=int, default=128, help="flash: 128 or 64")
     ap.add_argument("--iters", type=int, default=10)
-    ap.add_argument("--kv", default="bf16", choices=["bf16", "fp8"], help="decode: page type")
+    ap.add_argument("--kv", default="bf16", choices=["bf16", "fp8", "int8", "int4"],
+                    help="page type (decode: bf16, fp8; scored-decode: bf16, int8, int4)")
+    ap.add_argument("--cap", type=float, default=0.0, help="scored, scored-decode: score cap, 0: none")
+    ap.add_argument("--bias", action="store_true", help="scored, scored-decode: distance bias")
     ap.add_argument("--persist", action="store_true",
                     help="decode: the persistent kernel (bf16 pages)")
     a = ap.parse_args()
@@ -181,6 +186,40 @@ def main():
         out.update(tp=P, layers=a.layers, batch=a.batch, ctx=a.ctx, ms_per_step=ms,
                    launches=graph.launches, ms_per_layer=ms / a.layers,
                    note="includes embedding, head and sampling once per step")
+    elif a.op in ("scored", "scored-decode"):
+        # attention whose scores are capped or biased: one prompt, or a token of `--batch` sequences over pages of 16 rows
+        from ..ops import quant_pages as Q
+        from ..ops import scored as S
+        Hq, Hkv, D = a.q_heads, a.kv_heads, a.head_dim
+        slopes = torch.tensor([2.0 ** (-8.0 * (h + 1) / Hq) for h in range(Hq)], device=dev) if a.bias else None
+        rules = S.ScoreRules(cap=a.cap, slopes=slopes)
+        if a.op == "scored":
+            T = a.rows
+            q, k, v = rnd(T, Hq, D), rnd(T, Hkv, D), rnd(T, Hkv, D)
+            cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
+            o = torch.empty_like(q)
+            ms = timeit(lambda: S.prompt_attention(q, k, v, cu, cu, T, T, 1 / math.sqrt(D), rules, a.causal, out=o), a.iters)
+            flops = 4.0 * T * T * D * Hq * (0.5 if a.causal else 1.0)
+            out.update(rows=T, q_heads=Hq, kv_heads=Hkv, head_dim=D, cap=a.cap, bias=a.bias, ms=ms, tflops=flops / ms / 1e9,
+                       frac=flops / ms / 1e9 / tfl)
+        else:
+            if a.kv == "fp8":
+                raise SystemExit("scored-decode reads bf16, int8 or int4 pages")
+            B, page = a.batch, 16
+            each = -(-a.ctx // page)
+            table = torch.randperm(B * each, generator=g, device=dev).to(torch.int32).view(B, each)
+            lens = torch.full((B,), a.ctx, dtype=torch.int32, device=dev)
+            k, v = rnd(B * each, page, Hkv, D), rnd(B * each, page, Hkv, D)
+            planes = (k, v, None, None)
+            if a.kv != "bf16":
+                planes = Q.quant_planes(B * each, page, Hkv, D, 8 if a.kv == "int8" else 4, dev)
+                Q.kv_write_quant(k.flatten(0, 1), v.flatten(0, 1), torch.arange(B * each * page, device=dev), *planes)
+            q, work = rnd(B, Hq, D), S.decode_work(B, Hq, Hkv, D, dev)
+            ms = timeit(lambda: S.decode_attention(q, planes[0], planes[1], table, lens, 1 / math.sqrt(D), rules, k_scale=planes[2],
+                                                   v_scale=planes[3], work=work), a.iters)
+            byts = sum(t.numel() * t.element_size() for t in planes if t is not None) * (a.ctx / (each * page))
+            out.update(batch=B, ctx=a.ctx, q_heads=Hq, kv_heads=Hkv, head_dim=D, kv=a.kv, cap=a.cap, bias=a.bias, us=ms * 1e3,
+                       tbs=byts / ms / 1e9, frac_memory=byts / ms / 1e9 / tbs)
     elif a.op in ("gemm", "gated"):
         x = rnd(a.rows, a.k)
         w = rnd(a.m * (2 if a.op == "gated" else 1), a.k)
