@@ -196,3 +196,34 @@ def test_few_new_rows_behind_histories(Hq, Hkv, D, kind):
     got = S.prompt_attention(q, k, v, cq, ck, 128, 1024, D ** -0.5, S.ScoreRules(cap, sl, window), **kw)
     N.raise_on_device_error()
     O.check(got, *O.prompt(q, k, v, cq, ck, D ** -0.5, cap, sl, window=window, **kw))
+
+
+@pytest.mark.parametrize("case", [
+    # new rows, keys, Hq, Hkv, D, cap, bias, causal, window, docs, prefix
+    ([1], [5000], 32, 4, 128, 0.0, False, True, 0, None, None),
+    ([37], [3001], 32, 4, 128, 50.0, False, True, 0, None, None),
+    ([200, 3], [2000, 9000], 4, 1, 64, 0.0, True, True, 0, None, None),
+    ([65], [4100], 8, 1, 128, 30.0, True, True, 1000, None, [130]),       # most parts see nothing
+    ([30, 0, 9], [2500, 40, 0], 16, 1, 64, 50.0, False, True, 0, 900, None),      # and sequences without rows or keys
+    ([100], [1500], 3, 3, 64, 0.0, False, False, 0, None, None),
+    ([50], [2600], 4, 2, 128, 0.0, True, False, 0, 500, [700]),
+    ([2000], [1500], 1, 1, 128, 30.0, True, True, 0, None, None),         # rows before the first key
+])
+def test_few_rows_over_many_keys(case):
+    """The keys go in parts; rows past the last sequence stay."""
+    new, keys, Hq, Hkv, D, cap, bias, causal, window, docs, prefix = case
+    q, k, v, cq, ck = packed(12, new + [5], keys, Hq, Hkv, D, 3.0 if cap else 1.0)
+    cq = cq[:-1].contiguous()
+    n = sum(new)
+    assert N.kernels().us_scored_flash_parts(len(new), max(new), max(keys), Hq, Hkv) > 1
+    kw = dict(causal=causal, docs=None if docs is None else (torch.arange(sum(keys), device=DEV) // docs).to(I32),
+              prefix=None if prefix is None else torch.tensor(prefix, dtype=I32, device=DEV))
+    out = torch.full_like(q, 7.0)
+    sl = slopes(Hq) if bias else None
+    got = S.prompt_attention(q, k, v, cq, ck, max(new), max(keys), D ** -0.5, S.ScoreRules(cap, sl, window), out=out, **kw)
+    N.raise_on_device_error()
+    assert got is out and (out[n:] == 7).all()
+    want, bound = O.prompt(q[:n], k, v, cq, ck, D ** -0.5, cap, sl, window=window, **kw)
+    O.check(out[:n], want, bound)
+    again = S.prompt_attention(q, k, v, cq, ck, max(new), max(keys), D ** -0.5, S.ScoreRules(cap, sl, window), **kw)
+    assert torch.equal(again[:n], out[:n])

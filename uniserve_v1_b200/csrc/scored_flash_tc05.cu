@@ -63,6 +63,7 @@ struct ScoredArgs {
   const int2* exps;                           // and exponent fields of K and V [groups * Hkv]
   int key_stride;                             // > 0: packed keys, those of group g from row g * key_stride on
   int max_pages, pages, page, batch, pairs, parts, blocks_per_part;
+  int n, max_q;                               // sequences, the longest one's rows
   float *part_o, *part_ml;
   unsigned int* status;
 };
@@ -117,27 +118,29 @@ struct Blocks {
   }
 };
 
-// MODE 0: prompts.  1: shared prefixes.
+// MODE 0: prompts.  1: shared prefixes.  2: prompts of few rows, the keys in parts.
 // FIXED: no running maximum (see set_rules).  EMU: which of every eight exponential pairs go to the polynomial.
 template <int kD, bool CAP, bool BIAS, bool FIXED, int MODE, uint32_t EMU>
 __global__ void __launch_bounds__(kThreads, 1)
 scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const ScoredArgs a) {
-  if (MODE == 0) {
+  if (MODE != 1) {
     US_PDL_PROLOGUE();
   } else {       // the launch behind this one (scored_decode.cu) does not wait: it may start once what both read is there
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   }
+  constexpr bool PROMPT = MODE != 1, PARTS = MODE != 0;
   constexpr int kHalves = kD / 64, kTile = kHalves * kHalf;
   constexpr int kTmaWarp = 8, kMmaWarp = 9;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int share = a.Hq / a.Hkv;
   int seq, h = 0, hk, q0, q_start = 0, q_len, k_start, kv_len, shift = 0, per = kBM, pre = 0, part = 0;
   long long prow0 = 0;
-  if constexpr (MODE == 0) {
+  if constexpr (PROMPT) {
     seq = blockIdx.y;
-    h = blockIdx.x << a.pack;                                   // the first of the tile's heads
+    part = MODE == 2 ? (int)blockIdx.x % a.parts : 0;
+    h = (MODE == 2 ? (int)blockIdx.x / a.parts : (int)blockIdx.x) << a.pack;      // the first of the tile's heads
     hk = h / share;
     per = kBM >> a.pack;
     // under a causal mask the last rows walk the most blocks: those of all heads and sequences start first
@@ -169,6 +172,10 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     prow0 = ((((long long)seq * a.pairs + pair) * a.Hkv + hk) * a.parts + part) * (2 * kBM);
   }
   if (q0 >= q_len) return;
+  // where a row's part is: [part][sequence][row][head]
+  auto part_row = [&](int row, int head) -> long long {
+    return ((((long long)part * a.n + seq) * a.max_q + row) * a.Hq) + head;
+  };
   kv_len = max(kv_len, 0);
   int nb = min((kv_len + kBN - 1) / kBN, kMaxBlocks), jb = 0;
   if constexpr (MODE == 1) {
@@ -178,10 +185,11 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   }
 
   int first_known = -1;
-  if constexpr (MODE == 0) {
+  if constexpr (PROMPT) {
     const int last = min(q0 + 2 * per, q_len) - 1 + shift;     // position of the last row
     if (nb > 0 && a.causal && last >= 0 && (!a.docs || pre <= last + 1)) first_known = max(last, pre - 1) / kBN;
     else if (nb > 0 && !a.causal && !a.docs) first_known = nb - 1;
+    if (MODE == 2) first_known = -1;
   }
 
   extern __shared__ uint8_t smem_raw[];
@@ -215,13 +223,13 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     tc::mbar_fence_init();
     // Q is on its way while the blocks are looked up, and so is the first block's K where it is known: the last block,
     // or that of the last row's own key (which is of its document), or the one of the prefix's end
-    tc::mbar_expect_tx(q_full, MODE == 0 ? 2 * kTile : 2 * kHalves * per * share * 128);
+    tc::mbar_expect_tx(q_full, PROMPT ? 2 * kTile : 2 * kHalves * per * share * 128);
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int hf = 0; hf < kHalves; ++hf) {
         uint8_t* to = sQ + x * kTile + hf * kHalf;
-        tc::tma_load_3d(to, &tmQ, q_full, 64 * hf, MODE == 0 ? h : hk * share, q_start + q0 + x * per);
+        tc::tma_load_3d(to, &tmQ, q_full, 64 * hf, PROMPT ? h : hk * share, q_start + q0 + x * per);
       }
   }
   if (warp == kMmaWarp) {
@@ -238,18 +246,19 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   // ---- which blocks the tiles see ----
   const int words = (nb + 31) / 32;
   const int2* ranges = nullptr;
-  if constexpr (MODE == 0) {
+  if constexpr (PROMPT) {
     if (a.docs) ranges = a.ranges + (k_start / kBN + seq);
   }
   for (int w = warp; w < 2 * words; w += kThreads / 32) {
     const int x = w >= words, wi = w - x * words;
     const int j = wi * 32 + lane;
     bool see = j < nb;
-    if constexpr (MODE == 0) {
+    if constexpr (PROMPT) {
       const int r0 = q0 + x * per, r1 = min(r0 + per, q_len) - 1;          // the tile's rows
       const int pa = r0 + shift, pb = r1 + shift;                         // and their positions
       const int k0 = j * kBN, k1 = min(k0 + kBN, kv_len);
       see &= r0 < q_len;
+      if (MODE == 2) see &= j / a.blocks_per_part == part;
       bool by_place = !a.causal || k0 <= pb;
       if (a.window > 0) by_place &= k1 - 1 > pa - a.window;
       see &= by_place || k0 < pre;
@@ -275,11 +284,15 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   const uint32_t tmem_base = *tmem_slot;
   const int taken_a = taken[0], taken_b = taken[1];
 
-  if (MODE == 0 && tid < 2 * kBM) {    // rows that see nothing
-    const int x = tid >> 7, qi = q0 + (tid >> a.pack), head = h + (tid & ((1 << a.pack) - 1));
-    if ((x ? taken_b : taken_a) == 0 && qi < q_len) {
-      uint4* dst = reinterpret_cast<uint4*>(a.out + (long long)(q_start + qi) * a.ldo + (long long)head * kD);
-      for (int i = 0; i < kD / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+  if (PROMPT && tid < 2 * kBM) {    // rows that see nothing
+    const int x = tid >> 7, row = q0 + (tid >> a.pack), head = h + (tid & ((1 << a.pack) - 1));
+    if ((x ? taken_b : taken_a) == 0 && row < q_len) {
+      if constexpr (MODE == 2) {
+        *reinterpret_cast<float2*>(a.part_ml + part_row(row, head) * 2) = make_float2(-INFINITY, 0.f);
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(a.out + (long long)(q_start + row) * a.ldo + (long long)head * kD);
+        for (int i = 0; i < kD / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+      }
     }
   }
 
@@ -435,7 +448,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       float sl = 0.f;
       bool row_ok;
       [[maybe_unused]] int b_row = 0, head = 0;
-      if constexpr (MODE == 0) {
+      if constexpr (PROMPT) {
         const int row = q0 + x * per + (r >> a.pack);
         row_ok = row < q_len;
         p = min(row, q_len - 1) + shift;
@@ -490,7 +503,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const int kbase = (jb + j) * kBN;
         // what of the block is visible to the row (looked up while the scores are computed)
         bool whole = (lo <= kbase && hi >= kbase + kBN) || pr >= kbase + kBN;
-        if (MODE == 0 && ranges) {
+        if (PROMPT && ranges) {
           const int2 d = ranges[j];
           whole &= d.x == doc && d.y == doc;
         }
@@ -500,7 +513,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             see[c] = bits_between(lo - kbase - 32 * c, hi - kbase - 32 * c) | bits_between(0, pr - kbase - 32 * c);
-          if (MODE == 0 && a.docs) {
+          if (PROMPT && a.docs) {
             int kd[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -694,16 +707,19 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (n > 0 || !ok) {
         if (ok && __all_sync(0xffffffffu, tc::mbar_wait(&o_full[x], 0, abort_flag))) {
           tc::tc_fence_after_sync();
-          const float inv = MODE == 0 ? (l_sum == 0.f ? 0.f : 1.f / l_sum) : 1.f;
+          const float inv = MODE == 0 ? (l_sum == 0.f ? 0.f : 1.f / l_sum) : out_factor;
           const long long prow = prow0 + x * kBM;
-          if (MODE == 1 && row_ok) *reinterpret_cast<float2*>(a.part_ml + (prow + r) * 2) = make_float2(m_used, l_sum);
+          if (PARTS && row_ok) {
+            const long long to = MODE == 2 ? part_row(q0 + x * per + (r >> a.pack), h + (r & ((1 << a.pack) - 1))) : prow + r;
+            *reinterpret_cast<float2*>(a.part_ml + to * 2) = make_float2(m_used, l_sum);
+          }
           uint32_t all[kD];
 #pragma unroll
           for (int c = 0; c < kD; c += 32) tc::tmem_ld32(o_tmem + c, *reinterpret_cast<uint32_t(*)[32]>(all + c));
           tc::tmem_ld_wait();
           // 64 bytes of every row at a time through shared memory (the tile's Q, which no product reads any more): eight
           // rows a store in place of 32 (4096 causal rows x 32 heads: 139 -> 133 us; short documents: 119 -> 111)
-          constexpr int kPer = MODE == 0 ? 32 : 16;      // channels
+          constexpr int kPer = PARTS ? 16 : 32;      // channels
           const uint32_t rows_ok = __ballot_sync(0xffffffffu, row_ok);
           uint8_t* lines = sQ + x * kTile + (warp & 3) * 2048;
           const int row0 = (warp & 3) * 32 + (lane >> 2);
@@ -713,15 +729,15 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint4 piece;
-              if constexpr (MODE == 0) {
+              if constexpr (!PARTS) {
                 us::Pack16 o;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) o.b[k] = us::f2bf(__uint_as_float(all[c + i * 8 + k]) * inv);
                 piece = o.u;
               } else {
                 const uint32_t* w = all + c + i * 4;
-                piece = make_uint4(__float_as_uint(__uint_as_float(w[0]) * out_factor), __float_as_uint(__uint_as_float(w[1]) * out_factor),
-                                   __float_as_uint(__uint_as_float(w[2]) * out_factor), __float_as_uint(__uint_as_float(w[3]) * out_factor));
+                piece = make_uint4(__float_as_uint(__uint_as_float(w[0]) * inv), __float_as_uint(__uint_as_float(w[1]) * inv),
+                                   __float_as_uint(__uint_as_float(w[2]) * inv), __float_as_uint(__uint_as_float(w[3]) * inv));
               }
               *reinterpret_cast<uint4*>(lines + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16) = piece;
             }
@@ -730,12 +746,11 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             for (int i = 0; i < 4; ++i) {
               if (!((rows_ok >> (8 * i + (lane >> 2))) & 1u)) continue;
               const uint4 w = *reinterpret_cast<const uint4*>(lines + (8 * i + (lane >> 2)) * 64 + (((lane >> 3) ^ lane) & 3) * 16);
-              const int at = row0 + 8 * i;
+              const int at = row0 + 8 * i, at_row = q0 + x * per + (at >> a.pack), at_head = h + (at & ((1 << a.pack) - 1));
               if constexpr (MODE == 0)
-                *reinterpret_cast<uint4*>(a.out + (long long)(q_start + q0 + x * per + (at >> a.pack)) * a.ldo +
-                                          (h + (at & ((1 << a.pack) - 1))) * kD + c + (lane & 3) * 8) = w;
+                *reinterpret_cast<uint4*>(a.out + (long long)(q_start + at_row) * a.ldo + at_head * kD + c + (lane & 3) * 8) = w;
               else
-                *reinterpret_cast<uint4*>(a.part_o + (prow + at) * kD + c + (lane & 3) * 4) = w;
+                *reinterpret_cast<uint4*>(a.part_o + (MODE == 2 ? part_row(at_row, at_head) : prow + at) * kD + c + (lane & 3) * 4) = w;
             }
           }
         } else {
@@ -772,6 +787,44 @@ __global__ void __launch_bounds__(128) doc_ranges_kernel(const int* docs, const 
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   if (lane == 0) ranges[start / kBN + seq + j] = make_int2(lo, hi);
+}
+
+// Rows whose keys went in parts: a warp a row and head.
+template <int D>
+__global__ void __launch_bounds__(256) join_parts_kernel(const ScoredArgs a) {
+  US_PDL_PROLOGUE();
+  constexpr int kC = D / 32;
+  const int lane = threadIdx.x & 31;
+  const long long rows = (long long)a.n * a.max_q * a.Hq, i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= rows) return;
+  const int head = (int)(i % a.Hq), row = (int)(i / a.Hq % a.max_q), seq = (int)(i / a.Hq / a.max_q);
+  const int start = a.cu_q[seq];
+  if (row >= min(a.cu_q[seq + 1], a.Tq) - start) return;
+  float M = -INFINITY, L = 0.f, acc[kC] = {};
+  for (int p0 = 0; p0 < a.parts; p0 += 4) {            // four parts' loads in flight
+    float2 ml[4];
+    float o[4][kC];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long long at = (long long)min(p0 + k, a.parts - 1) * rows + i;
+      ml[k] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) o[k][c] = a.part_o[at * D + lane * kC + c];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (p0 + k >= a.parts || ml[k].x == -INFINITY || ml[k].y == 0.f) continue;      // such a part may hold anything
+      const float top = fmaxf(M, ml[k].x), f = M == -INFINITY ? 0.f : ex2f(M - top), w = ex2f(ml[k].x - top);
+      M = top;
+      L = fmaf(w, ml[k].y, L * f);
+#pragma unroll
+      for (int c = 0; c < kC; ++c) acc[c] = fmaf(w, o[k][c], acc[c] * f);
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  __nv_bfloat16* to = a.out + (long long)(start + row) * a.ldo + (long long)head * D + lane * kC;
+#pragma unroll
+  for (int c = 0; c < kC; c += 2) *reinterpret_cast<__nv_bfloat162*>(to + c) = __floats2bfloat162_rn(acc[c] * inv, acc[c + 1] * inv);
 }
 
 size_t shared_bytes(int D) { return 6 * (size_t)(D / 64) * kHalf + 11 * 8 + 16 + 2 * kWords * 4 + 1024; }
@@ -823,24 +876,45 @@ int start_any(int D, bool cap, dim3 grid, const CUtensorMap& q, const CUtensorMa
 
 }  // namespace
 
+namespace {
+// A tile has the largest power of two of a key head's query heads that divides them, with 128 rows shared out among
+// them.  Few new rows behind long histories fill tiles that way (11 requests of 9 rows and 64 heads over 4 behind 3,600
+// keys: 221 us with one head a tile, 66 so; 8 of 75 rows and 32 heads: 172, 106), and fewer blocks hang over a diagonal
+// or a document's ends (ragged batch: 214, 197; documents: 115, 111; 4096 rows: 141, 144).  Where a bias grows fast and
+// keys follow a row, the warp's steepest head decides for all (4096 rows that see all: 268, 293).
+int pack_of(int share, int max_q) {
+  int pack = 0;
+  while (pack < 7 && share % (2 << pack) == 0 && ((long long)max_q << (pack + 1)) <= 65535LL * 2 * kBM) ++pack;
+  return pack;
+}
+}  // namespace
+
+// Parts that the keys of a prompt call go in: as many as fill the GPU once where few rows would leave half of it idle, of
+// four blocks or more.  Parts are joined by a launch of their own; see us_scored_flash for their places.
+US_API int us_scored_flash_parts(int n, int max_q, int max_k, int Hq, int Hkv) {
+  int sms = 0;
+  if (n < 1 || max_q < 1 || Hkv < 1 || Hq < Hkv || us::sm_count(&sms) != cudaSuccess) return 1;
+  const int pack = pack_of(Hq / Hkv, max_q), blocks = (max_k + kBN - 1) / kBN;
+  const long long ctas = (long long)(Hq >> pack) * n * ((((long long)max_q << pack) + 2 * kBM - 1) / (2 * kBM));
+  const int parts = (int)min((long long)(blocks / 4), sms / ctas);
+  if (parts < 2) return 1;
+  const int each = (blocks + parts - 1) / parts;
+  return (blocks + each - 1) / each;
+}
+
 // q [Tq, Hq, D], k / v [Tk, Hkv, D], out [Tq, Hq, D], bf16 with row pitches; cu_q / cu_k [n + 1].  docs [Tk] with ranges
-// (int32 [2 (Tk / 128 + n + 1)], written here), prefix [n], slopes [Hq]: or null.  cap 0, window 0: none.
+// (int32 [2 (Tk / 128 + n + 1)], written here), prefix [n], slopes [Hq]: or null.  cap 0, window 0: none.  parts > 1: part_o,
+// part_ml [parts][n][max_q][Hq][D and 2] take the parts' results.
 US_API int us_scored_flash(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out,
                            long long ldo, const int* cu_q, const int* cu_k, int n, int Tq, int Tk, int Hq, int Hkv, int D,
                            int max_q, int max_k, float scale, float cap, const float* slopes, int causal, int window,
-                           const int* docs, const int* prefix, void* ranges, void* stream_) {
+                           const int* docs, const int* prefix, void* ranges, int parts, float* part_o, float* part_ml, void* stream_) {
   US_REQUIRE(q && k && v && out && cu_q && cu_k && n >= 1 && n <= 65535 && Tq >= 1 && Tk >= 1 && max_q >= 1 && max_q <= 65535 * 2 * kBM && max_k >= 0);
   US_REQUIRE((D == 64 || D == 128) && Hkv >= 1 && Hq >= 1 && Hq <= 65535 && Hq % Hkv == 0 && window >= 0 && cap >= 0.f);
   US_REQUIRE(((ldq | ldk | ldv | ldo) % 8) == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16) == 0);
   US_REQUIRE(!docs || ranges);
-  US_REQUIRE(max_k <= kMaxBlocks * kBN);
-  // A tile has the largest power of two of a key head's query heads that divides them, with 128 rows shared out among
-  // them.  Few new rows behind long histories fill tiles that way (11 requests of 9 rows and 64 heads over 4 behind 3,600
-  // keys: 221 us with one head a tile, 66 so; 8 of 75 rows and 32 heads: 172, 106), and fewer blocks hang over a diagonal
-  // or a document's ends (ragged batch: 214, 197; documents: 115, 111; 4096 rows: 141, 144).  Where a bias grows fast and
-  // keys follow a row, the warp's steepest head decides for all (4096 rows that see all: 268, 293).
-  int pack = 0;
-  while (pack < 7 && (Hq / Hkv) % (2 << pack) == 0 && ((long long)max_q << (pack + 1)) <= 65535LL * 2 * kBM) ++pack;
+  US_REQUIRE(max_k <= kMaxBlocks * kBN && parts >= 1 && (parts == 1 || (part_o && part_ml)));
+  const int pack = pack_of(Hq / Hkv, max_q);
   CUtensorMap tmQ, tmK, tmV;
   const uint64_t dims[3] = {(uint64_t)D, (uint64_t)Hq, (uint64_t)Tq};
   const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)ldq * 2};
@@ -869,7 +943,20 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   set_rules(a, scale, cap, slopes);
   if (docs && max_k > 0)
     US_CUDA_CHECK(us::launch_pdl(doc_ranges_kernel, dim3(((max_k + kBN - 1) / kBN + 3) / 4, n), dim3(128), 0, stream, docs, cu_k, Tk, (int2*)ranges));
-  return start_any<0>(D, cap > 0.f, dim3(Hq >> pack, n, (unsigned)((((long long)max_q << pack) + 2 * kBM - 1) / (2 * kBM))), tmQ, tmK, tmV, a, stream);
+  const unsigned tiles = (unsigned)((((long long)max_q << pack) + 2 * kBM - 1) / (2 * kBM));
+  if (parts == 1) return start_any<0>(D, cap > 0.f, dim3(Hq >> pack, n, tiles), tmQ, tmK, tmV, a, stream);
+  a.parts = parts;
+  a.blocks_per_part = ((max_k + kBN - 1) / kBN + parts - 1) / parts;
+  a.part_o = part_o;
+  a.part_ml = part_ml;
+  a.n = n;
+  a.max_q = max_q;
+  rc = start_any<2>(D, cap > 0.f, dim3((Hq >> pack) * parts, n, tiles), tmQ, tmK, tmV, a, stream);
+  if (rc) return rc;
+  const long long rows = (long long)n * max_q * Hq;
+  US_REQUIRE(rows < (1LL << 31));
+  US_CUDA_CHECK(us::launch_pdl(D == 128 ? join_parts_kernel<128> : join_parts_kernel<64>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream, a));
+  return US_OK;
 }
 
 // The part that the shared prefixes of a decode batch have in its attention (scored_decode.cu): rows

@@ -28,13 +28,15 @@ N.register_signatures({
     "us_scored_decode_scratch": (L, [I]),
     "us_scored_decode": (I, [P, L, P, P, P, P, P, I, P, P, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, P, P, P, P,
                              P, P, I, I, I, P]),
-    "us_scored_flash": (I, [P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, I, P, P, P, P]),
+    "us_scored_flash": (I, [P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, I, P, P, P, I, P, P, P]),
+    "us_scored_flash_parts": (I, [I, I, I, I, I]),
     "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
 })
 
 MAX_SEQS = 704             # sequences of one decode launch; larger batches go in slices
 MAX_KEYS = 1 << 20         # keys of a prompt's sequence
 MAX_CAP = 1024.0           # scores under a larger one lose what a tanh near 1, less 1, loses of FP32
+_FEW_ROWS = 1 << 15        # rows times heads: more of them have tiles for over half of a GPU
 _TILE = 128                # rows of a tile, keys of a block of the prompt kernel
 
 
@@ -179,9 +181,16 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
         if not (cu_q.is_contiguous() and cu_k.is_contiguous()):
             cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
         prefix = None if prefix is None else prefix.contiguous()
-        launch("us_scored_flash", 1 if docs is None else 2, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0),
+        parts, po, pm = 1, None, None
+        if max_k > 8 * _TILE and n * max_q * Hq <= _FEW_ROWS:      # few rows over many keys: the keys in parts
+            parts = N.kernels().us_scored_flash_parts(n, max_q, max_k, Hq, Hkv)
+            if parts > 1:
+                po = torch.empty(parts * n * max_q * Hq * D, dtype=F32, device=q.device)
+                pm = torch.empty(parts * n * max_q * Hq * 2, dtype=F32, device=q.device)
+        launch("us_scored_flash", 1 + (docs is not None) + (parts > 1), q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0),
                v.data_ptr(), v.stride(0), to.data_ptr(), to.stride(0), cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, Hq, Hkv, D,
-               max_q, max_k, scale, rules.cap, _at(rules.slopes), causal, rules.window, _at(docs), _at(prefix), _at(ranges))
+               max_q, max_k, scale, rules.cap, _at(rules.slopes), causal, rules.window, _at(docs), _at(prefix), _at(ranges), parts, _at(po),
+               _at(pm))
     if out is not None and to is not out:
         return out.copy_(to)
     return to
