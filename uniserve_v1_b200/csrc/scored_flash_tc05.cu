@@ -890,7 +890,8 @@ int pack_of(int share, int max_q) {
 }  // namespace
 
 // Parts that the keys of a prompt call go in: as many as fill the GPU once where few rows would leave half of it idle, of
-// four blocks or more.  Parts are joined by a launch of their own; see us_scored_flash for their places.
+// four blocks or more (37 rows of 32 heads over 8,000 keys: 107 us in one part, 28 in 36; 200 rows over 16,000: 111, 42).
+// Parts are joined by a launch of their own; see us_scored_flash for their places.
 US_API int us_scored_flash_parts(int n, int max_q, int max_k, int Hq, int Hkv) {
   int sms = 0;
   if (n < 1 || max_q < 1 || Hkv < 1 || Hq < Hkv || us::sm_count(&sms) != cudaSuccess) return 1;
