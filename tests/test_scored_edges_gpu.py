@@ -227,3 +227,32 @@ def test_few_rows_over_many_keys(case):
     O.check(out[:n], want, bound)
     again = S.prompt_attention(q, k, v, cq, ck, max(new), max(keys), D ** -0.5, S.ScoreRules(cap, sl, window), **kw)
     assert torch.equal(again[:n], out[:n])
+
+
+@pytest.mark.parametrize("told_q,told_k", [(37, 3000), (60, 1100)])
+def test_rows_and_keys_past_what_was_told_set_the_status(told_q, told_k):
+    """60 and 12 rows over 3000 and 2000 keys.  Rows that were told of are whole where their keys are."""
+    q, k, v, cq, ck = packed(13, [12, 60], [2000, 3000], 32, 4, 128)
+    assert N.kernels().us_scored_flash_parts(2, told_q, told_k, 32, 4) > 1
+    N.raise_on_device_error()
+    guard = torch.full((q.shape[0] + 64, 32, 128), 7.0, dtype=BF16, device=DEV)
+    got = S.prompt_attention(q, k, v, cq, ck, told_q, told_k, 0.1, out=guard[:72])
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+    assert (guard[72:] == 7).all()
+    if told_k == 3000:
+        want, bound = O.prompt(q, k, v, cq, ck, 0.1)
+        for rows in (slice(0, 12), slice(12, 12 + told_q)):
+            O.check(got[rows], want[rows], bound[rows])
+
+
+def test_longer_sequences_than_told_under_documents_set_the_status():
+    q, k, v, cq, ck = packed(14, [300], [700], 4, 2, 128)
+    docs = (torch.arange(700, device=DEV) // 50).to(I32)
+    N.raise_on_device_error()
+    S.prompt_attention(q, k, v, cq, ck, 300, 500, 0.1, docs=docs)
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+    got = S.prompt_attention(q, k, v, cq, ck, 300, 700, 0.1, docs=docs)
+    N.raise_on_device_error()
+    O.check(got, *O.prompt(q, k, v, cq, ck, 0.1, docs=docs))

@@ -63,7 +63,7 @@ struct ScoredArgs {
   const int2* exps;                           // and exponent fields of K and V [groups * Hkv]
   int key_stride;                             // > 0: packed keys, those of group g from row g * key_stride on
   int max_pages, pages, page, batch, pairs, parts, blocks_per_part;
-  int n, max_q;                               // sequences, the longest one's rows
+  int n, max_q, max_k;                        // sequences, the longest one's rows and keys
   float *part_o, *part_ml;
   unsigned int* status;
 };
@@ -151,6 +151,13 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     kv_len = min(a.cu_k[seq + 1] - k_start, a.Tk - k_start);
     shift = (a.cu_k[seq + 1] - k_start) - (a.cu_q[seq + 1] - q_start);
     if (a.prefix) pre = max(0, min(a.prefix[seq], kv_len));
+    // rows and keys past what the host was told of the longest sequence: some or all are left out
+    bool short_of = q_len > (int)gridDim.z * 2 * per || kv_len > a.max_k;
+    if (MODE == 2) {
+      short_of |= q_len > a.max_q;
+      q_len = min(q_len, a.max_q);
+    }
+    if (short_of && tid == 0) us_dev_fail(a.status, US_DEV_BOUNDS);
   } else {
     seq = blockIdx.z;
     hk = blockIdx.y % a.Hkv;
@@ -936,6 +943,9 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   a.Hkv = Hkv;
   a.causal = causal;
   a.pack = pack;
+  a.n = n;
+  a.max_q = max_q;
+  a.max_k = max_k;
   a.window = window;
   a.docs = docs;
   a.prefix = prefix;
@@ -950,8 +960,6 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   a.blocks_per_part = ((max_k + kBN - 1) / kBN + parts - 1) / parts;
   a.part_o = part_o;
   a.part_ml = part_ml;
-  a.n = n;
-  a.max_q = max_q;
   rc = start_any<2>(D, cap > 0.f, dim3((Hq >> pack) * parts, n, tiles), tmQ, tmK, tmV, a, stream);
   if (rc) return rc;
   const long long rows = (long long)n * max_q * Hq;
