@@ -950,7 +950,9 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   a.n = n;
   a.max_q = max_q;
   a.max_k = max_k;
-  a.window = window;
+  // (a window of all keys that a sequence may have is none; rows stand before the first key too, and their positions less the
+  // window have to be 32-bit numbers)
+  a.window = window < kMaxBlocks * kBN ? window : kMaxBlocks * kBN;
   a.docs = docs;
   a.prefix = prefix;
   a.ranges = (const int2*)ranges;
