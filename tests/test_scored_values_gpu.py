@@ -1,0 +1,82 @@
+"""Scored attention over values that are not numbers: what they reach is not a number either, however the keys were split,
+and they reach nothing else."""
+import pytest
+import torch
+
+import scored_oracle as O
+from test_scored_decode_gpu import make, slopes
+from test_scored_flash_gpu import cu, packed, shared_batch
+from uniserve_v1_b200.ops import native as N
+from uniserve_v1_b200.ops import scored as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, I32 = torch.bfloat16, torch.int32
+NAN = float("nan")
+
+
+def check_but(got, want, bound, lost):
+    """`lost` [rows, heads]: rows that are NaN in every channel; the others are within their bounds."""
+    assert got[lost].isnan().all(), f"finite where it cannot be: {torch.nonzero(~got[lost].isnan())[:4].tolist()}"
+    O.check(got[~lost], want[~lost], bound[~lost])
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (64, 4, 64)])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_a_query_that_is_not_a_number_over_many_keys(bits, Hq, Hkv, D, cap):
+    """Its pair is spread over many warps and CTAs."""
+    q, kc, vc, ks, vs, table, n = make(31, [9000, 33, 4000], Hq, Hkv, D, 16, bits)
+    sl = slopes(Hq)
+    want, bound = O.decode(q, kc, vc, table, n, 0.1, cap, sl, ks=ks, vs=vs)
+    lost = torch.zeros(3, Hq, dtype=torch.bool, device=DEV)
+    lost[0, 1] = lost[1, Hq - 1] = lost[2, 0] = True
+    q[lost] = NAN
+    got = S.decode_attention(q, kc, vc, table, n, 0.1, S.ScoreRules(cap, sl), k_scale=ks, v_scale=vs)
+    N.raise_on_device_error()
+    check_but(got, want, bound, lost)
+
+
+@pytest.mark.parametrize("length", [33, 65, 129, 4097])
+@pytest.mark.parametrize("D,bits", [(128, 16), (64, 16), (128, 8), (64, 8), (128, 4)])
+def test_the_newest_key_is_not_a_number(length, D, bits):
+    """It is alone in its tile, and that tile may be a warp's whole range."""
+    q, kc, vc, ks, vs, table, n = make(32, [length, 20], 8, 2, D, 16, bits)
+    want, bound = O.decode(q, kc, vc, table, n, 0.1, ks=ks, vs=vs)
+    page, at = table[0, (length - 1) // 16].long(), (length - 1) % 16
+    if bits == 16:
+        kc[page, at, 1] = NAN
+    else:
+        ks[page, 1, at] = NAN
+    got = S.decode_attention(q, kc, vc, table, n, 0.1, k_scale=ks, v_scale=vs)
+    N.raise_on_device_error()
+    lost = torch.zeros(2, 8, dtype=torch.bool, device=DEV)
+    lost[0, 4:] = True
+    check_but(got, want, bound, lost)
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0, 100.0])
+def test_prompts_whose_keys_go_in_parts(cap):
+    q, k, v, cu_q, cu_k = packed(33, [37, 3], [6000, 3000], 8, 2, 128)
+    assert N.kernels().us_scored_flash_parts(2, 37, 6000, 8, 2) > 1
+    want, bound = O.prompt(q, k, v, cu_q, cu_k, 0.1, cap)
+    lost = torch.zeros(40, 8, dtype=torch.bool, device=DEV)
+    lost[0, 3] = lost[36, 0] = lost[39, 7] = True
+    q[lost] = NAN
+    got = S.prompt_attention(q, k, v, cu_q, cu_k, 37, 6000, 0.1, S.ScoreRules(cap))
+    N.raise_on_device_error()
+    check_but(got, want, bound, lost)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_shared_prefixes(bits, cap):
+    case = ([5, 3], [1500, 700], 1, [40, 1, 0, 200, 17, 5, 9, 1000, 3], 8, 2, 64, 16, bits, cap, False)
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(case)
+    want, bound = O.decode(q, kc, vc, table, n, scale, cap, ks=ks, vs=vs, expanded=[1500] * 5 + [700] * 3 + [0] if ks is not None else None)
+    lost = torch.zeros(9, 8, dtype=torch.bool, device=DEV)
+    lost[1, 2] = lost[2, 5] = lost[8, 0] = True          # one without keys of its own, one that shares nothing
+    q[lost] = NAN
+    got = S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(cap), k_scale=ks, v_scale=vs, shared=sh)
+    N.raise_on_device_error()
+    check_but(got, want, bound, lost)

@@ -784,7 +784,8 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
     w = ex2(x - top);
     M = top;
   };
-  // accumulator tile t of up to four parts into acc under maxima M with sums L (a maximum of -inf: no key has a weight)
+  // accumulator tile t of up to four parts into acc under maxima M with sums L.  A maximum of -inf: no key has a weight and the
+  // sum is zero, or no score is a number and the sum is none, which then is the pair's sum too (its outputs may hold anything).
   auto add_parts = [&](const float* (&at)[4], int t, float (&acc)[1][NT][4], float (&M)[NT][2], float (&L)[NT][2]) {
     float4 v[4][NT], p[4][NT];
 #pragma unroll
@@ -802,13 +803,17 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f, w;
-        if (v[k][nt].x != -INFINITY) {
+        if (v[k][nt].x == -INFINITY) {
+          L[nt][0] += v[k][nt].y;
+        } else {
           join(v[k][nt].x, M[nt][0], f, w);
           L[nt][0] = fmaf(w, v[k][nt].y, L[nt][0] * f);
           acc[0][nt][0] = fmaf(w, p[k][nt].x, acc[0][nt][0] * f);
           acc[0][nt][2] = fmaf(w, p[k][nt].z, acc[0][nt][2] * f);
         }
-        if (v[k][nt].z != -INFINITY) {
+        if (v[k][nt].z == -INFINITY) {
+          L[nt][1] += v[k][nt].w;
+        } else {
           join(v[k][nt].z, M[nt][1], f, w);
           L[nt][1] = fmaf(w, v[k][nt].w, L[nt][1] * f);
           acc[0][nt][1] = fmaf(w, p[k][nt].y, acc[0][nt][1] * f);
@@ -827,7 +832,10 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float x = e ? v.z : v.x;
-        if (x == -INFINITY) continue;
+        if (x == -INFINITY) {
+          L[nt][e] += e ? v.w : v.y;
+          continue;
+        }
         float f, w;
         join(x, M[nt][e], f, w);
         L[nt][e] = fmaf(w, e ? v.w : v.y, L[nt][e] * f);
@@ -1045,8 +1053,7 @@ __global__ void __launch_bounds__(256) scored_merge_kernel(const MergeArgs a) {
 #pragma unroll
   for (int c = 0; c < kC; ++c) acc[c] = a.own_o[(long long)row * D + lane * kC + c];
   float M = a.own_ml[row * 2], L = a.own_ml[row * 2 + 1];
-  if (M == -INFINITY) {          // no key of it has a weight
-    L = 0.f;
+  if (M == -INFINITY) {          // no key of it has a weight (L is zero), or no score is a number (nor is L)
 #pragma unroll
     for (int c = 0; c < kC; ++c) acc[c] = 0.f;
   }
@@ -1077,7 +1084,11 @@ __global__ void __launch_bounds__(256) scored_merge_kernel(const MergeArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (i0 + i >= np || v[i].x == -INFINITY || v[i].y == 0.f) continue;   // a part of weight zero may hold anything
+        if (i0 + i >= np || v[i].y == 0.f) continue;   // a part of weight zero may hold anything
+        if (v[i].x == -INFINITY) {                     // no score is a number
+          L += v[i].y;
+          continue;
+        }
         const float top = fmaxf(M, v[i].x), f = M == -INFINITY ? 0.f : ex2(M - top), w = ex2(v[i].x - top);
         M = top;
         L = fmaf(w, v[i].y, L * f);

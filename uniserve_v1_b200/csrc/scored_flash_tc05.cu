@@ -824,7 +824,11 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const ScoredArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (p0 + k >= a.parts || ml[k].x == -INFINITY || ml[k].y == 0.f) continue;      // such a part may hold anything
+      if (p0 + k >= a.parts || ml[k].y == 0.f) continue;      // such a part may hold anything
+      if (ml[k].x == -INFINITY) {                             // no score is a number
+        L += ml[k].y;
+        continue;
+      }
       const float top = fmaxf(M, ml[k].x), f = M == -INFINITY ? 0.f : ex2f(M - top), w = ex2f(ml[k].x - top);
       M = top;
       L = fmaf(w, ml[k].y, L * f);
