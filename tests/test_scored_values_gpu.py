@@ -80,3 +80,24 @@ def test_shared_prefixes(bits, cap):
     got = S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(cap), k_scale=ks, v_scale=vs, shared=sh)
     N.raise_on_device_error()
     check_but(got, want, bound, lost)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,bias,cap", [(128, 4, 2, False, 0.0), (64, 4, 2, False, 0.0), (128, 2, 2, True, 0.0), (64, 2, 1, True, 0.0),
+                                               (128, 4, 2, False, 30.0), (64, 2, 1, True, 100.0)])
+def test_a_key_that_is_not_a_number_in_every_place_of_a_block(D, Hq, Hkv, bias, cap):
+    """256 sequences of 383 to 385 keys, each with one such key: in any place of a block that all rows of a tile see, and that
+    comes after the first one.  The rows that see it are NaN, and those before its block are what they were."""
+    n = 256
+    keys = [383 + i % 3 for i in range(n)]
+    q, k, v, cu_q, cu_k = packed(34, keys, keys, Hq, Hkv, D)
+    sl = slopes(Hq) if bias else None
+    want, bound = O.prompt(q, k, v, cu_q, cu_k, 0.1, cap, sl)
+    p = torch.cat([torch.arange(x, device=DEV) for x in keys])
+    seq = torch.repeat_interleave(torch.arange(n, device=DEV), torch.tensor(keys, device=DEV))
+    at = torch.arange(n, device=DEV)                     # the key of sequence s: key s, of its first or second block
+    k[cu_k[:-1].long() + at] = NAN
+    got = S.prompt_attention(q, k, v, cu_q, cu_k, 385, 385, 0.1, S.ScoreRules(cap, sl))
+    N.raise_on_device_error()
+    sees, before = p >= at[seq], p < at[seq] // 128 * 128
+    assert got[sees].isnan().all(), f"finite where it cannot be: {torch.nonzero(sees & ~got.isnan().flatten(1).all(1))[:4].tolist()}"
+    O.check(got[before], want[before], bound[before])

@@ -77,7 +77,18 @@ __device__ __forceinline__ unsigned long long add2_rm(unsigned long long a, unsi
   asm("add.rm.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 2^t for two arguments in [-126, 128) on the FMA pipe (flash_attn2_tc05.cu): relative error 8.6e-5.
+// The largest of two, three; NaN if one of them is.
+__device__ __forceinline__ float max2_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^t for two arguments in [-126, 128) on the FMA pipe (flash_attn2_tc05.cu): relative error 8.6e-5.  (It takes NaN for -126.)
 __device__ __forceinline__ void ex2_poly2(float t0, float t1, float& p0, float& p1) {
   const float kMagic = 12582912.f;
   const unsigned long long x = pack2(fmaxf(t0, -126.f), fmaxf(t1, -126.f));
@@ -645,12 +656,13 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                 if (!((see[c] >> i) & 1u)) t0 = -INFINITY;
                 if (!((see[c] >> (i + 1)) & 1u)) t1 = -INFINITY;
               }
-              if (!FIXED) mxs[c] = max3(mxs[c], t0, t1);
+              if (!FIXED) mxs[c] = max3_nan(mxs[c], t0, t1);
               pk[16 * c + (i >> 1)] = weigh(t0, t1, ls[c], !MASK && ((EMU >> (((i >> 1) & 1) * 4 + c)) & 1u));
             }
           }
           if (!FIXED) {
-            const float over = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));     // of the maximum so far
+            // of the maximum so far; a NaN fails the comparison, and the general form passes it on where the polynomial does not
+            const float over = max2_nan(max2_nan(mxs[0], mxs[1]), max2_nan(mxs[2], mxs[3]));
             through = __all_sync(0xffffffffu, over <= (MODE == 1 && half ? kRescaleThreshold : 64.f));    // FP16 ends at 2^16
             m_next = fmaxf(m_used, m_used + over);
           } else {
