@@ -101,3 +101,54 @@ def test_a_key_that_is_not_a_number_in_every_place_of_a_block(D, Hq, Hkv, bias, 
     sees, before = p >= at[seq], p < at[seq] // 128 * 128
     assert got[sees].isnan().all(), f"finite where it cannot be: {torch.nonzero(sees & ~got.isnan().flatten(1).all(1))[:4].tolist()}"
     O.check(got[before], want[before], bound[before])
+
+
+def lose(n, Hq, D, row, heads, group):
+    """Outputs that a value of `row`, key head and 64-channel group that is not a number reaches."""
+    lost = torch.zeros(n, Hq, D, dtype=torch.bool, device=DEV)
+    lost[row, heads, 64 * group:64 * group + 64] = True
+    return lost
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("group", [0, 1])
+@pytest.mark.parametrize("where", [0, 700, 2999])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (32, 2)])
+def test_a_value_that_is_not_a_number_loses_its_own_channels(bits, group, where, Hq, Hkv):
+    """The 64 channels that share its scale, and none of the other 64."""
+    q, kc, vc, ks, vs, table, n = make(35, [3000, 40], Hq, Hkv, 128, 16, bits)
+    want, bound = O.decode(q, kc, vc, table, n, 0.1, ks=ks, vs=vs)
+    vs[table[0, where // 16].long(), 1, where % 16, group] = NAN
+    got = S.decode_attention(q, kc, vc, table, n, 0.1, k_scale=ks, v_scale=vs)
+    N.raise_on_device_error()
+    lost = lose(2, Hq, 128, 0, slice(Hq // 2, Hq), group)
+    assert torch.equal(got.isnan(), lost)
+    O.check(got[~lost], want[~lost], bound[~lost])
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("group", [0, 1])
+def test_a_value_of_a_shared_prefix_that_is_not_a_number(bits, group):
+    case = ([5], [1500], 1, [40, 1, 0, 200, 17, 300], 8, 2, 128, 16, bits, 0.0, False)
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(case)
+    want, bound = O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[1500] * 5 + [0])
+    vs[table[0, 30].long(), 1, 3, group] = NAN
+    got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=sh)
+    N.raise_on_device_error()
+    lost = lose(6, 8, 128, slice(0, 5), slice(4, 8), group)
+    assert torch.equal(got.isnan(), lost)
+    O.check(got[~lost], want[~lost], bound[~lost])
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_a_key_of_a_shared_prefix_that_is_not_a_number(bits):
+    """Its key head's rows are lost, those of the other one are what they were."""
+    case = ([5], [1500], 1, [40, 1, 0, 200, 17, 300], 8, 2, 128, 16, bits, 0.0, False)
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(case)
+    want, bound = O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[1500] * 5 + [0])
+    ks[table[0, 30].long(), 1, 3, 0] = NAN
+    got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=sh)
+    N.raise_on_device_error()
+    lost = torch.zeros(6, 8, dtype=torch.bool, device=DEV)
+    lost[:5, 4:] = True
+    check_but(got, want, bound, lost)

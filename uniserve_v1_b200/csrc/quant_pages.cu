@@ -301,8 +301,9 @@ __global__ void __launch_bounds__(512) prefix_scales_kernel(const PrefixArgs a) 
       if (slot < 0) continue;
       const long long p = slot / a.page, at = ((p * a.heads + head) * a.page + (slot - p * a.page)) * groups;
       for (int i = 0; i < groups; ++i) {
-        k = max(k, (uint32_t)__bfloat16_as_ushort(a.ks[at + i]) & 0x7fffu);
-        v = max(v, (uint32_t)__bfloat16_as_ushort(a.vs[at + i]) & 0x7fffu);
+        const uint32_t x = (uint32_t)__bfloat16_as_ushort(a.ks[at + i]) & 0x7fffu, y = (uint32_t)__bfloat16_as_ushort(a.vs[at + i]) & 0x7fffu;
+        k = max(k, x < 0x7f80u ? x : 0u);      // (of those that are numbers: the others lose their own group, not the prefix)
+        v = max(v, y < 0x7f80u ? y : 0u);
       }
     }
     k = __reduce_max_sync(0xffffffffu, k);

@@ -616,13 +616,18 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
     float lift = 1.f;                        // 2^(14 - E)
     float shrink = 1.f;
     if constexpr (FMT != 16) {
-      uint32_t big = 0;                      // scales are not negative: as integers they are in order
+      // Scales are not negative: as integers they are in order.  One that is no number has no part in this: its group's outputs
+      // are lost, those of the other group are not.
+      uint32_t big = 0;
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
         float f[G];
         scales(sv, i * 32 + lane, j0, f);
 #pragma unroll
-        for (int g = 0; g < G; ++g) big = max(big, __float_as_uint(f[g]) & 0x7fffffffu);
+        for (int g = 0; g < G; ++g) {
+          const uint32_t x = __float_as_uint(f[g]) & 0x7fffffffu;
+          big = max(big, x < 0x7f800000u ? x : 0u);
+        }
       }
       const int e = max(top_scale, (int)(__reduce_max_sync(0xffffffffu, big) >> 23));
       shrink = power_of_two(127 - (e - top_scale));
