@@ -1,0 +1,68 @@
+"""Decode batches with shared prefixes whose plans say more or less than the pages hold."""
+import pytest
+import torch
+
+import scored_oracle as O
+from test_scored_decode_gpu import make, slopes
+from test_scored_flash_gpu import shared_batch
+from uniserve_v1_b200.ops import native as N
+from uniserve_v1_b200.ops import scored as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, I32 = torch.bfloat16, torch.int32
+
+
+def soiled(work):
+    """A workspace as an earlier call may have left it."""
+    for t in (work.prefix_o, work.prefix_ml, work.own_o, work.own_ml, work.scratch):
+        t.fill_(float("nan"))
+    work.prefix_ml[::2] = 3.0          # maxima that look like some
+    work.prefix_ml[1::2] = 1.0
+    return work
+
+
+def test_a_prefix_of_more_than_a_million_keys():
+    """Its last part counts like its first: values behind key 2^20 stand out."""
+    long, rows = 1_500_000, 8
+    q, kc, vc, _, _, table, n = make(41, [long] + [1] * (rows - 1), 2, 1, 64, 64, 16)
+    vc.view(-1, 1, 64)[(table[0, (1 << 20) // 64:].long()[:, None] * 64 + torch.arange(64, device=DEV)).flatten()] += 4.0
+    table = table[:1].expand(rows, -1).contiguous()
+    n = torch.tensor([long - i * 7 for i in range(rows)], dtype=I32, device=DEV)
+    plan = S.SharedPrefix(torch.tensor([0, rows], dtype=I32, device=DEV), torch.tensor([long - 100], dtype=I32, device=DEV), rows, long - 100)
+    work = soiled(S.decode_work(rows, 2, 1, 64, DEV, plan))
+    got = S.decode_attention(q, kc, vc, table, n, 0.125, shared=plan, work=work)
+    N.raise_on_device_error()
+    want, bound = O.decode(q, kc, vc, table, n, 0.125)
+    assert float(want.mean()) > 1.0
+    O.check(got, want, bound)
+
+
+@pytest.mark.parametrize("bits,page,told", [(16, 16, 1000), (16, 16, 520), (16, 24, 1000), (8, 16, 1000), (4, 16, 1000)])
+def test_a_prefix_past_the_page_lists(bits, page, told):
+    """Lists of 480 keys, a prefix of `told`: rows of up to 480 keys are whole, and the status says so."""
+    lens = [480, 300, 1, 0, 479, 128, 33]
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([7], [480], 0, [0] * 7, 8, 2, 64, page, bits, 0.0, True))
+    table = table[:, :480 // page].contiguous() if 480 % page == 0 else table[:, :-(-480 // page)].contiguous()
+    n.copy_(torch.tensor(lens, dtype=I32, device=DEV))
+    plan = S.SharedPrefix(sh.cu_rows, torch.full_like(sh.lens, told), 7, told)
+    work = soiled(S.decode_work(7, 8, 2, 64, DEV, plan))
+    N.raise_on_device_error()
+    got = S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(slopes=sl), k_scale=ks, v_scale=vs, shared=plan, work=work)
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+    O.check(got, *O.decode(q, kc, vc, table, n, scale, slopes=sl, ks=ks, vs=vs, expanded=[480] * 7 if ks is not None else None))
+
+
+@pytest.mark.parametrize("bits,page", [(16, 16), (16, 24), (8, 16)])
+def test_the_rest_of_a_prefix_longer_than_told_is_read_row_by_row(bits, page):
+    """2000 keys where 600 were told: no key is lost, and the status says so."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([4], [2000], 1, [9, 1, 0, 70, 40], 8, 2, 64, page, bits, 30.0, False))
+    plan = S.SharedPrefix(sh.cu_rows, sh.lens, 4, 600)
+    work = soiled(S.decode_work(5, 8, 2, 64, DEV, plan))
+    N.raise_on_device_error()
+    got = S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(cap), k_scale=ks, v_scale=vs, shared=plan, work=work)
+    if bits != 16 or page != 16 or S._prefix_plan(plan, 8, 2, S._sm_count(0))[1] * S._prefix_plan(plan, 8, 2, S._sm_count(0))[2] * 128 < 2000:
+        with pytest.raises(RuntimeError):
+            N.raise_on_device_error()
+    O.check(got, *O.decode(q, kc, vc, table, n, scale, cap, ks=ks, vs=vs, expanded=[600] * 4 + [0] if ks is not None else None))

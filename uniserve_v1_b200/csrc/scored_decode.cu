@@ -59,11 +59,11 @@ struct DecodeArgs {
   long long ldq, ldo;
   int B, Hq, Hkv, chunks, max_pages, pages, page, shift, window;
   float scale_log2, scale_cap, cap_log2;    // cap_log2 == 0: no cap; scale_cap = 2 scale log2(e) / cap
-  // shared prefixes: rows [cu_rows[g], cu_rows[g + 1]) share their first shared[g] keys, which are not this launch's; its
-  // results then go unnormalised to own_o [B][Hq][D], own_ml [B][Hq][2] for scored_merge_kernel
+  // shared prefixes: rows [cu_rows[g], cu_rows[g + 1]) share their first min(shared[g], most_shared) keys, which are not this
+  // launch's; its results then go unnormalised to own_o [B][Hq][D], own_ml [B][Hq][2] for scored_merge_kernel
   const int *cu_rows, *shared;
   float *own_o, *own_ml;
-  int groups;
+  int groups, most_shared;
   unsigned int* status;
   uint32_t magic;                           // see bytes_even, nibbles
 };
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
         const int mid = (g + h + 1) >> 1;
         if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
       }
-      if (b < a.cu_rows[a.groups]) lo = max(lo, a.shared[g]);
+      if (b < a.cu_rows[a.groups]) lo = max(lo, min(a.shared[g], a.most_shared));
     }
     const long long room = (long long)a.max_pages * a.page;
     int hi = len;
@@ -1042,7 +1042,7 @@ struct MergeArgs {
   const int *cu_rows, *shared;
   __nv_bfloat16* out;
   long long ldo;
-  int B, Hq, Hkv, groups, pairs, parts, blocks_per_part;
+  int B, Hq, Hkv, groups, most_shared, pairs, parts, blocks_per_part;
   unsigned int* status;
 };
 
@@ -1068,12 +1068,13 @@ __global__ void __launch_bounds__(256) scored_merge_kernel(const MergeArgs a) {
       const int mid = (g + h + 1) >> 1;
       if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
     }
-    const int blocks = (a.shared[g] + 127) >> 7;
-    int np = min((blocks + a.blocks_per_part - 1) / a.blocks_per_part, a.parts);
+    // the parts that the prefix launch wrote: as many as its keys fill
+    const int blocks = (min(a.shared[g], a.most_shared) + 127) >> 7;
+    int np = (blocks + a.blocks_per_part - 1) / a.blocks_per_part;
     const int per = 128 / share, r = b - a.cu_rows[g];       // sequences of a 128-row tile of the prefix kernel
-    if (blocks > a.parts * a.blocks_per_part || r >= a.pairs * 2 * per) {   // a group larger than the host was told
+    if (r >= a.pairs * 2 * per) {                            // a group of more rows than the host was told
       us_dev_fail(a.status, US_DEV_BOUNDS);
-      if (r >= a.pairs * 2 * per) np = 0;
+      np = 0;
     }
     const int tile = r / per, in_tile = (r - tile * per) * share + head - hk * share;
     const long long at = ((((long long)g * a.pairs + (tile >> 1)) * a.Hkv + hk) * a.parts) * 256 + (tile & 1) * 128 + in_tile;
@@ -1130,15 +1131,15 @@ US_API long long us_scored_decode_scratch(int D) {
 
 // q [B, Hq, D] bf16 (row pitch ldq); pages [pages, page, Hkv, D] bf16 or integer codes with scales (bits 8, 4; 16: bf16);
 // table [B, max_pages], lens [B], starts [B] or null.  scratch, counters: see above; counters are zero before the first
-// call and left zero; calls that share them are ordered on the device.  groups > 0: the keys below shared[g] of rows
-// [cu_rows[g], cu_rows[g + 1]) are in pre_o / pre_ml by us_scored_prefix, the launch before this one on the stream, and
-// own_o, own_ml ([B][Hq][D and 2] floats) take the rest until both are joined.
+// call and left zero; calls that share them are ordered on the device.  groups > 0: the keys below min(shared[g],
+// most_shared) of rows [cu_rows[g], cu_rows[g + 1]) are in pre_o / pre_ml by us_scored_prefix (with the same numbers), the
+// launch before this one on the stream, and own_o, own_ml ([B][Hq][D and 2] floats) take the rest until both are joined.
 US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const void* vc, const void* ks, const void* vs,
                             const int* table, int max_pages, const int* lens, const int* starts, void* out, long long ldo,
                             void* scratch, int* counters, int B, int Hq, int Hkv, int D, int bits, int pages, int page,
                             int window, float scale, float cap, const float* slopes, int groups, const int* cu_rows,
-                            const int* shared, const float* pre_o, const float* pre_ml, float* own_o, float* own_ml, int pairs,
-                            int parts, int blocks_per_part, void* stream_) {
+                            const int* shared, int most_shared, const float* pre_o, const float* pre_ml, float* own_o,
+                            float* own_ml, int pairs, int parts, int blocks_per_part, void* stream_) {
   US_REQUIRE(B >= 0 && B <= kMaxSeqs && (D == 64 || D == 128) && Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0);
   if (B == 0) return US_OK;
   US_REQUIRE(q && kc && vc && table && lens && out && scratch && counters && max_pages >= 1 && pages >= 1 && page >= 1);
@@ -1149,7 +1150,7 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
              ((uintptr_t)out % 4) == 0);
   const int share = Hq / Hkv;
   if (groups > 0) US_REQUIRE(cu_rows && shared && pre_o && pre_ml && own_o && own_ml && pairs >= 1 && parts >= 1 && blocks_per_part >= 1 && share <= 128 &&
-                             window == 0 && !starts);
+                             window == 0 && !starts && most_shared >= 0 && (long long)most_shared <= (long long)parts * blocks_per_part * 128);
   DecodeArgs a = {};
   a.q = (const __nv_bfloat16*)q;
   a.kc = (const uint8_t*)kc;
@@ -1181,6 +1182,7 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   a.cap_log2 = cap * kLog2e;
   a.scale_cap = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
   a.groups = groups;
+  a.most_shared = most_shared;
   a.cu_rows = cu_rows;
   a.shared = shared;
   a.own_o = own_o;
@@ -1212,6 +1214,7 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   m.Hq = Hq;
   m.Hkv = Hkv;
   m.groups = groups;
+  m.most_shared = most_shared;
   m.pairs = pairs;
   m.parts = parts;
   m.blocks_per_part = blocks_per_part;

@@ -66,6 +66,7 @@ struct ScoredArgs {
   const float* q_back;                        // FP16 operands (quant_pages.cu): factors of the rows of Q,
   const int2* exps;                           // and exponent fields of K and V [groups * Hkv]
   int key_stride;                             // > 0: packed keys, those of group g from row g * key_stride on
+  int most_shared;                            // keys of a prefix at most
   int max_pages, pages, page, batch, pairs, parts, blocks_per_part;
   int n, max_q, max_k;                        // sequences, the longest one's rows and keys
   float *part_o, *part_ml;
@@ -183,12 +184,14 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     q_len = min(a.cu_rows[seq + 1], a.batch) - q_start;
     q0 = pair * 2 * per;
     k_start = seq * a.key_stride;
-    kv_len = (int)min((long long)a.shared[seq], a.key_stride > 0 ? (long long)a.key_stride : (long long)a.max_pages * a.page);
-    // packed keys: pages outside the cache and prefixes longer than told were left out of them
-    if (a.key_stride > 0 && part == 0 && blockIdx.y == 0 && q_len > 0) {
-      bool bad = a.shared[seq] > a.key_stride;
-      for (int pi = threadIdx.x; pi * a.page < kv_len; pi += kThreads)
-        bad |= pi >= a.max_pages || (unsigned)a.table[(long long)q_start * a.max_pages + pi] >= (unsigned)a.pages;
+    kv_len = min(a.shared[seq], a.most_shared);
+    if (part == 0 && blockIdx.y == 0 && q_len > 0) {
+      // a prefix past the page lists or longer than told: what is left of it is the rows' own
+      bool bad = a.shared[seq] > a.most_shared;
+      if (a.key_stride > 0) {                  // packed keys: pages outside the cache were left out of them
+        for (int pi = threadIdx.x; pi * a.page < kv_len; pi += kThreads)
+          bad |= (unsigned)a.table[(long long)q_start * a.max_pages + pi] >= (unsigned)a.pages;
+      }
       if (bad) us_dev_fail(a.status, US_DEV_BOUNDS);
     }
     prow0 = ((((long long)seq * a.pairs + pair) * a.Hkv + hk) * a.parts + part) * (2 * kBM);
@@ -199,11 +202,13 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     return ((((long long)part * a.n + seq) * a.max_q + row) * a.Hq) + head;
   };
   kv_len = max(kv_len, 0);
-  int nb = min((kv_len + kBN - 1) / kBN, kMaxBlocks), jb = 0;
+  int nb = kv_len / kBN + (kv_len % kBN != 0), jb = 0;
   if constexpr (MODE == 1) {
     jb = part * a.blocks_per_part;
-    nb = min(nb - jb, a.blocks_per_part);
+    nb = min(nb - jb, a.blocks_per_part);                       // kMaxBlocks at most
     if (nb <= 0) return;                                        // such a part is not read
+  } else {
+    nb = min(nb, kMaxBlocks);
   }
 
   int first_known = -1;
@@ -993,10 +998,11 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
 // The part that the shared prefixes of a decode batch have in its attention (scored_decode.cu): rows
 // [cu_rows[g], cu_rows[g + 1]) of q [B, Hq, D] against the first shared[g] keys behind row cu_rows[g]'s page list in
 // k / v [pages, page, Hkv, D], or, with key_stride > 0, in rows g * key_stride .. of packed k / v [key_rows, Hkv, D]; with q_back and
-// exps q, k and v are FP16 (us_quant_prefix).
+// exps q, k and v are FP16 (us_quant_prefix).  Of a prefix the first most_shared keys are taken at most: those that the page
+// lists, the packed rows and the parts have room for.
 // part_o, part_ml: [groups][pairs][Hkv][parts][256][D and 2].
 US_API int us_scored_prefix(const void* q, long long ldq, const void* k, long long pages, const void* v, long long page,
-                            const float* q_back, const void* exps, int key_stride, const int* table, int max_pages, int key_rows, int B, const int* lens,
+                            const float* q_back, const void* exps, int key_stride, int most_shared, const int* table, int max_pages, int key_rows, int B, const int* lens,
                             const int* cu_rows, const int* shared, int groups, int Hq, int Hkv, int D, int max_rows, float scale,
                             float cap, const float* slopes, float* part_o, float* part_ml, int pairs, int parts,
                             int blocks_per_part, void* stream_) {
@@ -1006,6 +1012,8 @@ US_API int us_scored_prefix(const void* q, long long ldq, const void* k, long lo
              blocks_per_part >= 1 && blocks_per_part <= kMaxBlocks && (long long)pairs * Hkv <= 65535);
   const int share = Hq / Hkv, per = kBM / share;
   US_REQUIRE((long long)pairs * 2 * per >= max_rows);
+  US_REQUIRE(most_shared >= 0 && (long long)most_shared <= (long long)parts * blocks_per_part * kBN && (key_stride == 0 || most_shared <= key_stride) &&
+             page >= 1 && (long long)most_shared <= (long long)max_pages * page);
   uint64_t rows = (uint64_t)key_rows;
   uint32_t box = kBN;
   if (key_stride == 0) {
@@ -1033,6 +1041,7 @@ US_API int us_scored_prefix(const void* q, long long ldq, const void* k, long lo
   a.q_back = q_back;
   a.exps = (const int2*)exps;
   a.key_stride = key_stride;
+  a.most_shared = most_shared;
   a.lens = lens;
   a.cu_rows = cu_rows;
   a.shared = shared;

@@ -26,11 +26,11 @@ P, I, L = N.P, N.I, N.L
 BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
 N.register_signatures({
     "us_scored_decode_scratch": (L, [I]),
-    "us_scored_decode": (I, [P, L, P, P, P, P, P, I, P, P, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, P, P, P, P,
-                             P, P, I, I, I, P]),
+    "us_scored_decode": (I, [P, L, P, P, P, P, P, I, P, P, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, P, P, I,
+                             P, P, P, P, I, I, I, P]),
     "us_scored_flash": (I, [P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, I, P, P, P, I, P, P, P]),
     "us_scored_flash_parts": (I, [I, I, I, I, I]),
-    "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
+    "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, I, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
 })
 
 MAX_SEQS = 704             # sequences of one decode launch; larger batches go in slices
@@ -396,11 +396,12 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
             bad = bad.repeat_interleave(page, 1)[:, :stride, None, None]
             for t in (k, v):
                 t.view(groups, stride, Hkv, D)[:, :bad.shape[1]].masked_fill_(bad, 0)
+        most = min(page_table.shape[1] * page, stride or parts * each * _TILE, 1 << 30)      # keys of a prefix that are read so
         cu_rows, lens, po, pm = shared.cu_rows.data_ptr(), shared.lens.data_ptr(), work.prefix_o.data_ptr(), work.prefix_ml.data_ptr()
         launch("us_scored_prefix", 1, qp.data_ptr(), qp.stride(0), k.data_ptr(), pages, v.data_ptr(), page, _at(back), _at(exps),
-               stride, page_table.data_ptr(), page_table.shape[1], k.shape[0], B, seq_lens.data_ptr(), cu_rows, lens, groups, Hq,
+               stride, most, page_table.data_ptr(), page_table.shape[1], k.shape[0], B, seq_lens.data_ptr(), cu_rows, lens, groups, Hq,
                Hkv, D, shared.max_rows, scale, rules.cap, _at(rules.slopes), po, pm, pairs, parts, each)
-        pre = (cu_rows, lens, po, pm, work.own_o.data_ptr(), work.own_ml.data_ptr(), pairs, parts, each)
+        pre = (cu_rows, lens, most, po, pm, work.own_o.data_ptr(), work.own_ml.data_ptr(), pairs, parts, each)
     launch("us_scored_decode", 2 if groups else 1, q.data_ptr(), q.stride(0), kcache.data_ptr(), vcache.data_ptr(), _at(k_scale),
            _at(v_scale), page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), _at(starts), to.data_ptr(), to.stride(0),
            work.scratch.data_ptr(), work.counters.data_ptr(), B, Hq, Hkv, D, bits, pages, page, rules.window, scale, rules.cap,
@@ -410,7 +411,7 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
     return to
 
 
-_NO_PREFIX = (None, None, None, None, None, None, 1, 1, 1)
+_NO_PREFIX = (None, None, 0, None, None, None, None, 1, 1, 1)
 
 
 def _decode_cpu(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k_scale, v_scale, shared):
