@@ -38,7 +38,7 @@ def test_a_prefix_of_more_than_a_million_keys():
     O.check(got, want, bound)
 
 
-@pytest.mark.parametrize("bits,page,told", [(16, 16, 1000), (16, 16, 520), (16, 24, 1000), (8, 16, 1000), (4, 16, 1000)])
+@pytest.mark.parametrize("bits,page,told", [(16, 16, 1000), (16, 16, 520), (16, 24, 1000), (8, 16, 1000), (4, 16, 1000), (16, 128, 100_000)])
 def test_a_prefix_past_the_page_lists(bits, page, told):
     """Lists of 480 keys, a prefix of `told`: rows of up to 480 keys are whole, and the status says so."""
     lens = [480, 300, 1, 0, 479, 128, 33]
@@ -66,3 +66,26 @@ def test_the_rest_of_a_prefix_longer_than_told_is_read_row_by_row(bits, page):
         with pytest.raises(RuntimeError):
             N.raise_on_device_error()
     O.check(got, *O.decode(q, kc, vc, table, n, scale, cap, ks=ks, vs=vs, expanded=[600] * 4 + [0] if ks is not None else None))
+
+
+@pytest.mark.parametrize("bits,page,cap", [(16, 16, 0.0), (16, 128, 30.0), (16, 24, 0.0), (8, 16, 0.0), (4, 16, 30.0)])
+def test_what_a_prefix_holds_behind_its_rows_reaches_none(bits, page, cap):
+    """A prefix of 900 keys over rows of up to 300: behind them the pages hold NaN and infinities."""
+    lens = [300, 300, 129, 1, 0, 257]
+    q, kc, vc, ks, vs, table, n, sh, _, sl, scale = shared_batch(([6], [900], 0, [0] * 6, 8, 2, 64, page, bits, cap, False))
+    n.copy_(torch.tensor(lens, dtype=I32, device=DEV))
+    want, bound = O.decode(q, kc, vc, table, n, scale, cap, ks=ks, vs=vs, expanded=[900] * 6 if ks is not None else None)
+    pos = torch.arange(300, 900, device=DEV)
+    at, off = table[0, pos // page].long(), pos % page
+    if bits == 16:
+        kc[at, off] = float("nan")
+        vc[at, off] = float("inf")
+        vc[at[::3], off[::3]] = float("nan")
+    else:
+        ks[at, :, off] = float("nan")
+        vs[at, :, off] = float("nan")
+    got = S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(cap), k_scale=ks, v_scale=vs, shared=sh)
+    N.raise_on_device_error()
+    if ks is not None:          # the largest scale of the prefix may have been behind its rows: another power of two
+        want, bound = O.decode(q, kc, vc, table, n, scale, cap, ks=ks.nan_to_num(), vs=vs.nan_to_num(), expanded=[900] * 6)
+    O.check(got, want, bound)

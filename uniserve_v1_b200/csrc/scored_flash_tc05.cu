@@ -20,8 +20,8 @@
 //   tanh's values); a warp that meets a larger score in a block takes the exponential form there.
 // * Bias.  Keys on one side of a row are a line in j, added within the polynomial's last multiply-add; a block
 //   with keys on both sides takes magnitudes.
-// * Values behind the last key of a sequence are put to zero in shared memory before their product: they belong to
-//   another sequence, or to nobody, and 0 x NaN is NaN.
+// * Values behind the last key of a sequence (of a shared prefix: of the longest row) are put to zero in shared memory before
+//   their product: they belong to another sequence, or to nobody, and 0 x NaN is NaN.
 //
 // A shared prefix: rows of a tile are (sequence, query head of the key head) pairs of one group, the keys come through
 // the page list of the group's first row (or packed), split into `parts` of the blocks; unnormalised outputs, maxima and
@@ -419,6 +419,12 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       Blocks walk(bits, words);
       bool a0 = false, b0 = false, a1 = false, b1 = false;
       int j = walk.next(a0, b0), na = 0, nbb = 0;
+      int v_end = kv_len;                // values from here on nobody sees
+      if constexpr (MODE == 1) {         // a prefix may be longer than the rows that share it
+        int most = 0;
+        for (int r = q0 + lane; r < min(q0 + 2 * per, q_len); r += 32) most = max(most, a.lens[q_start + r]);
+        v_end = min(kv_len, __reduce_max_sync(0xffffffffu, most));
+      }
       bool ok = warp_wait(q_full, 0);
       if (ok) {
         tc::tc_fence_after_sync();
@@ -430,9 +436,9 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         a1 = b1 = false;
         const int jn = walk.next(a1, b1);
         if (!warp_wait(&kv_full[e & 1], (uint32_t)(e >> 1) & 1u)) { ok = false; break; }
-        const int there = kv_len - (jb + j) * kBN;
-        if (there < kBN) {               // the sequence ends in this block
-          for (int r = there + (lane >> 3); r < kBN; r += 4)
+        const int there = v_end - (jb + j) * kBN;
+        if (there < kBN) {               // the sequence ends in this block, or before it
+          for (int r = max(there, 0) + (lane >> 3); r < kBN; r += 4)
 #pragma unroll
             for (int hf = 0; hf < kHalves; ++hf)
               *reinterpret_cast<uint4*>(sV + (e & 1) * kTile + hf * kHalf + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);

@@ -51,7 +51,8 @@ class ScoreRules(NamedTuple):
 class SharedPrefix:
     """Rows [cu_rows[g], cu_rows[g + 1]) of a decode batch share their first lens[g] keys: those are read through the
     page list of the group's first row, once for all its rows.  ``max_rows`` and ``max_len`` bound the groups' sizes
-    for the host.  Rows past the last group share nothing."""
+    for the host.  Rows past the last group share nothing.  A prefix may be longer than some of its rows, which end in it;
+    a value in it that is not finite may then reach a shorter row, as one of the row's own group sees it."""
     cu_rows: torch.Tensor      # int32 [groups + 1]
     lens: torch.Tensor         # int32 [groups]
     max_rows: int
