@@ -1,0 +1,23 @@
+"""Plans of shared prefixes on the CPU: what is refused, and rows that share nothing."""
+import pytest
+import torch
+
+from test_scored_cpu import decode_args
+from uniserve_v1_b200.ops import scored as S
+
+I32 = torch.int32
+
+
+@pytest.mark.parametrize("cu_rows,lens", [(torch.tensor([[0], [2]], dtype=I32), torch.tensor([2], dtype=I32)),
+                                          (torch.tensor([0, 2], dtype=I32), torch.tensor([[2]], dtype=I32)),
+                                          (torch.tensor([0, 1, 2], dtype=I32), torch.tensor([2], dtype=I32))])
+def test_plans_of_other_shapes_are_refused(cu_rows, lens):
+    with pytest.raises(ValueError, match="cu_rows"):
+        S.decode_attention(**decode_args(shared=S.SharedPrefix(cu_rows, lens, 2, 2)))
+
+
+def test_a_plan_may_be_columns_of_a_table():
+    plan = torch.tensor([[0, 3], [1, 2], [2, 9]], dtype=I32)
+    args = decode_args(seq_lens=torch.tensor([5, 6], dtype=I32), page_table=torch.tensor([[1, 2], [0, 2]], dtype=I32))
+    dense = S.decode_attention(**args, shared=S.SharedPrefix(plan[:, 0].contiguous(), plan[:2, 1].contiguous(), 1, 3))
+    assert torch.equal(S.decode_attention(**args, shared=S.SharedPrefix(plan[:, 0], plan[:2, 1], 1, 3)), dense)

@@ -89,3 +89,13 @@ def test_what_a_prefix_holds_behind_its_rows_reaches_none(bits, page, cap):
     if ks is not None:          # the largest scale of the prefix may have been behind its rows: another power of two
         want, bound = O.decode(q, kc, vc, table, n, scale, cap, ks=ks.nan_to_num(), vs=vs.nan_to_num(), expanded=[900] * 6)
     O.check(got, want, bound)
+
+
+@pytest.mark.parametrize("bits,page", [(16, 16), (16, 24), (8, 16)])
+def test_a_plan_may_be_columns_of_a_table(bits, page):
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([3, 4], [600, 250], 1, [9, 1, 0, 70, 40, 5, 6, 8], 8, 2, 64, page, bits, 0.0, False))
+    plan = torch.stack([sh.cu_rows, torch.cat([sh.lens, sh.lens[:1]])], 1)
+    got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=S.SharedPrefix(plan[:, 0], plan[:2, 1], 4, 600))
+    N.raise_on_device_error()
+    assert torch.equal(got, S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=sh))
+    O.check(got, *O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[600] * 3 + [250] * 4 + [0] if ks is not None else None))

@@ -337,10 +337,12 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
             shared = None
         elif starts is not None or rules.window:
             raise ValueError("a shared prefix goes with neither starts nor a window")
-        elif shared.cu_rows.dtype != I32 or shared.lens.dtype != I32 or shared.cu_rows.numel() != shared.groups + 1:
+        elif shared.cu_rows.dtype != I32 or shared.lens.dtype != I32 or shared.cu_rows.shape != (shared.groups + 1,) or shared.lens.dim() != 1:
             raise ValueError("a shared prefix has int32 cu_rows [groups + 1] and lens [groups]")
         elif Hq // Hkv > _TILE or B > MAX_SEQS:
             raise ValueError(f"a shared prefix is served for up to {_TILE} query heads a key head and {MAX_SEQS} sequences")
+        elif not (shared.cu_rows.is_contiguous() and shared.lens.is_contiguous()):     # columns of a plan
+            shared = SharedPrefix(shared.cu_rows.contiguous(), shared.lens.contiguous(), shared.max_rows, shared.max_len)
     if at < 0:
         res = _decode_cpu(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k_scale, v_scale, shared)
         return res if out is None else out.copy_(res)
