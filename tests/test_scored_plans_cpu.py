@@ -21,3 +21,16 @@ def test_a_plan_may_be_columns_of_a_table():
     args = decode_args(seq_lens=torch.tensor([5, 6], dtype=I32), page_table=torch.tensor([[1, 2], [0, 2]], dtype=I32))
     dense = S.decode_attention(**args, shared=S.SharedPrefix(plan[:, 0].contiguous(), plan[:2, 1].contiguous(), 1, 3))
     assert torch.equal(S.decode_attention(**args, shared=S.SharedPrefix(plan[:, 0], plan[:2, 1], 1, 3)), dense)
+
+
+def test_rows_before_the_first_group_share_nothing():
+    args = decode_args(seq_lens=torch.tensor([5, 6], dtype=I32), page_table=torch.tensor([[1, 2], [0, 2]], dtype=I32))
+    alone = S.decode_attention(**args)
+    plan = S.SharedPrefix(torch.tensor([1, 2], dtype=I32), torch.tensor([4], dtype=I32), 1, 4)
+    assert torch.equal(S.decode_attention(**args, shared=plan), alone)
+
+
+def test_a_group_that_begins_before_the_batch_raises():
+    plan = S.SharedPrefix(torch.tensor([-1, 2], dtype=I32), torch.tensor([2], dtype=I32), 3, 2)
+    with pytest.raises(IndexError, match="begins"):
+        S.decode_attention(**decode_args(shared=plan))

@@ -99,3 +99,43 @@ def test_a_plan_may_be_columns_of_a_table(bits, page):
     N.raise_on_device_error()
     assert torch.equal(got, S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=sh))
     O.check(got, *O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[600] * 3 + [250] * 4 + [0] if ks is not None else None))
+
+
+@pytest.mark.parametrize("bits,page,cap", [(16, 16, 0.0), (16, 24, 30.0), (8, 16, 0.0), (4, 16, 30.0)])
+def test_rows_before_the_first_group_and_past_the_last_share_nothing(bits, page, cap):
+    """The lists of rows that do share hold no pages below the prefix, but for the first one's."""
+    case = ([1, 1, 3, 4], [0, 0, 600, 250], 2, [700, 33, 1, 0, 70, 40, 5, 6, 300, 90, 513], 8, 2, 64, page, bits, cap, False)
+    q, kc, vc, ks, vs, table, n, _, cap, sl, scale = shared_batch(case)
+    want, bound = O.decode(q, kc, vc, table, n, scale, cap, ks=ks, vs=vs, expanded=[0] * 2 + [600] * 3 + [250] * 4 + [0] * 2 if ks is not None else None)
+    table[3:5, :600 // page] = -1
+    table[6:9, :250 // page] = kc.shape[0]
+    plan = S.SharedPrefix(torch.tensor([2, 5, 5, 9], dtype=I32, device=DEV), torch.tensor([600, 77, 250], dtype=I32, device=DEV), 4, 600)
+    work = soiled(S.decode_work(11, 8, 2, 64, DEV, plan))
+    got = S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(cap), k_scale=ks, v_scale=vs, shared=plan, work=work)
+    N.raise_on_device_error()
+    O.check(got, want, bound)
+
+
+@pytest.mark.parametrize("bits,page", [(16, 16), (16, 24), (8, 16)])
+def test_a_group_that_begins_before_the_batch_shares_nothing(bits, page):
+    """Rows 0 and 1 of the first group; the second one is served.  The status says so."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([2, 3], [300, 450], 0, [9, 1, 0, 70, 40], 8, 2, 64, page, bits, 0.0, False))
+    plan = S.SharedPrefix(torch.tensor([-3, 2, 5], dtype=I32, device=DEV), sh.lens, 5, 450)
+    work = soiled(S.decode_work(5, 8, 2, 64, DEV, plan))
+    N.raise_on_device_error()
+    got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=plan, work=work)
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+    O.check(got, *O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[0] * 2 + [450] * 3 if ks is not None else None))
+
+
+def test_rows_of_a_group_past_those_told_read_their_own_lists():
+    """Six rows of 64 query heads a key head, of which two were told and four have room.  The status says so."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([6], [300], 0, [9, 1, 0, 70, 40, 5], 64, 1, 64, 16, 16, 0.0, False))
+    plan = S.SharedPrefix(sh.cu_rows, sh.lens, 2, 300)
+    work = soiled(S.decode_work(6, 64, 1, 64, DEV, plan))
+    N.raise_on_device_error()
+    got = S.decode_attention(q, kc, vc, table, n, scale, shared=plan, work=work)
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+    O.check(got, *O.decode(q, kc, vc, table, n, scale))

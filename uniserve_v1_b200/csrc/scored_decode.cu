@@ -63,7 +63,7 @@ struct DecodeArgs {
   // launch's; its results then go unnormalised to own_o [B][Hq][D], own_ml [B][Hq][2] for scored_merge_kernel
   const int *cu_rows, *shared;
   float *own_o, *own_ml;
-  int groups, most_shared;
+  int groups, most_shared, most_rows;       // most_rows: of a group
   unsigned int* status;
   uint32_t magic;                           // see bytes_even, nibbles
 };
@@ -119,6 +119,22 @@ constexpr uint32_t kOne = 0x3C003C00u;          // FP16 pairs: 1, -1152 = -(1024
 constexpr uint32_t kMinus1152 = 0xE480E480u, kMinus72 = 0xD480D480u;
 __device__ __forceinline__ float power_of_two(int field) {     // 2^(field - 127), field clamped to what a float has
   return __uint_as_float((uint32_t)min(max(field, 0), 254) << 23);
+}
+
+// The group with whose rows row b shares keys, or -1.  A group that begins before the batch has no page list to read, and rows
+// past those that the prefix launch was planned for are not in its results: such rows have all their keys to themselves, and the
+// status says so.
+__device__ __forceinline__ int group_of(const int* cu_rows, int groups, int b, int most_rows, unsigned int* status) {
+  int g = 0, h = groups - 1;
+  while (g < h) {
+    const int mid = (g + h + 1) >> 1;
+    if (cu_rows[mid] <= b) g = mid; else h = mid - 1;
+  }
+  const int first = cu_rows[g];
+  if (b < first || b >= cu_rows[g + 1]) return -1;
+  if (first >= 0 && b - first < most_rows) return g;
+  us_dev_fail(status, US_DEV_BOUNDS);
+  return -1;
 }
 
 // A position in the tile list.
@@ -185,12 +201,8 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
     int len = max(a.lens[b], 0), lo = a.starts ? max(a.starts[b], 0) : 0;
     if (a.window > 0) lo = max(lo, len - a.window);
     if (a.groups > 0) {
-      int g = 0, h = a.groups - 1;
-      while (g < h) {
-        const int mid = (g + h + 1) >> 1;
-        if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
-      }
-      if (b < a.cu_rows[a.groups]) lo = max(lo, min(a.shared[g], a.most_shared));
+      const int g = group_of(a.cu_rows, a.groups, b, a.most_rows, a.status);
+      if (g >= 0) lo = max(lo, min(a.shared[g], a.most_shared));
     }
     const long long room = (long long)a.max_pages * a.page;
     int hi = len;
@@ -1062,21 +1074,13 @@ __global__ void __launch_bounds__(256) scored_merge_kernel(const MergeArgs a) {
 #pragma unroll
     for (int c = 0; c < kC; ++c) acc[c] = 0.f;
   }
-  if (b < a.cu_rows[a.groups]) {
-    int g = 0, h = a.groups - 1;
-    while (g < h) {
-      const int mid = (g + h + 1) >> 1;
-      if (a.cu_rows[mid] <= b) g = mid; else h = mid - 1;
-    }
+  const int per = 128 / share;                               // sequences of a 128-row tile of the prefix kernel
+  const int g = group_of(a.cu_rows, a.groups, b, a.pairs * 2 * per, a.status);
+  if (g >= 0) {
     // the parts that the prefix launch wrote: as many as its keys fill
     const int blocks = (min(a.shared[g], a.most_shared) + 127) >> 7;
-    int np = (blocks + a.blocks_per_part - 1) / a.blocks_per_part;
-    const int per = 128 / share, r = b - a.cu_rows[g];       // sequences of a 128-row tile of the prefix kernel
-    if (r >= a.pairs * 2 * per) {                            // a group of more rows than the host was told
-      us_dev_fail(a.status, US_DEV_BOUNDS);
-      np = 0;
-    }
-    const int tile = r / per, in_tile = (r - tile * per) * share + head - hk * share;
+    const int np = (blocks + a.blocks_per_part - 1) / a.blocks_per_part;
+    const int r = b - a.cu_rows[g], tile = r / per, in_tile = (r - tile * per) * share + head - hk * share;
     const long long at = ((((long long)g * a.pairs + (tile >> 1)) * a.Hkv + hk) * a.parts) * 256 + (tile & 1) * 128 + in_tile;
     for (int i0 = 0; i0 < np; i0 += 8) {
       float2 v[8];
@@ -1183,6 +1187,7 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   a.scale_cap = cap > 0.f ? 2.f * scale * kLog2e / cap : 0.f;
   a.groups = groups;
   a.most_shared = most_shared;
+  a.most_rows = pairs * 2 * (128 / share);
   a.cu_rows = cu_rows;
   a.shared = shared;
   a.own_o = own_o;

@@ -181,7 +181,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     part = blockIdx.x;
     per = kBM / share;
     q_start = a.cu_rows[seq];                                   // sequences of the group
-    q_len = min(a.cu_rows[seq + 1], a.batch) - q_start;
+    q_len = q_start < 0 ? 0 : min(a.cu_rows[seq + 1], a.batch) - q_start;      // (see group_of in scored_decode.cu)
     q0 = pair * 2 * per;
     k_start = seq * a.key_stride;
     kv_len = min(a.shared[seq], a.most_shared);

@@ -51,7 +51,8 @@ class ScoreRules(NamedTuple):
 class SharedPrefix:
     """Rows [cu_rows[g], cu_rows[g + 1]) of a decode batch share their first lens[g] keys: those are read through the
     page list of the group's first row, once for all its rows.  ``max_rows`` and ``max_len`` bound the groups' sizes
-    for the host.  Rows past the last group share nothing.  A prefix may be longer than some of its rows, which end in it;
+    for the host.  Rows before the first group and past the last one share nothing; rows of a group that begins before
+    row 0 or has more rows than told neither, and set the device status (on the CPU the former raises).  A prefix may be longer than some of its rows, which end in it;
     a value in it that is not finite may then reach a shorter row, as one of the row's own group sees it."""
     cu_rows: torch.Tensor      # int32 [groups + 1]
     lens: torch.Tensor         # int32 [groups]
@@ -432,7 +433,9 @@ def _decode_cpu(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k
         at = page_table[b, j // page].long()
         if shared is not None:
             g = int(torch.searchsorted(shared.cu_rows, b, right=True)) - 1
-            if g < shared.groups:
+            if 0 <= g < shared.groups:
+                if int(shared.cu_rows[g]) < 0:
+                    raise IndexError(f"group {g} begins at row {int(shared.cu_rows[g])}")
                 other = page_table[int(shared.cu_rows[g]), j // page].long()
                 at = torch.where(j < int(shared.lens[g]), other, at)
         if int(at.min()) < 0 or int(at.max()) >= pages:
