@@ -32,3 +32,45 @@ def test_a_window_of_all_keys_is_no_window_for_single_rows(bits):
     got = S.decode_attention(q, kc, vc, table, n, 0.125, S.ScoreRules(window=2 ** 31 - 1), k_scale=ks, v_scale=vs)
     N.raise_on_device_error()
     O.check(got, *O.decode(q, kc, vc, table, n, 0.125, ks=ks, vs=vs))
+
+
+def saturated(rows, keys, Hq, Hkv, D, cap, near, slope):
+    """Queries and keys whose scores are all at -cap, a slope under which keys `near` away weigh half a percent of the row's own,
+    and values that make up for it: 1 near a row, 100 far from the last one."""
+    u = torch.where(torch.arange(D, device=DEV) % 3 == 0, 1.0, -1.0)
+    q = u.expand(rows, Hq, D).to(BF16).contiguous()
+    k = (-u * (10 * cap * 8 / D)).expand(keys, Hkv, D).to(BF16).contiguous()      # scale 1 / 8: scores of -10 cap
+    v = torch.ones(keys, Hkv, D, device=DEV)
+    v[:max(0, keys - near)] = 100.0
+    return q, k, v.to(BF16), torch.full((Hq,), slope, device=DEV)
+
+
+@pytest.mark.parametrize("rows", [4000, 20])
+@pytest.mark.parametrize("cap,slope,near", [(55.0, 0.004, 1300), (55.4, 0.01, 500), (50.0, 0.03, 170), (28.0, 0.004, 1300)])
+def test_far_keys_under_a_cap_and_a_bias_keep_their_weight(rows, cap, slope, near):
+    """All scores at the cap's lower end: the weights that stand in for a running maximum start from the smallest."""
+    keys = 4000
+    q, k, v, sl = saturated(rows, keys, 4, 2, 64, cap, near, slope)
+    cu_q, cu_k = (torch.tensor([0, x], dtype=I32, device=DEV) for x in (rows, keys))
+    assert rows > 1000 or N.kernels().us_scored_flash_parts(1, rows, keys, 4, 2) > 1
+    got = S.prompt_attention(q, k, v, cu_q, cu_k, rows, keys, 0.125, S.ScoreRules(cap, sl))
+    N.raise_on_device_error()
+    O.check(got, *O.prompt(q, k, v, cu_q, cu_k, 0.125, cap, sl))
+
+
+@pytest.mark.parametrize("cap,slope,near", [(55.0, 0.004, 1300), (55.4, 0.01, 500)])
+def test_a_far_shared_prefix_under_a_cap_and_a_bias_keeps_its_weight(cap, slope, near):
+    """Eight rows with `near` keys of their own behind a prefix of 3008."""
+    page, prefix, rows = 16, 3008, 8
+    lens = [prefix + near + i for i in range(rows)]
+    q, kc, vc, _, _, table, n = make(23, lens, 4, 2, 64, page, 16)
+    qs, k, v, sl = saturated(rows, prefix + 2 * near, 4, 2, 64, cap, 2 * near, slope)
+    for b in range(rows):
+        table[b, :prefix // page] = table[0, :prefix // page]
+        pos = torch.arange(lens[b], device=DEV)
+        kc[table[b, pos // page].long(), pos % page] = k[:lens[b]]
+        vc[table[b, pos // page].long(), pos % page] = v[:lens[b]]
+    plan = S.SharedPrefix(torch.tensor([0, rows], dtype=I32, device=DEV), torch.tensor([prefix], dtype=I32, device=DEV), rows, prefix)
+    got = S.decode_attention(qs, kc, vc, table, n, 0.125, S.ScoreRules(cap, sl), shared=plan)
+    N.raise_on_device_error()
+    O.check(got, *O.decode(qs, kc, vc, table, n, 0.125, cap, sl))

@@ -880,11 +880,15 @@ void set_rules(ScoredArgs& a, float scale, float cap, const float* slopes) {
     a.reach = mag > 1e-4 && mag < 1e4 ? (float)(kPolyReach / mag) : -1.f;
     a.scale_cap = (float)(2.0 * k * kLog2e);
     a.cap_log2 = cap * kLog2e;
-    a.base = a.cap_log2 > 40.f ? a.cap_log2 - 40.f : 0.f;      // weights in [2^(-cap_log2 - base), 2^40]
+    // Weights in [2^(-cap_log2 - base), 2^40], or, as a distance bias takes them down from there, in [.., 2^64]: 2^20 keys of
+    // values up to 2^44 stay in FP32's range
+    const float top = slopes ? 64.f : 40.f;
+    a.base = a.cap_log2 > top ? a.cap_log2 - top : 0.f;
   }
 }
-// Caps under which weights need no maximum: the smallest one is above 2^-121.
-bool small_cap(const ScoredArgs& a) { return a.cap_log2 + a.base <= 120.f; }
+// Caps under which weights need no maximum (those up to 55.45).  Without a bias the smallest weight is 2^-120 at least, and
+// none is lost.  With one a row's own key weighs 2^-96 at least, so a key that FP32 ends above (2^-126) weighs under 2^-30 of it.
+bool small_cap(const ScoredArgs& a) { return a.cap_log2 + a.base <= (a.slopes ? 96.f : 120.f); }
 
 template <int D, bool CAP, bool BIAS, bool FIXED, int MODE>
 int start(dim3 grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const ScoredArgs& a, cudaStream_t stream) {
