@@ -74,3 +74,31 @@ def test_a_far_shared_prefix_under_a_cap_and_a_bias_keeps_its_weight(cap, slope,
     got = S.decode_attention(qs, kc, vc, table, n, 0.125, S.ScoreRules(cap, sl), shared=plan)
     N.raise_on_device_error()
     O.check(got, *O.decode(qs, kc, vc, table, n, 0.125, cap, sl))
+
+
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("call", ["prompt", "parts", "single", "single-8", "shared"])
+def test_negative_slopes_set_the_status(call, cap):
+    """In every launch that reads them; zeros do not."""
+    for value, bad in ((-0.25, True), (0.0, False)):
+        sl = slopes(8)
+        sl[5] = value
+        rules = S.ScoreRules(cap, sl)
+        N.raise_on_device_error()
+        if call in ("prompt", "parts"):
+            rows, keys = (300, 300) if call == "prompt" else (9, 5000)
+            q, k, v, cu_q, cu_k = packed(24, [rows], [keys], 8, 2, 64)
+            got = S.prompt_attention(q, k, v, cu_q, cu_k, rows, keys, 0.125, rules)
+        else:
+            q, kc, vc, ks, vs, table, n = make(25, [400, 390], 8, 2, 64, 16, 8 if call == "single-8" else 16)
+            plan = None
+            if call == "shared":
+                table[1, :20] = table[0, :20]
+                plan = S.SharedPrefix(torch.tensor([0, 2], dtype=I32, device=DEV), torch.tensor([320], dtype=I32, device=DEV), 2, 320)
+            got = S.decode_attention(q, kc, vc, table, n, 0.125, rules, k_scale=ks, v_scale=vs, shared=plan)
+        if bad:
+            with pytest.raises(RuntimeError):
+                N.raise_on_device_error()
+        else:
+            N.raise_on_device_error()
+            assert torch.isfinite(got).all()

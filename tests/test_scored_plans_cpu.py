@@ -1,8 +1,8 @@
-"""Plans of shared prefixes on the CPU: what is refused, and rows that share nothing."""
+"""Plans of shared prefixes and slopes on the CPU: what is refused, and rows that share nothing."""
 import pytest
 import torch
 
-from test_scored_cpu import decode_args
+from test_scored_cpu import decode_args, prompt_args
 from uniserve_v1_b200.ops import scored as S
 
 I32 = torch.int32
@@ -34,3 +34,11 @@ def test_a_group_that_begins_before_the_batch_raises():
     plan = S.SharedPrefix(torch.tensor([-1, 2], dtype=I32), torch.tensor([2], dtype=I32), 3, 2)
     with pytest.raises(IndexError, match="begins"):
         S.decode_attention(**decode_args(shared=plan))
+
+
+def test_negative_slopes_are_refused():
+    rules = S.ScoreRules(slopes=torch.tensor([0.5, 0.0, -0.25, 0.1]))
+    with pytest.raises(ValueError, match="negative"):
+        S.prompt_attention(**prompt_args(rules=rules))
+    with pytest.raises(ValueError, match="negative"):
+        S.decode_attention(**decode_args(rules=rules))

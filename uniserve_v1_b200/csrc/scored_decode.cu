@@ -448,6 +448,7 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
         m[nt][e] = -INFINITY;
         l[nt][e] = 0.f;
         bias[nt][e] = a.slopes && h < share ? a.slopes[hk * share + h] * 1.4426950408889634f : 0.f;
+        if (bias[nt][e] < 0.f) us_dev_fail(a.status, US_DEV_BOUNDS);
         factor[nt][e] = (a.cap_log2 > 0.f ? a.scale_cap : a.scale_log2) * (FMT == 16 ? 1.f : __shfl_sync(0xffffffffu, back, (c4 * 2 + e) * 4));
       }
 #pragma unroll

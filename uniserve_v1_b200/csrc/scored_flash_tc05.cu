@@ -501,6 +501,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         hi = min(kv_len, p + 1);
         if (BIAS) sl = a.slopes[head] * kLog2e;
       }
+      if (BIAS && sl < 0.f) us_dev_fail(a.status, US_DEV_BOUNDS);      // (a fixed base has no room for scores that grow with distance)
       // FP16 operands: the scores' and the outputs' factors
       const bool half = MODE == 1 && a.q_back;
       float row_factor = 1.f, out_factor = 1.f;

@@ -43,7 +43,8 @@ _TILE = 128                # rows of a tile, keys of a block of the prompt kerne
 class ScoreRules(NamedTuple):
     """What happens to a score between scale q.k and the softmax."""
     cap: float = 0.0                            # > 0 (2^-20 to 1024): cap * tanh(score / cap)
-    slopes: Optional[torch.Tensor] = None       # FP32 [Hq], not negative: - slope * |position - key|
+    # FP32 [Hq]: - slope * |position - key|.  A negative one that a call uses sets the device status (on the CPU it raises).
+    slopes: Optional[torch.Tensor] = None
     window: int = 0                             # > 0: the last `window` keys, the row's own included
 
 
@@ -103,6 +104,8 @@ def _check_rules(rules, Hq, at):
         raise ValueError(f"a cap is 0 (none) or in [2^-20, {MAX_CAP}], a window in [0, 2^31); got {cap}, {window}")
     if s is not None and (s.dtype != F32 or s.shape != (Hq,) or not s.is_contiguous() or s.get_device() != at):
         raise ValueError(f"slopes are a contiguous float32 [{Hq}] beside the queries; got {tuple(s.shape)} {s.dtype}")
+    if s is not None and at < 0 and bool((s < 0).any()):
+        raise ValueError("slopes are not negative")
 
 
 def _heads(q, k, v, what):
