@@ -82,6 +82,8 @@ def main():
     ap.add_argument("--persist", action="store_true",
                     help="decode: the persistent kernel (bf16 pages)")
     a = ap.parse_args()
+    if a.kv in ("int8", "int4") and a.op != "scored-decode":
+        ap.error(f"argument --kv: {a.kv} pages are scored-decode's; {a.op} has none")
     tbs, tfl, tag = peaks()
     dev, bf = "cuda", torch.bfloat16
     g = torch.Generator(device=dev).manual_seed(0)
