@@ -102,3 +102,35 @@ def test_negative_slopes_set_the_status(call, cap):
         else:
             N.raise_on_device_error()
             assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("D", [128, 64, 40])
+@pytest.mark.parametrize("new,keys,before,behind,most", [([200, 31], [200, 60], 0, 50, 200), ([200, 31], [200, 60], 3, 160, 200),
+                                                         ([5], [3000], 2, 9, 16), ([5], [3000], 0, 0, 5), ([0, 0], [7, 0], 0, 40, 64),
+                                                         ([1, 2], [1, 2], 0, 3000, 2), ([3], [3], 700, 700, 3)])
+def test_rows_of_no_sequence(new, keys, before, behind, most, D):
+    """Zeros in an output of the call's own, whatever the memory held; as they were in a given one."""
+    q, k, v, _, cu_k = packed(26, [before + sum(new) + behind], keys, 4, 2, D)
+    cu_q = (torch.tensor([0] + new, device=DEV).cumsum(0) + before).to(I32)
+    end = before + sum(new)
+    want, bound = O.prompt(q, k, v, cu_q, cu_k, 0.125)
+    for _ in range(3):
+        soil = [torch.full_like(q, float("nan")) for _ in range(4)]
+        del soil
+        got = S.prompt_attention(q, k, v, cu_q, cu_k, most, max(keys), 0.125)
+        N.raise_on_device_error()
+        O.check(got, want, bound)
+        assert not got[:before].any() and not got[end:].any()
+    out = torch.full_like(q, 7.0)
+    S.prompt_attention(q, k, v, cu_q, cu_k, most, max(keys), 0.125, out=out)
+    N.raise_on_device_error()
+    assert (out[:before] == 7).all() and (out[end:] == 7).all()
+    O.check(out[before:end], want[before:end], bound[before:end])
+
+
+def test_no_sequences_at_all():
+    q, k, v, _, _ = packed(27, [20], [5], 4, 2, 64)
+    none = torch.zeros(1, dtype=I32, device=DEV)
+    soil = torch.full_like(q, float("nan"))
+    del soil
+    assert not S.prompt_attention(q, k, v, none, none, 0, 0, 0.125).any()

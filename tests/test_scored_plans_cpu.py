@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_scored_cpu import decode_args, prompt_args
+from test_scored_cpu import decode_args, prompt_args, rnd
 from uniserve_v1_b200.ops import scored as S
 
 I32 = torch.int32
@@ -42,3 +42,13 @@ def test_negative_slopes_are_refused():
         S.prompt_attention(**prompt_args(rules=rules))
     with pytest.raises(ValueError, match="negative"):
         S.decode_attention(**decode_args(rules=rules))
+
+
+def test_rows_of_no_sequence_before_the_first_and_past_the_last():
+    """Zeros, or what a given output held."""
+    args = prompt_args(q=rnd(9, 4, 16), cu_q=torch.tensor([2, 6], dtype=I32))
+    got = S.prompt_attention(**args)
+    assert not got[:2].any() and not got[6:].any() and got[2:6].any()
+    out = torch.full_like(got, 5.0)
+    S.prompt_attention(**args, out=out)
+    assert (out[:2] == 5).all() and (out[6:] == 5).all() and torch.equal(out[2:6], got[2:6])

@@ -69,6 +69,7 @@ struct ScoredArgs {
   int most_shared;                            // keys of a prefix at most
   int max_pages, pages, page, batch, pairs, parts, blocks_per_part;
   int n, max_q, max_k;                        // sequences, the longest one's rows and keys
+  int fill;                                   // zeros in the output rows of no sequence
   float *part_o, *part_ml;
   unsigned int* status;
 };
@@ -174,6 +175,14 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       q_len = min(q_len, a.max_q);
     }
     if (short_of && tid == 0) us_dev_fail(a.status, US_DEV_BOUNDS);
+    if (a.fill && warp == kThreads / 32 - 1) {      // a warp that has nothing else to do
+      const int before = max(0, min(a.cu_q[0], a.Tq)), end = max(before, min(a.cu_q[a.n], a.Tq));
+      const long long ctas = (long long)gridDim.x * gridDim.y * gridDim.z;
+      for (long long i = blockIdx.x + (long long)gridDim.x * (blockIdx.y + (long long)gridDim.y * blockIdx.z); i < before + a.Tq - end; i += ctas) {
+        uint4* row = reinterpret_cast<uint4*>(a.out + (i < before ? i : end + i - before) * a.ldo);
+        for (int c = lane; c < a.Hq * (kD / 8); c += 32) row[c] = make_uint4(0, 0, 0, 0);
+      }
+    }
   } else {
     seq = blockIdx.z;
     hk = blockIdx.y % a.Hkv;
@@ -947,12 +956,13 @@ US_API int us_scored_flash_parts(int n, int max_q, int max_k, int Hq, int Hkv) {
 }
 
 // q [Tq, Hq, D], k / v [Tk, Hkv, D], out [Tq, Hq, D], bf16 with row pitches; cu_q / cu_k [n + 1].  docs [Tk] with ranges
-// (int32 [2 (Tk / 128 + n + 1)], written here), prefix [n], slopes [Hq]: or null.  cap 0, window 0: none.  parts > 1: part_o,
+// (int32 [2 (Tk / 128 + n + 1)], written here), prefix [n], slopes [Hq]: or null.  cap 0, window 0: none.  fill: output rows of
+// no sequence become zeros (some warps of the launch have time for n max_q of them).  parts > 1: part_o,
 // part_ml [parts][n][max_q][Hq][D and 2] take the parts' results.
 US_API int us_scored_flash(const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, void* out,
                            long long ldo, const int* cu_q, const int* cu_k, int n, int Tq, int Tk, int Hq, int Hkv, int D,
                            int max_q, int max_k, float scale, float cap, const float* slopes, int causal, int window,
-                           const int* docs, const int* prefix, void* ranges, int parts, float* part_o, float* part_ml, void* stream_) {
+                           const int* docs, const int* prefix, void* ranges, int fill, int parts, float* part_o, float* part_ml, void* stream_) {
   US_REQUIRE(q && k && v && out && cu_q && cu_k && n >= 1 && n <= 65535 && Tq >= 1 && Tk >= 1 && max_q >= 1 && max_q <= 65535 * 2 * kBM && max_k >= 0);
   US_REQUIRE((D == 64 || D == 128) && Hkv >= 1 && Hq >= 1 && Hq <= 65535 && Hq % Hkv == 0 && window >= 0 && cap >= 0.f);
   US_REQUIRE(((ldq | ldk | ldv | ldo) % 8) == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16) == 0);
@@ -982,6 +992,7 @@ US_API int us_scored_flash(const void* q, long long ldq, const void* k, long lon
   a.n = n;
   a.max_q = max_q;
   a.max_k = max_k;
+  a.fill = fill;
   // (a window of all keys that a sequence may have is none; rows stand before the first key too, and their positions less the
   // window have to be 32-bit numbers)
   a.window = window < kMaxBlocks * kBN ? window : kMaxBlocks * kBN;

@@ -28,7 +28,7 @@ N.register_signatures({
     "us_scored_decode_scratch": (L, [I]),
     "us_scored_decode": (I, [P, L, P, P, P, P, P, I, P, P, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, P, P, I,
                              P, P, P, P, I, I, I, P]),
-    "us_scored_flash": (I, [P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, I, P, P, P, I, P, P, P]),
+    "us_scored_flash": (I, [P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, I, N.F, N.F, P, I, I, P, P, P, I, I, P, P, P]),
     "us_scored_flash_parts": (I, [I, I, I, I, I]),
     "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, I, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
 })
@@ -128,8 +128,8 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
 
     and, with ``docs`` (int32 [Tk], a number for every key; a row has that of the key at its position), where both
     belong to the same document.  A row before its sequence's first key (nq > nk) has no document and sees nothing
-    under ``docs``.  ``prefix``: int32 [n].  Returns bf16 [Tq, Hq, D]; rows past cu_q[n] of a given ``out`` are left
-    as they were.  What keys and values hold past a sequence's end never reaches it; a key or value that is not finite
+    under ``docs``.  ``prefix``: int32 [n].  Returns bf16 [Tq, Hq, D]; rows of no sequence (past cu_q[n]) are zeros, and
+    left as they were in a given ``out``.  What keys and values hold past a sequence's end never reaches it; a key or value that is not finite
     may reach any row of its own sequence that shares a block of 128 keys with one that sees it."""
     _heads(q, k, v, "prompt_attention")
     Tq, Hq, D = q.shape
@@ -149,8 +149,8 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
         res = _prompt_cpu(q, k, v, cu_q, cu_k, scale, rules, causal, docs, prefix)
         if out is None:
             return res
-        end = int(cu_q[-1])
-        out[:end] = res[:end]
+        first, end = int(cu_q[0]), int(cu_q[-1])
+        out[first:end] = res[first:end]
         return out
     if q.dtype != BF16 or k.dtype != BF16 or v.dtype != BF16:
         raise ValueError(f"scored attention is served in bfloat16; got {q.dtype}, {k.dtype}, {v.dtype}")
@@ -167,12 +167,14 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
         got = prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules, causal, docs, prefix)[..., :D]
         if out is None:
             return got.contiguous()
-        keep = torch.arange(Tq, device=q.device)[:, None, None] < cu_q[-1]
-        return out.copy_(torch.where(keep, got, out))
+        rows = torch.arange(Tq, device=q.device)[:, None, None]
+        return out.copy_(torch.where((rows >= cu_q[0]) & (rows < cu_q[-1]), got, out))
     q, k, v = _dense_heads(q), _dense_heads(k), _dense_heads(v)
     to = out
-    if out is None:
-        to = torch.empty_like(q) if q.is_contiguous() else q.new_empty(Tq, Hq, D)
+    fill = False
+    if out is None:        # rows of no sequence: the launch's, unless they may be most of the work
+        fill = Tq <= n * max_q
+        to = q.new_empty(Tq, Hq, D) if fill else q.new_zeros(Tq, Hq, D)
     elif not _fits(out):
         to = out.contiguous() if not out.is_contiguous() else out.clone()
     if n and Tq and max_q > 0:
@@ -194,8 +196,8 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
                 pm = torch.empty(parts * n * max_q * Hq * 2, dtype=F32, device=q.device)
         launch("us_scored_flash", 1 + (docs is not None) + (parts > 1), q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0),
                v.data_ptr(), v.stride(0), to.data_ptr(), to.stride(0), cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, Hq, Hkv, D,
-               max_q, max_k, scale, rules.cap, _at(rules.slopes), causal, rules.window, _at(docs), _at(prefix), _at(ranges), parts, _at(po),
-               _at(pm))
+               max_q, max_k, scale, rules.cap, _at(rules.slopes), causal, rules.window, _at(docs), _at(prefix), _at(ranges), fill, parts,
+               _at(po), _at(pm))
     if out is not None and to is not out:
         return out.copy_(to)
     return to
