@@ -134,3 +134,29 @@ def test_no_sequences_at_all():
     soil = torch.full_like(q, float("nan"))
     del soil
     assert not S.prompt_attention(q, k, v, none, none, 0, 0, 0.125).any()
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("power", [127, 126, -126, -130])
+def test_queries_at_the_ends_of_their_range(bits, power):
+    """The largest power of two of bf16 over small keys, and channels under its smallest normal number."""
+    lens = [700, 33, 5]
+    q, kc, vc, ks, vs, table, n = make(28, lens, 8, 2, 64, 16, bits)
+    if bits == 16:
+        kc.mul_(2.0 ** -12)
+    else:
+        ks.mul_(2.0 ** -12)
+    q = (q.double().clamp(-1.99, 1.99) * 2.0 ** (power - 1)).to(BF16)
+    q[:, :, 7] = 1.5 * 2.0 ** power
+    scale = 0.125 * 2.0 ** (12 - power) if power > 0 else 0.125 * 2.0 ** 120
+    want, bound = O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs)
+    got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs)
+    N.raise_on_device_error()
+    O.check(got, want, bound)
+    if bits == 16:
+        return
+    table[1:, 0] = table[0, 0]
+    plan = S.SharedPrefix(torch.tensor([0, 3], dtype=I32, device=DEV), torch.tensor([5], dtype=I32, device=DEV), 3, 5)
+    got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=plan)
+    N.raise_on_device_error()
+    O.check(got, *O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[5] * 3))

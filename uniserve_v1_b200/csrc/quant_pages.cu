@@ -329,11 +329,10 @@ __global__ void __launch_bounds__(512) prefix_scales_kernel(const PrefixArgs a) 
   uint32_t most = 0;
   for (int i = lane; i < a.dim; i += 32) most = max(most, (uint32_t)__bfloat16_as_ushort(from[i]) & 0x7fffu);
   most = __reduce_max_sync(0xffffffffu, most);
-  const int e = (int)(most >> 7);
-  const bool scaled = e > 0 && e < 254;
-  const float down = scaled ? power_of_two(254 - e) : 1.f;
+  const int e = min(max((int)(most >> 7), 1), 253);       // (the ends of the range beside the ones that have a reciprocal)
+  const float down = power_of_two(254 - e);
   for (int i = lane; i < a.dim; i += 32) a.qo[(long long)row * a.dim + i] = __float2half_rn(us::bf2f(from[i]) * down);
-  if (lane == 0) a.q_back[row] = scaled ? power_of_two(e) : 1.f;
+  if (lane == 0) a.q_back[row] = power_of_two(e);
 }
 
 template <int BITS>

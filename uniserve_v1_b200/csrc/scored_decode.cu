@@ -421,10 +421,10 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
         for (int k = 0; k < KS; ++k) most = __vmaxu2(most, __vmaxu2(qf[nt][k][0] & 0x7fff7fffu, qf[nt][k][1] & 0x7fff7fffu));
         most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = (int)(max(most & 0xffffu, most >> 16) >> 7);
-        const bool scaled = e > 0 && e < 254;
-        const float down = scaled ? power_of_two(254 - e) : 1.f;
-        back = scaled ? power_of_two(e) : 1.f;
+        // (the ends of the range beside the ones that have a reciprocal: channels of up to 4, and under 1)
+        const int e = min(max((int)(max(most & 0xffffu, most >> 16) >> 7), 1), 253);
+        const float down = power_of_two(254 - e);
+        back = power_of_two(e);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
