@@ -160,3 +160,17 @@ def test_queries_at_the_ends_of_their_range(bits, power):
     got = S.decode_attention(q, kc, vc, table, n, scale, k_scale=ks, v_scale=vs, shared=plan)
     N.raise_on_device_error()
     O.check(got, *O.decode(q, kc, vc, table, n, scale, ks=ks, vs=vs, expanded=[5] * 3))
+
+
+def test_batches_over_huge_page_tables_go_in_slices():
+    """Five short sequences whose lists have room for 2^33 keys."""
+    q, kc, vc, _, _, table, n = make(29, [700, 33, 0, 300, 65], 32, 4, 64, 16, 16)
+    wide = torch.zeros(5, 1 << 28, dtype=I32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    assert 0 < S._most_seqs(32, 4, (1 << 28) * 16) < 5
+    got = S.decode_attention(q, kc, vc, wide, n, 0.125)
+    N.raise_on_device_error()
+    O.check(got, *O.decode(q, kc, vc, table, n, 0.125))
+    plan = S.SharedPrefix(torch.tensor([0, 5], dtype=I32, device=DEV), torch.tensor([8], dtype=I32, device=DEV), 5, 8)
+    with pytest.raises(ValueError, match="counts"):
+        S.decode_attention(q, kc, vc, wide, n, 0.125, shared=plan)

@@ -52,3 +52,16 @@ def test_rows_of_no_sequence_before_the_first_and_past_the_last():
     out = torch.full_like(got, 5.0)
     S.prompt_attention(**args, out=out)
     assert (out[:2] == 5).all() and (out[6:] == 5).all() and torch.equal(out[2:6], got[2:6])
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(32, 4), (64, 64), (17, 1), (128, 128), (300, 100)])
+@pytest.mark.parametrize("keys", [0, 1, 4096, 1 << 20, 1 << 27, (1 << 31) - 1, 1 << 40])
+def test_the_tile_list_of_a_launch_stays_in_31_bits(Hq, Hkv, keys):
+    """Tiles of 32 keys of every sequence and key head (or sixteen of its query heads); one more sequence would not fit."""
+    most = S._most_seqs(Hq, Hkv, keys)
+    tiles = Hkv * -(-(Hq // Hkv) // 16) * max(1, -(-keys // 32))
+    assert 0 <= most <= S.MAX_SEQS and most * tiles < 1 << 31
+    assert most == S.MAX_SEQS or (most + 1) * (tiles + Hkv * -(-(Hq // Hkv) // 16)) >= 1 << 31
+    # (the call's own shorter test never passes what does not fit)
+    for B in (1, most, most + 1, 700):
+        assert B <= most or B > S.MAX_SEQS or B * Hq * (keys + 64) >= 1 << 36

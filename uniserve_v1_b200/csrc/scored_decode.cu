@@ -1151,6 +1151,8 @@ US_API int us_scored_decode(const void* q, long long ldq, const void* kc, const 
   US_REQUIRE(bits == 16 || ((bits == 8 || bits == 4) && ks && vs && page % 2 == 0 && (((uintptr_t)ks | (uintptr_t)vs) % 4) == 0));
   US_REQUIRE((long long)pages * page <= 0x7fffffffLL && window >= 0 && cap >= 0.f);
   if ((long long)pages * page * Hkv * (D * bits / 128) >= 0xffffffffLL) return US_ERR_LIMIT;   // places are 32 bits of 16 bytes
+  // the tile list of the longest sequences that the page table holds is counted in 31 bits
+  if ((((long long)max_pages * page + 31) / 32 + 1) * B > 0x7fffffffLL / (Hkv * ((Hq / Hkv + 15) / 16))) return US_ERR_LIMIT;
   US_REQUIRE((ldq % 8) == 0 && (ldo % 2) == 0 && (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) % 16) == 0 &&
              ((uintptr_t)out % 4) == 0);
   const int share = Hq / Hkv;

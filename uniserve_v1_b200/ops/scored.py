@@ -33,7 +33,7 @@ N.register_signatures({
     "us_scored_prefix": (I, [P, L, P, L, P, L, P, P, I, I, P, I, I, I, P, P, P, I, I, I, I, I, N.F, N.F, P, P, P, I, I, I, P]),
 })
 
-MAX_SEQS = 704             # sequences of one decode launch; larger batches go in slices
+MAX_SEQS = 704             # sequences of one decode launch; larger batches (and ones of huge page tables) go in slices
 MAX_KEYS = 1 << 20         # keys of a prompt's sequence
 MAX_CAP = 1024.0           # scores under a larger one lose what a tanh near 1, less 1, loses of FP32
 _FEW_ROWS = 1 << 15        # rows times heads: more of them have tiles for over half of a GPU
@@ -270,6 +270,11 @@ def _chunks(Hq, Hkv):
     return -(-(Hq // Hkv) // 16)
 
 
+def _most_seqs(Hq, Hkv, keys):
+    """Sequences of a decode launch over page lists of ``keys``: its list of tiles (of 32 keys) is counted in 31 bits."""
+    return min(MAX_SEQS, ((1 << 31) - 1) // (Hkv * _chunks(Hq, Hkv) * (-(-keys // 32) + 1)))
+
+
 def _prefix_plan(shared: SharedPrefix, Hq, Hkv, sms):
     """(tile pairs a group, parts, key blocks a part) of the prefix launch: its CTAs have 256 rows (query heads of a
     key head times sequences) and a share of the prefix's 128-key blocks, as many shares as fill the GPU once."""
@@ -362,10 +367,14 @@ def decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules: Scor
     if at != current_device():
         with torch.cuda.device(at):
             return decode_attention(q, kcache, vcache, page_table, seq_lens, scale, rules, starts, k_scale, v_scale, shared, work, out)
-    if B > MAX_SEQS:
+    keys = page_table.shape[1] * page
+    if B > MAX_SEQS or B * Hq * (keys + 64) >= 1 << 36 and B > _most_seqs(Hq, Hkv, keys):
+        most = _most_seqs(Hq, Hkv, keys)
+        if not most or shared is not None:
+            raise ValueError(f"{B} sequences of {Hq} heads over page lists of {page_table.shape[1]} pages of {page} are more than a launch counts")
         out = q.new_empty(B, Hq, D) if out is None else out
-        for b in range(0, B, MAX_SEQS):
-            e = min(B, b + MAX_SEQS)
+        for b in range(0, B, most):
+            e = min(B, b + most)
             decode_attention(q[b:e], kcache, vcache, page_table[b:e], seq_lens[b:e], scale, rules,
                              None if starts is None else starts[b:e], k_scale, v_scale, None, work, out[b:e])
         return out
