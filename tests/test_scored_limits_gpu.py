@@ -174,3 +174,27 @@ def test_batches_over_huge_page_tables_go_in_slices():
     plan = S.SharedPrefix(torch.tensor([0, 5], dtype=I32, device=DEV), torch.tensor([8], dtype=I32, device=DEV), 5, 8)
     with pytest.raises(ValueError, match="counts"):
         S.decode_attention(q, kc, vc, wide, n, 0.125, shared=plan)
+
+
+@pytest.mark.parametrize("more", [0, 512])
+@pytest.mark.parametrize("kind", ["plain", "documents", "window", "parts"])
+def test_sequences_that_leave_the_tensors_set_the_status(kind, more):
+    """The second of two ends behind the last key, or row, or begins before the first; the first one is served.
+    (Told of more keys, the plain one goes in parts too.)"""
+    rows, keys = ([20, 9], [4000, 3000]) if kind == "parts" else ([300, 200], [300, 700])
+    q, k, v, cu_q, cu_k = packed(30, rows, keys, 4, 2, 64)
+    docs = (torch.arange(sum(keys), device=DEV) // 50).to(I32) if kind == "documents" else None
+    rules = S.ScoreRules(window=100 if kind == "window" else 0)
+    want, bound = O.prompt(q, k, v, cu_q, cu_k, 0.125, window=rules.window, docs=docs)
+    guard = torch.full((sum(rows) + 200, 4, 64), 7.0, dtype=BF16, device=DEV)
+    for which, i, by in (("k", 2, 500), ("k", 2, 100_000), ("q", 2, 60), ("k", 1, -keys[0] - 400), ("q", 1, -rows[0] - 3)):
+        a, b = cu_q.clone(), cu_k.clone()
+        (a if which == "q" else b)[i] += by
+        N.raise_on_device_error()
+        guard.fill_(7.0)
+        S.prompt_attention(q, k, v, a, b, max(rows), max(keys) + more, 0.125, rules, docs=docs, out=guard[:sum(rows)])
+        with pytest.raises(RuntimeError):
+            N.raise_on_device_error()
+        assert (guard[sum(rows):] == 7).all()
+        if i == 2:
+            O.check(guard[:rows[0]], want[:rows[0]], bound[:rows[0]])

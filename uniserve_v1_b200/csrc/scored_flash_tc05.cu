@@ -168,8 +168,12 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     kv_len = min(a.cu_k[seq + 1] - k_start, a.Tk - k_start);
     shift = (a.cu_k[seq + 1] - k_start) - (a.cu_q[seq + 1] - q_start);
     if (a.prefix) pre = max(0, min(a.prefix[seq], kv_len));
-    // rows and keys past what the host was told of the longest sequence: some or all are left out
-    bool short_of = q_len > (int)gridDim.z * 2 * per || kv_len > a.max_k;
+    // rows and keys past what the host was told of the longest sequence, or past the tensors: some or all are left out
+    bool short_of = q_len > (int)gridDim.z * 2 * per || kv_len > a.max_k || a.cu_q[seq + 1] > a.Tq || a.cu_k[seq + 1] > a.Tk;
+    if (q_start < 0 || k_start < 0) {
+      short_of = true;
+      q_len = 0;
+    }
     if (MODE == 2) {
       short_of |= q_len > a.max_q;
       q_len = min(q_len, a.max_q);
@@ -301,7 +305,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (see && ranges) {
         see = pb >= 0;
         if (see) {
-          const int2 d0 = ranges[max(pa, 0) / kBN], d1 = ranges[min(pb, kv_len - 1) / kBN], d = ranges[j];
+          const int2 d0 = ranges[min(max(pa, 0), kv_len - 1) / kBN], d1 = ranges[min(pb, kv_len - 1) / kBN], d = ranges[j];
           see = d.x <= max(d0.y, d1.y) && d.y >= min(d0.x, d1.x);
         }
       }
@@ -817,7 +821,7 @@ __global__ void __launch_bounds__(128) doc_ranges_kernel(const int* docs, const 
   US_PDL_PROLOGUE();
   const int seq = blockIdx.y, j = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int start = cu_k[seq], end = min(cu_k[seq + 1], Tk);
-  if (start + j * kBN >= end) return;
+  if (start < 0 || start + j * kBN >= end) return;
   int lo = 0x7fffffff, hi = -0x7fffffff - 1;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
@@ -843,7 +847,7 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const ScoredArgs a) {
   if (i >= rows) return;
   const int head = (int)(i % a.Hq), row = (int)(i / a.Hq % a.max_q), seq = (int)(i / a.Hq / a.max_q);
   const int start = a.cu_q[seq];
-  if (row >= min(a.cu_q[seq + 1], a.Tq) - start) return;
+  if (start < 0 || a.cu_k[seq] < 0 || row >= min(a.cu_q[seq + 1], a.Tq) - start) return;      // (such parts were not written)
   float M = -INFINITY, L = 0.f, acc[kC] = {};
   for (int p0 = 0; p0 < a.parts; p0 += 4) {            // four parts' loads in flight
     float2 ml[4];

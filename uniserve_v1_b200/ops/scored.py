@@ -121,7 +121,8 @@ def _heads(q, k, v, what):
 def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules = ScoreRules(), causal=True, docs=None,
                      prefix=None, out=None):
     """q [Tq, Hq, D], k / v [Tk, Hkv, D] bf16 (any strides; D a multiple of 8 up to 128), cu_q / cu_k int32 [n + 1] on the device,
-    max_q / max_k at least the longest sequence's rows and keys (more of them than that set the device status).  Row i of a
+    max_q / max_k at least the longest sequence's rows and keys (more of them than that set the device status, as do
+    sequences that leave the tensors: what is there of them is read, and no more).  Row i of a
     sequence with nq rows and nk keys stands at position p = i + nk - nq.  A key j is visible where
 
         (not causal or j <= p) and (no window or j > p - window),    or j < prefix[sequence],
