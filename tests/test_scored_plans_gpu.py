@@ -6,6 +6,7 @@ import scored_oracle as O
 from test_scored_decode_gpu import make, slopes
 from test_scored_flash_gpu import shared_batch
 from uniserve_v1_b200.ops import native as N
+from uniserve_v1_b200.ops import quant_pages as Q
 from uniserve_v1_b200.ops import scored as S
 
 pytestmark = pytest.mark.gpu
@@ -139,3 +140,30 @@ def test_rows_of_a_group_past_those_told_read_their_own_lists():
     with pytest.raises(RuntimeError):
         N.raise_on_device_error()
     O.check(got, *O.decode(q, kc, vc, table, n, scale))
+
+
+def one_key_above(bits, keys, rows, Hq, away, at):
+    """Queries and integer pages of a prefix of `keys` that `rows` share: key `at`'s weight is e^away times that of each other;
+    values of 1, and 0 there.  Scale 1 / 8, 64 channels."""
+    page = 64
+    kc, vc, ks, vs = Q.quant_planes(keys // page + 1, page, 1, 64, bits, DEV)
+    k, v = torch.zeros(keys, 1, 64, dtype=BF16, device=DEV), torch.ones(keys, 1, 64, dtype=BF16, device=DEV)
+    if away:
+        k[at], v[at] = away / 8, 0.0
+    Q.kv_write_quant(k, v, torch.arange(keys, device=DEV), kc, vc, ks, vs)
+    table = torch.arange(keys // page, device=DEV).to(I32).expand(rows, -1).contiguous()
+    n = torch.full((rows,), keys, dtype=I32, device=DEV)
+    plan = S.SharedPrefix(torch.tensor([0, rows], dtype=I32, device=DEV), torch.tensor([keys], dtype=I32, device=DEV), rows, keys)
+    return torch.ones(rows, Hq, 64, dtype=BF16, device=DEV), kc, vc, ks, vs, table, n, plan
+
+
+@pytest.mark.parametrize("rows,Hq", [(3, 2), (150, 128)])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("keys,away", [(1 << 20, 0.0), (1 << 20, 10.0), (1 << 21, 0.0)])
+def test_sums_of_millions_of_values_of_one_sign(keys, away, bits, rows, Hq):
+    """For many rows of many heads a prefix would be one part, and each of its sums one chain of products."""
+    q, kc, vc, ks, vs, table, n, plan = one_key_above(bits, keys, rows, Hq, away, 777)
+    got = S.decode_attention(q, kc, vc, table, n, 0.125, k_scale=ks, v_scale=vs, shared=plan)
+    N.raise_on_device_error()
+    want, bound = O.decode(q[:1, :1], kc, vc, table[:1], n[:1], 0.125, ks=ks, vs=vs, expanded=[keys])
+    O.check(got, want.expand(rows, Hq, -1), bound.expand(rows, Hq, -1))
