@@ -167,3 +167,15 @@ def test_sums_of_millions_of_values_of_one_sign(keys, away, bits, rows, Hq):
     N.raise_on_device_error()
     want, bound = O.decode(q[:1, :1], kc, vc, table[:1], n[:1], 0.125, ks=ks, vs=vs, expanded=[keys])
     O.check(got, want.expand(rows, Hq, -1), bound.expand(rows, Hq, -1))
+
+
+@pytest.mark.parametrize("rows,Hq", [(3, 2), (150, 128)])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("away", [17.5, 20.0, 24.0])
+def test_small_weights_of_an_integer_prefix_add_up(away, bits, rows, Hq):
+    """A key near the prefix's end, which is walked first, outweighs each of the others by more than FP16 has room for."""
+    q, kc, vc, ks, vs, table, n, plan = one_key_above(bits, 1 << 20, rows, Hq, away, (1 << 20) - 5)
+    got = S.decode_attention(q, kc, vc, table, n, 0.125, k_scale=ks, v_scale=vs, shared=plan)
+    N.raise_on_device_error()
+    want, bound = O.decode(q[:1, :1], kc, vc, table[:1], n[:1], 0.125, ks=ks, vs=vs, expanded=[1 << 20])
+    O.check(got, want.expand(rows, Hq, -1), bound.expand(rows, Hq, -1))

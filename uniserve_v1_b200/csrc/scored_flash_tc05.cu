@@ -517,6 +517,9 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (BIAS && sl < 0.f) us_dev_fail(a.status, US_DEV_BOUNDS);      // (a fixed base has no room for scores that grow with distance)
       // FP16 operands: the scores' and the outputs' factors
       const bool half = MODE == 1 && a.q_back;
+      // FP16 weights are held 2^14 times as large, 2^15 at most (the maximum may lag by one power of two): like those of the
+      // integer pages' own decode they keep their bits down to 2^-28 of the largest, and end at 2^-39
+      const float lift = half ? 14.f : 0.f, lag = half ? 1.f : kRescaleThreshold;
       float row_factor = 1.f, out_factor = 1.f;
       if (half) {
         const int2 top = a.exps[seq * a.Hkv + hk];
@@ -614,7 +617,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         };
         tc::tmem_ld_wait();
         by_row();
-        if (!FIXED && __any_sync(0xffffffffu, m_next - m_used > kRescaleThreshold)) rescale(m_next);
+        if (!FIXED && __any_sync(0xffffffffu, m_next - m_used > lag)) rescale(m_next);
         const int delta = p - kbase;
         // Whether the row's scores are cap's polynomial's.  (A comparison that a NaN fails: such a block takes the other
         // form, which passes it on.)
@@ -655,7 +658,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         bool through = false;
         auto pass = [&](auto with_mask) {
           constexpr bool MASK = decltype(with_mask)::value;
-          const float less = FIXED ? -base : m_used == -INFINITY ? 0.f : -m_used;
+          const float less = FIXED ? -base : m_used == -INFINITY ? lift : lift - m_used;
           const float step = delta > 0 ? sl : -sl, at = BIAS ? fmaf(-sl, fabsf((float)delta), less) : less;
           unsigned long long b2[4];
           const unsigned long long st2 = pack2(2.f * step, 2.f * step);
@@ -688,8 +691,8 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (!FIXED) {
             // of the maximum so far; a NaN fails the comparison, and the general form passes it on where the polynomial does not
             const float over = max2_nan(max2_nan(mxs[0], mxs[1]), max2_nan(mxs[2], mxs[3]));
-            through = __all_sync(0xffffffffu, over <= (MODE == 1 && half ? kRescaleThreshold : 64.f));    // FP16 ends at 2^16
-            m_next = fmaxf(m_used, m_used + over);
+            through = __all_sync(0xffffffffu, over <= (half ? lift + lag : 64.f));    // FP16 ends at 2^16
+            m_next = fmaxf(m_used, m_used + (over - lift));
           } else {
             through = true;
           }
@@ -731,7 +734,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             if (__any_sync(0xffffffffu, m_new > m_used)) rescale(m_new);
             m_next = m_used;
           }
-          const float less = FIXED || m_used == -INFINITY ? 0.f : m_used;
+          const float less = FIXED ? 0.f : m_used == -INFINITY ? -lift : m_used - lift;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             ls[c] = 0ull;
@@ -759,7 +762,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           const long long prow = prow0 + x * kBM;
           if (PARTS && row_ok) {
             const long long to = MODE == 2 ? part_row(q0 + x * per + (r >> a.pack), h + (r & ((1 << a.pack) - 1))) : prow + r;
-            *reinterpret_cast<float2*>(a.part_ml + to * 2) = make_float2(m_used, l_sum);
+            *reinterpret_cast<float2*>(a.part_ml + to * 2) = make_float2(m_used - lift, l_sum);
           }
           uint32_t all[kD];
 #pragma unroll
