@@ -198,3 +198,26 @@ def test_sequences_that_leave_the_tensors_set_the_status(kind, more):
         assert (guard[sum(rows):] == 7).all()
         if i == 2:
             O.check(guard[:rows[0]], want[:rows[0]], bound[:rows[0]])
+
+
+@pytest.mark.parametrize("rows,Hq,keys", [(600, 64, 1 << 20), (600, 64, 300_000), (9, 64, 1 << 20)])
+@pytest.mark.parametrize("window", [0, 700_000])
+def test_sums_of_a_million_values_of_one_sign(rows, Hq, keys, window):
+    """Products of weights and values that end just under a power of two, where cutting takes most.  A key of the block that is
+    walked first weighs e^9.7 times as much as each other."""
+    q = torch.ones(rows, Hq, 64, dtype=BF16, device=DEV)
+    k, v = torch.zeros(keys, 1, 64, dtype=BF16, device=DEV), torch.full((keys, 1, 64), 127 / 128, dtype=BF16, device=DEV)
+    far = 14 * 0.6931471805599453 - 0.0077821404420549    # weights of 129 / 128 2^-14 beside it
+    first = torch.full((64,), far / 8, dtype=torch.float64).to(BF16)      # scale 1 / 8, 64 channels
+    first[63] = (far * 8 - float(first[:63].double().sum()))
+    at = keys - rows - 1            # that every row sees
+    k[at], v[at] = first.to(DEV), 0.0
+    cu_q, cu_k = (torch.tensor([0, x], dtype=I32, device=DEV) for x in (rows, keys))
+    got = S.prompt_attention(q, k, v, cu_q, cu_k, rows, keys, 0.125, S.ScoreRules(window=window))
+    N.raise_on_device_error()
+    few = [0, rows // 2, rows - 1]
+    for i in few:                   # a row as the only one of its sequence: the same keys up to its own
+        end = keys - rows + 1 + i
+        want, bound = O.prompt(q[i:i + 1, :1], k[:end], v[:end], torch.tensor([0, 1], dtype=I32, device=DEV),
+                               torch.tensor([0, end], dtype=I32, device=DEV), 0.125, window=window)
+        O.check(got[i:i + 1], want.expand(1, Hq, -1), bound.expand(1, Hq, -1))

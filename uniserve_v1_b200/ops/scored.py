@@ -40,6 +40,9 @@ _FEW_ROWS = 1 << 15        # rows times heads: more of them have tiles for over 
 # Blocks of a part of a shared prefix.  The tensor unit cuts each product at some 2^-25 of the sum it is added to: 2^20 values of
 # one sign in one sum came out 0.9 % too small, 2^16 lose under 0.1 %.
 _LONGEST = 512
+# For the same reason prompts of more keys than this (which lose 0.4 % at most) go in parts of so many, as far as the parts have
+# room in some memory.
+_LONG_PROMPT, _LONG_ROOM = 1 << 18, 1 << 32
 _TILE = 128                # rows of a tile, keys of a block of the prompt kernel
 
 
@@ -134,7 +137,9 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
     belong to the same document.  A row before its sequence's first key (nq > nk) has no document and sees nothing
     under ``docs``.  ``prefix``: int32 [n].  Returns bf16 [Tq, Hq, D]; rows of no sequence (past cu_q[n]) are zeros, and
     left as they were in a given ``out``.  What keys and values hold past a sequence's end never reaches it; a key or value that is not finite
-    may reach any row of its own sequence that shares a block of 128 keys with one that sees it."""
+    may reach any row of its own sequence that shares a block of 128 keys with one that sees it.  The tensor unit cuts
+    what it adds: a sum of N values of one sign comes out up to N 2^-26 of itself small (N 2^18 at most, unless rows times
+    heads have no room for parts of the keys)."""
     _heads(q, k, v, "prompt_attention")
     Tq, Hq, D = q.shape
     Tk, Hkv, _ = k.shape
@@ -193,11 +198,15 @@ def prompt_attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, rules: ScoreRules
             cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
         prefix = None if prefix is None else prefix.contiguous()
         parts, po, pm = 1, None, None
-        if max_k > 8 * _TILE and n * max_q * Hq <= _FEW_ROWS:      # few rows over many keys: the keys in parts
-            parts = N.kernels().us_scored_flash_parts(n, max_q, max_k, Hq, Hkv)
+        if max_k > 8 * _TILE:
+            rows = n * max_q * Hq
+            if rows <= _FEW_ROWS:          # few rows over many keys: the keys in parts
+                parts = N.kernels().us_scored_flash_parts(n, max_q, max_k, Hq, Hkv)
+            if max_k > _LONG_PROMPT and -(-max_k // _LONG_PROMPT) * rows * D * 4 <= _LONG_ROOM:
+                parts = max(parts, -(-max_k // _LONG_PROMPT))
             if parts > 1:
-                po = torch.empty(parts * n * max_q * Hq * D, dtype=F32, device=q.device)
-                pm = torch.empty(parts * n * max_q * Hq * 2, dtype=F32, device=q.device)
+                po = torch.empty(parts * rows * D, dtype=F32, device=q.device)
+                pm = torch.empty(parts * rows * 2, dtype=F32, device=q.device)
         launch("us_scored_flash", 1 + (docs is not None) + (parts > 1), q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0),
                v.data_ptr(), v.stride(0), to.data_ptr(), to.stride(0), cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, Hq, Hkv, D,
                max_q, max_k, scale, rules.cap, _at(rules.slopes), causal, rules.window, _at(docs), _at(prefix), _at(ranges), fill, parts,
