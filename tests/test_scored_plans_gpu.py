@@ -179,3 +179,29 @@ def test_small_weights_of_an_integer_prefix_add_up(away, bits, rows, Hq):
     N.raise_on_device_error()
     want, bound = O.decode(q[:1, :1], kc, vc, table[:1], n[:1], 0.125, ks=ks, vs=vs, expanded=[1 << 20])
     O.check(got, want.expand(rows, Hq, -1), bound.expand(rows, Hq, -1))
+
+
+@pytest.mark.parametrize("case", [([9, 5], [1500, 700], 1, [10 + i for i in range(15)], 32, 4, 128, 16, 8, 50.0, False),
+                                  ([9, 5], [1500, 700], 0, [10 + i for i in range(14)], 16, 2, 64, 16, 4, 0.0, True),
+                                  ([40], [4000], 0, [1 + i % 9 for i in range(40)], 8, 1, 128, 16, 8, 0.0, False),
+                                  ([6], [300], 0, [9] * 6, 16, 4, 64, 16, 8, 30.0, True)])
+def test_integer_prefixes_against_the_values_of_the_pages(case):
+    """The definition itself, without the prefix's rounding to FP16 in the oracle.  That rounding moves each key's and value's
+    channel by 2^-11 of it (scales here are within 2^10 of the largest, so none is under FP16's normal numbers by more than
+    their own last bit): a score by 2^-11 sum |q k| scale, a weight by twice that, a value's share by 2^-11 of it."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(case)
+    want, bound = O.decode(q, kc, vc, table, n, scale, cap, sl, ks=ks, vs=vs)
+    for b, length in enumerate(n.tolist()):
+        pages = table[b, :-(-length // kc.shape[1])].long()
+        k, v = (O.cached(c, s, pages, length).repeat_interleave(q.shape[1] // kc.shape[2], 1) for c, s in ((kc, ks), (vc, vs)))
+        s = torch.einsum("hd,khd->hk", q[b].double(), k) * scale
+        err = torch.einsum("hd,khd->hk", q[b].double().abs(), k.abs()).amax() * scale * 2.0 ** -11
+        if cap:
+            s = cap * torch.tanh(s / cap)
+        if sl is not None:
+            s = s - sl.double()[:, None] * (length - 1 - torch.arange(length, device=DEV))
+        mass = torch.einsum("hk,khd->hd", torch.softmax(s, -1), v.abs())
+        bound[b] += mass * (2 * err + 2.0 ** -11)
+    got = S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(cap, sl), k_scale=ks, v_scale=vs, shared=sh)
+    N.raise_on_device_error()
+    O.check(got, want, bound)
