@@ -65,3 +65,15 @@ def test_the_tile_list_of_a_launch_stays_in_31_bits(Hq, Hkv, keys):
     # (the call's own shorter test never passes what does not fit)
     for B in (1, most, most + 1, 700):
         assert B <= most or B > S.MAX_SEQS or B * Hq * (keys + 64) >= 1 << 36
+
+
+def test_rows_whose_scores_are_all_minus_infinity_are_zeros():
+    """Like rows that see nothing; a score that is no number beside them makes the row none."""
+    q, k, v = rnd(3, 2, 16), rnd(3, 1, 16, seed=1), rnd(3, 1, 16, seed=2)
+    k[:, :, 0], q[:, :, 0] = 1.0, 0.5
+    q[0, 1, 0] = q[1, 0, 0] = float("-inf")
+    got = S.prompt_attention(**prompt_args(q=q, k=k, v=v, cu_q=torch.tensor([0, 3], dtype=I32), cu_k=torch.tensor([0, 3], dtype=I32)))
+    assert not got[0, 1].any() and not got[1, 0].any() and torch.isfinite(got).all() and got[2].any()
+    k[0, 0, 3] = float("nan")
+    got = S.prompt_attention(**prompt_args(q=q, k=k, v=v, cu_q=torch.tensor([0, 3], dtype=I32), cu_k=torch.tensor([0, 3], dtype=I32)))
+    assert got.isnan().all()

@@ -152,3 +152,25 @@ def test_a_key_of_a_shared_prefix_that_is_not_a_number(bits):
     lost = torch.zeros(6, 8, dtype=torch.bool, device=DEV)
     lost[:5, 4:] = True
     check_but(got, want, bound, lost)
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("bits,length", [(16, 20), (16, 5000)])
+def test_scores_of_minus_infinity_weigh_nothing(bits, length, cap):
+    """A row of them is zeros, as on the CPU; under a cap they are the cap's lower end."""
+    q, kc, vc, _, _, table, n = make(36, [length, 70], 8, 2, 64, 16, bits)
+    pos = torch.arange(length, device=DEV)
+    kc[table[0, pos // 16].long(), pos % 16, :, 0] = 1.0
+    q[:, :, 0] = 0.5
+    plain, bound = O.decode(q, kc, vc, table, n, 0.1, cap)
+    q[0, 3, 0] = float("-inf")
+    got = S.decode_attention(q, kc, vc, table, n, 0.1, S.ScoreRules(cap))
+    N.raise_on_device_error()
+    rest = torch.ones(2, 8, dtype=torch.bool, device=DEV)
+    rest[0, 3] = False
+    O.check(got[rest], plain[rest], bound[rest])
+    if cap:
+        mean = vc[table[0, pos // 16].long(), pos % 16, 0].double().mean(0)
+        assert (got[0, 3].double() - mean).abs().max() < 2.0 ** -7 * float(vc[table[0, pos // 16].long(), pos % 16, 0].double().abs().mean(0).max())
+    else:
+        assert not got[0, 3].any()

@@ -4,7 +4,8 @@ A row at position p of its sequence (the last row stands at the last key) sees k
 
     s = scale q . k_j        s = cap tanh(s / cap)        s -= slope_h |p - j|
 
-where ``ScoreRules`` says so, and out_h = softmax(s) V over the keys that are visible to it, zeros where none is.
+where ``ScoreRules`` says so, and out_h = softmax(s) V over the keys that are visible to it, zeros where none is, or where
+all of their scores are -inf.
 
 * ``prompt_attention``: packed sequences of rows against packed keys (``attention.varlen_attention`` with rules); a
   mask by documents, by a prefix that every row sees, by a window.  On a GPU ``csrc/scored_flash_tc05.cu``.
@@ -261,8 +262,10 @@ def _softmax(s, rules, distance, see):
     if rules.slopes is not None:
         s = s - rules.slopes.view(s.shape[0], s.shape[1], 1, 1) * distance.float()
     s = s.masked_fill(~see, float("-inf"))
+    if not s.numel():
+        return s
     w = torch.softmax(s, -1)
-    return torch.where(see.any(-1, keepdim=True), w, torch.zeros_like(w))
+    return torch.where(s.amax(-1, keepdim=True) == float("-inf"), torch.zeros_like(w), w)
 
 
 # ------------------------------------------------------------- single rows --
