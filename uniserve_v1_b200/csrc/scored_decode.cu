@@ -130,8 +130,8 @@ __device__ __forceinline__ int group_of(const int* cu_rows, int groups, int b, i
     const int mid = (g + h + 1) >> 1;
     if (cu_rows[mid] <= b) g = mid; else h = mid - 1;
   }
-  const int first = cu_rows[g];
-  if (b < first || b >= cu_rows[g + 1]) return -1;
+  const int first = cu_rows[g], end = cu_rows[g + 1];
+  if (b < first || b >= end) return -1;
   if (first >= 0 && b - first < most_rows) return g;
   us_dev_fail(status, US_DEV_BOUNDS);
   return -1;
@@ -448,7 +448,6 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
         m[nt][e] = -INFINITY;
         l[nt][e] = 0.f;
         bias[nt][e] = a.slopes && h < share ? a.slopes[hk * share + h] * 1.4426950408889634f : 0.f;
-        if (bias[nt][e] < 0.f) us_dev_fail(a.status, US_DEV_BOUNDS);
         factor[nt][e] = (a.cap_log2 > 0.f ? a.scale_cap : a.scale_log2) * (FMT == 16 ? 1.f : __shfl_sync(0xffffffffu, back, (c4 * 2 + e) * 4));
       }
 #pragma unroll
@@ -456,6 +455,9 @@ __global__ void __launch_bounds__((Shape<D, FMT, NT>::kWarps * 32), 1) scored_de
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
     }
+    float least = fminf(bias[0][0], bias[0][1]);
+    if constexpr (NT == 2) least = fminf(least, fminf(bias[1][0], bias[1][1]));
+    if (least < 0.f) us_dev_fail(a.status, US_DEV_BOUNDS);
   };
 
   // a key's scales out of a stage: two, or (64 channels) the one whose half its parity says, the page size being even

@@ -162,6 +162,7 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     per = kBM >> a.pack;
     // under a causal mask the last rows walk the most blocks: those of all heads and sequences start first
     q0 = (a.causal ? (int)gridDim.z - 1 - (int)blockIdx.z : (int)blockIdx.z) * 2 * per;
+    const int rows_from = a.cu_q[0], rows_to = a.cu_q[a.n];      // (of all sequences; fetched beside the others)
     q_start = a.cu_q[seq];
     q_len = min(a.cu_q[seq + 1], a.Tq) - q_start;
     k_start = a.cu_k[seq];
@@ -179,8 +180,8 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       q_len = min(q_len, a.max_q);
     }
     if (short_of && tid == 0) us_dev_fail(a.status, US_DEV_BOUNDS);
-    if (a.fill && warp == kThreads / 32 - 1) {      // a warp that has nothing else to do
-      const int before = max(0, min(a.cu_q[0], a.Tq)), end = max(before, min(a.cu_q[a.n], a.Tq));
+    if (a.fill && warp == kThreads / 32 - 1) {      // a warp that has nothing else to do; a share of those rows a CTA
+      const int before = max(0, min(rows_from, a.Tq)), end = max(before, min(rows_to, a.Tq));
       const long long ctas = (long long)gridDim.x * gridDim.y * gridDim.z;
       for (long long i = blockIdx.x + (long long)gridDim.x * (blockIdx.y + (long long)gridDim.y * blockIdx.z); i < before + a.Tq - end; i += ctas) {
         uint4* row = reinterpret_cast<uint4*>(a.out + (i < before ? i : end + i - before) * a.ldo);
@@ -432,18 +433,18 @@ scored_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       Blocks walk(bits, words);
       bool a0 = false, b0 = false, a1 = false, b1 = false;
       int j = walk.next(a0, b0), na = 0, nbb = 0;
-      int v_end = kv_len;                // values from here on nobody sees
-      if constexpr (MODE == 1) {         // a prefix may be longer than the rows that share it
-        int most = 0;
-        for (int r = q0 + lane; r < min(q0 + 2 * per, q_len); r += 32) most = max(most, a.lens[q_start + r]);
-        v_end = min(kv_len, __reduce_max_sync(0xffffffffu, most));
-      }
       bool ok = warp_wait(q_full, 0);
       if (ok) {
         tc::tc_fence_after_sync();
         if (a0) issue_qk(0, 0);
         if (b0) issue_qk(1, 0);
         umma_commit_elect(&kv_empty[1]);
+      }
+      int v_end = kv_len;                // values from here on nobody sees
+      if constexpr (MODE == 1) {         // a prefix may be longer than the rows that share it
+        int most = 0;
+        for (int r = q0 + lane; r < min(q0 + 2 * per, q_len); r += 32) most = max(most, a.lens[q_start + r]);
+        v_end = min(kv_len, __reduce_max_sync(0xffffffffu, most));
       }
       for (int e = 0; ok && j >= 0; ++e) {
         a1 = b1 = false;
@@ -849,8 +850,8 @@ __global__ void __launch_bounds__(256) join_parts_kernel(const ScoredArgs a) {
   const long long rows = (long long)a.n * a.max_q * a.Hq, i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (i >= rows) return;
   const int head = (int)(i % a.Hq), row = (int)(i / a.Hq % a.max_q), seq = (int)(i / a.Hq / a.max_q);
-  const int start = a.cu_q[seq];
-  if (start < 0 || a.cu_k[seq] < 0 || row >= min(a.cu_q[seq + 1], a.Tq) - start) return;      // (such parts were not written)
+  const int start = a.cu_q[seq], end = a.cu_q[seq + 1], keys = a.cu_k[seq];
+  if (min(start, keys) < 0 || row >= min(end, a.Tq) - start) return;      // such parts were not written
   float M = -INFINITY, L = 0.f, acc[kC] = {};
   for (int p0 = 0; p0 < a.parts; p0 += 4) {            // four parts' loads in flight
     float2 ml[4];
