@@ -1,4 +1,6 @@
 """Plans of shared prefixes and slopes on the CPU: what is refused, and rows that share nothing."""
+import random
+
 import pytest
 import torch
 
@@ -77,3 +79,16 @@ def test_rows_whose_scores_are_all_minus_infinity_are_zeros():
     k[0, 0, 3] = float("nan")
     got = S.prompt_attention(**prompt_args(q=q, k=k, v=v, cu_q=torch.tensor([0, 3], dtype=I32), cu_k=torch.tensor([0, 3], dtype=I32)))
     assert got.isnan().all()
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_a_workspace_has_room_for_every_plan_of_up_to_its_sizes(seed):
+    r = random.Random(seed)
+    for _ in range(400):
+        Hkv = r.choice([1, 2, 4, 8])
+        Hq, groups, rows, longest = Hkv * r.choice([1, 3, 8, 16, 64, 128]), r.randint(1, 9), r.randint(1, 700), r.choice([1, 500, 9000, 70_000, 1 << 21])
+        room = S._prefix_room(S.SharedPrefix(None, torch.zeros(groups), rows, longest), Hq, Hkv, 148)
+        for _ in range(5):
+            small = S.SharedPrefix(None, torch.zeros(r.randint(1, groups)), r.randint(1, rows), r.randint(1, longest))
+            pairs, parts, each = S._prefix_plan(small, Hq, Hkv, 148)
+            assert small.groups * pairs * Hkv * parts * 256 <= room and parts * each * 128 >= small.max_len and each <= 512

@@ -303,6 +303,14 @@ def _prefix_plan(shared: SharedPrefix, Hq, Hkv, sms):
     return pairs, -(-blocks // each), each
 
 
+def _prefix_room(shared: SharedPrefix, Hq, Hkv, sms):
+    """Rows of parts that a workspace for prefixes of up to these sizes holds: fewer or shorter groups of fewer rows may be cut
+    into more parts, as many as fill the GPU."""
+    pairs = _prefix_plan(shared, Hq, Hkv, sms)[0]
+    blocks = max(1, -(-shared.max_len // _TILE))
+    return max(sms, shared.groups * pairs * Hkv * -(-blocks // _LONGEST)) * 2 * _TILE
+
+
 _sms: dict = {}
 
 
@@ -320,8 +328,7 @@ def decode_work(B, Hq, Hkv, D, device, shared: Optional[SharedPrefix] = None) ->
         w = DecodeWork(torch.empty(bytes_ // 4, dtype=F32, device=device),
                        torch.zeros(min(B, MAX_SEQS) * Hkv * _chunks(Hq, Hkv), dtype=I32, device=device), D)
         if shared is not None and shared.groups:
-            pairs, parts, _ = _prefix_plan(shared, Hq, Hkv, _sm_count(device.index if device.index is not None else current_device()))
-            rows = shared.groups * pairs * Hkv * parts * 2 * _TILE
+            rows = _prefix_room(shared, Hq, Hkv, _sm_count(device.index if device.index is not None else current_device()))
             w.prefix_o = torch.empty(rows * D, dtype=F32, device=device)
             w.prefix_ml = torch.empty(rows * 2, dtype=F32, device=device)
             w.own_o = torch.empty(B * Hq * D, dtype=F32, device=device)
