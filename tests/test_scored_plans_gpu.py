@@ -207,11 +207,13 @@ def test_integer_prefixes_against_the_values_of_the_pages(case):
     O.check(got, want, bound)
 
 
-def test_a_workspace_serves_smaller_plans():
-    """One for three prefixes of up to 19,000 keys; steps with two, with one that is told to be as long, with shorter ones."""
+@pytest.mark.parametrize("told", [19_000, 148 * 128])
+def test_a_workspace_serves_smaller_plans(told):
+    """One for three prefixes of up to `told` keys (three are cut into 22 parts of 148 blocks, one into 74); steps with two, with
+    one that is told to be as long, with shorter ones."""
     q, kc, vc, _, _, table, n, sh, _, sl, scale = shared_batch(([6, 2], [2000, 700], 0, [9, 1, 0, 70, 40, 5, 6, 8], 8, 2, 64, 16, 16, 0.0, False))
-    work = S.decode_work(8, 8, 2, 64, DEV, S.SharedPrefix(None, torch.zeros(3), 8, 19_000))
+    work = S.decode_work(8, 8, 2, 64, DEV, S.SharedPrefix(None, torch.zeros(3), 8, told))
     want, bound = O.decode(q, kc, vc, table, n, scale)
-    for plan in (sh, S.SharedPrefix(sh.cu_rows[:2], sh.lens[:1], 6, 19_000), S.SharedPrefix(sh.cu_rows[:2], sh.lens[:1], 6, 2000), S.SharedPrefix(sh.cu_rows[1:], sh.lens[1:], 2, 700)):
+    for plan in (S.SharedPrefix(sh.cu_rows[:2], sh.lens[:1], 6, told), sh, S.SharedPrefix(sh.cu_rows[:2], sh.lens[:1], 6, 2000), S.SharedPrefix(sh.cu_rows[1:], sh.lens[1:], 2, 700)):
         O.check(S.decode_attention(q, kc, vc, table, n, scale, shared=plan, work=work), want, bound)
     N.raise_on_device_error()
