@@ -4,8 +4,9 @@ import torch
 
 import scored_oracle as O
 from test_scored_decode_gpu import make, slopes
-from test_scored_flash_gpu import packed
+from test_scored_flash_gpu import cu, packed
 from uniserve_v1_b200.ops import native as N
+from uniserve_v1_b200.ops import quant_pages as Q
 from uniserve_v1_b200.ops import scored as S
 
 pytestmark = pytest.mark.gpu
@@ -221,3 +222,18 @@ def test_sums_of_a_million_values_of_one_sign(rows, Hq, keys, window):
         want, bound = O.prompt(q[i:i + 1, :1], k[:end], v[:end], torch.tensor([0, 1], dtype=I32, device=DEV),
                                torch.tensor([0, end], dtype=I32, device=DEV), 0.125, window=window)
         O.check(got[i:i + 1], want.expand(1, Hq, -1), bound.expand(1, Hq, -1))
+
+
+@pytest.mark.parametrize("bits,rows", [(8, 40), (4, 40), (8, 20_000)])
+def test_reading_back_more_rows_than_told_sets_the_status(bits, rows):
+    """Those that were told of are read."""
+    planes = Q.quant_planes(rows // 8 + 2, 8, 2, 64, bits, DEV)
+    x = torch.randn(rows, 2, 64, device=DEV).to(BF16)
+    Q.kv_write_quant(x, x, torch.arange(rows, device=DEV), *planes)
+    table = torch.arange(rows // 8 + 2, device=DEV).to(I32)[None]
+    whole, _ = Q.kv_gather_quant(*planes, table, cu([rows]), rows)
+    N.raise_on_device_error()
+    got, _ = Q.kv_gather_quant(*planes, table, cu([rows]), rows - 3)
+    with pytest.raises(RuntimeError):
+        N.raise_on_device_error()
+    assert torch.equal(got, whole[:rows - 3])

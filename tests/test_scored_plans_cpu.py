@@ -4,7 +4,8 @@ import random
 import pytest
 import torch
 
-from test_scored_cpu import decode_args, prompt_args, rnd
+from test_scored_cpu import cu, decode_args, prompt_args, rnd
+from uniserve_v1_b200.ops import quant_pages as Q
 from uniserve_v1_b200.ops import scored as S
 
 I32 = torch.int32
@@ -92,3 +93,11 @@ def test_a_workspace_has_room_for_every_plan_of_up_to_its_sizes(seed):
             small = S.SharedPrefix(None, torch.zeros(r.randint(1, groups)), r.randint(1, rows), r.randint(1, longest))
             pairs, parts, each = S._prefix_plan(small, Hq, Hkv, 148)
             assert small.groups * pairs * Hkv * parts * 256 <= room and parts * each * 128 >= small.max_len and each <= 512
+
+
+@pytest.mark.parametrize("into", [None, 9])
+def test_reading_back_refuses_more_rows_than_told(into):
+    planes = Q.quant_planes(3, 4, 2, 64, 8, "cpu")
+    out = None if into is None else (rnd(into, 2, 64), rnd(into, 2, 64))
+    with pytest.raises(IndexError, match="told"):
+        Q.kv_gather_quant(*planes, torch.tensor([[0, 1]], dtype=I32), cu([6]), 5, out=out)

@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(256) quant_gather_kernel(const ReadArgs a) {
     dst[threadIdx.x] = d;
     at[threadIdx.x] = w;
   }
+  if (r0 == 0 && threadIdx.x == ROWS && a.cu[a.B] > a.total) us_dev_fail(a.status, US_DEV_BOUNDS);      // rows left out
   __syncthreads();
   const int per_row = a.heads * (a.dim >> 3), groups = a.dim >> 6;
   const int together = max(1, 256 / per_row);            // rows that the block's threads stand on
@@ -411,7 +412,7 @@ US_API int us_quant_write(const void* k, const void* v, long long ldk, long long
 
 // The first cu[s + 1] - cu[s] cached rows of every sequence as bf16 rows [total, heads, dim] (row pitch ldo), packed,
 // or from row out_cu[s] on.  Rows past cu[B] are not written; a page outside the cache is read as zeros and sets the status word, as
-// does a row outside the out_rows of the outputs, which is not written.
+// does a row past `total` or outside the out_rows of the outputs, which is not written.
 US_API int us_quant_gather(const void* kc, const void* vc, const void* ks, const void* vs, const int* table,
                            int max_pages, const int* cu, const int* out_cu, int B, int total, int pages, int page,
                            int heads, int dim, int bits, void* ko, void* vo, long long ldo, int out_rows, void* stream_) {

@@ -126,8 +126,8 @@ def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows
     cu[s + 1] - cu[s] positions through ``page_table`` [B, max_pages] to rows [cu[s], cu[s + 1]) of the result
     ([total_rows, Hkv, D] for K and for V), or to the rows from ``out_cu[s]`` on of a larger ``out``.  cu and out_cu
     are int32 on the device, total_rows is at least cu[B]; rows that no sequence brings are left as they were.  A page
-    outside the cache is read as zeros and sets the device status, as does a row past the end of ``out``, which is left
-    out (on the CPU both raise)."""
+    outside the cache is read as zeros and sets the device status, as does a row past total_rows or the end of ``out``,
+    which is left out (on the CPU all three raise)."""
     bits = page_bits(kcache, vcache, k_scale, v_scale)
     pages, page, heads, _ = kcache.shape
     dim, B = k_scale.shape[3] * GROUP, page_table.shape[0]
@@ -145,6 +145,8 @@ def kv_gather_quant(kcache, vcache, k_scale, v_scale, page_table, cu, total_rows
             raise ValueError(f"out is two bfloat16 [>= {total_rows}, {heads}, {dim}] with dense heads and one row pitch")
     if not kcache.is_cuda:
         ends, starts = cu.tolist(), (out_cu if out_cu is not None else cu).tolist()
+        if ends[-1] > total_rows:
+            raise IndexError(f"{ends[-1]} rows where {total_rows} were told")
         for s in range(B):
             pos = torch.arange(ends[s + 1] - ends[s])
             at = page_table[s, pos // page].long()
