@@ -14,9 +14,11 @@
 //
 // Writing and reading are bound by memory.  A thread has one column of 8 channels (16 bytes of bf16) in the rows of its
 // block, so what depends on the column is computed once, and loads of several rows are in flight; the rows' places are looked
-// up once a block.  (A division of 64 bits a piece made 12 us of 5 when 8168 rows of 4 heads were written; 16 channels a
-// thread, which leave sectors half written, 32 us of 25 when 41,000 were read.)  8,168 rows of 4 heads of 128 as 8 bits are
-// written in 7 us, 41,000 read in 29: 0.75 of a copy's rate.
+// up once a block.  (A division of 64 bits a piece more than doubled the time of a write; 16 channels a thread, which leave
+// sectors half written, made reading a quarter slower.)  8,168 rows of 4 heads of 128 channels are written in 7.6 us as 8 bits
+// (25.4 MB in and out, 0.52 of a copy's rate) and in 7.9 as 4 bits (21.2 MB, 0.42): two rows' loads are in flight a thread, and
+// the shuffles wait for them.  41,394 are read in 30.1 us (128.5 MB, 0.66) and in 22.4 (107.3 MB, 0.74): a block waits for its
+// places before its first load.
 #include "include/us_common.cuh"
 
 namespace {

@@ -28,8 +28,10 @@
 // sums go to the workspace.  Every wait is bounded.
 //
 // Bound by the softmax: 3,200 to 3,500 cycles a block of two tiles, 2,048 of them products.  4096 causal rows of 32 / 4 heads
-// of 128: 133 to 143 us with or without a cap (0.97 - 1.03 PFLOP/s); documents of 600 keys in 8,192 rows: 107 - 113 us, a
-// third of it starts and ends of CTAs.
+// of 128: 133 to 143 us with or without a cap (0.97 - 1.03 PFLOP/s), 148 with a cap and a bias; documents of 600 keys in 8,192
+// rows: 107 - 114 us, a third of it starts and ends of CTAs.  Caps above 55.45 have no fixed base and take the general form in
+// every block, an exponential and a reciprocal more a score: 300 us at 56 and at 100, 139 at 55.  A capped prefix of integer
+// pages takes it too (FP16 weights need a maximum).
 #include <type_traits>
 #include "include/us_common.cuh"
 #include "include/us_flash.cuh"

@@ -61,7 +61,11 @@ class SharedPrefix:
     page list of the group's first row, once for all its rows.  ``max_rows`` and ``max_len`` bound the groups' sizes
     for the host.  Rows before the first group and past the last one share nothing; rows of a group that begins before
     row 0 or has more rows than told neither, and set the device status (on the CPU the former raises).  A prefix may be longer than some of its rows, which end in it;
-    a value in it that is not finite may then reach a shorter row, as one of the row's own group sees it."""
+    a value in it that is not finite may then reach a shorter row, as one of the row's own group sees it.
+
+    On bf16 pages a shared prefix is read once.  On integer pages it is also expanded to FP16 anew in every call, which pays
+    for large groups alone: 64 rows of 32 heads behind two prefixes of 8,200 and 5,740 keys take 51 us on bf16 pages (90
+    without a plan), 97 on 8-bit ones (79 without); 96 rows of 64 heads behind one of 16,000 take 96 (328) and 209 (364)."""
     cu_rows: torch.Tensor      # int32 [groups + 1]
     lens: torch.Tensor         # int32 [groups]
     max_rows: int
