@@ -217,3 +217,55 @@ def test_a_workspace_serves_smaller_plans(told):
     for plan in (S.SharedPrefix(sh.cu_rows[:2], sh.lens[:1], 6, told), sh, S.SharedPrefix(sh.cu_rows[:2], sh.lens[:1], 6, 2000), S.SharedPrefix(sh.cu_rows[1:], sh.lens[1:], 2, 700)):
         O.check(S.decode_attention(q, kc, vc, table, n, scale, shared=plan, work=work), want, bound)
     N.raise_on_device_error()
+
+
+def test_shared_prefixes_on_two_streams_at_once():
+    """Each with its workspace; other launches between them."""
+    cases = [([8], [2033], 0, [61, 1, 0, 16, 17, 40, 3, 9], 32, 4, 128, 16, 16, 30.0, False),
+             ([9, 5], [1500, 700], 0, [10 + i for i in range(14)], 32, 4, 128, 16, 8, 50.0, False)]
+    both = [shared_batch(c, seed=50 + i) for i, c in enumerate(cases)]
+    works = [S.decode_work(b[0].shape[0], 32, 4, 128, DEV, b[7]) for b in both]
+
+    def call(i):
+        q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = both[i]
+        return S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(cap), k_scale=ks, v_scale=vs, shared=sh, work=works[i])
+    alone = [call(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in both]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    N.raise_on_device_error()
+    for i in range(2):
+        assert all(torch.equal(g, alone[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_integer_prefixes_in_a_captured_graph(bits):
+    """Replayed with other queries, lengths and a shorter prefix: what was expanded before does not stay."""
+    q, kc, vc, ks, vs, table, n, sh, cap, sl, scale = shared_batch(([6], [900], 1, [61, 1, 0, 16, 17, 40, 300], 8, 2, 64, 16, bits, 30.0, False))
+    work = S.decode_work(7, 8, 2, 64, DEV, sh)
+    out = torch.empty_like(q)
+
+    def call():
+        S.decode_attention(q, kc, vc, table, n, scale, S.ScoreRules(cap), k_scale=ks, v_scale=vs, shared=sh, work=work, out=out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for length, less in ((900, 0), (512, 300), (0, 0), (899, 1)):
+        q.mul_(-0.75)
+        sh.lens.fill_(length)
+        n.sub_(less).clamp_(min=0)
+        out.fill_(9.0)
+        graph.replay()
+        N.raise_on_device_error()
+        O.check(out, *O.decode(q, kc, vc, table, n, scale, cap, ks=ks, vs=vs, expanded=[length] * 6 + [0]))
